@@ -46,6 +46,15 @@ class RoundStats(C.Structure):
         return {k: int(getattr(self, k)) for k, _ in self._fields_}
 
 
+class Mx4LinearArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("out_features", C.c_int64),
+                ("x", C.c_void_p), ("x_row_stride", C.c_int64), ("x_col_stride", C.c_int64),
+                ("x_codes", C.c_void_p), ("x_scales", C.c_void_p),
+                ("w_codes", C.c_void_p), ("w_scales", C.c_void_p),
+                ("bias", C.c_void_p), ("y", C.c_void_p), ("y_row_stride", C.c_int64),
+                ("x_type", C.c_int32), ("bias_type", C.c_int32), ("y_type", C.c_int32), ("relu", C.c_int32)]
+
+
 TRAJECTORY_BYTES = 32 + 42 * 32
 PLY_BYTES = 32
 
@@ -74,6 +83,10 @@ SIGNATURES = {
     "nnb_selfplay_stream": (C.c_int, [_P, _P, C.POINTER(SearchParams), C.c_int32, C.c_int32, C.c_int32, _P, _P,
                                       C.c_int32, _P, _P, C.c_int32, C.POINTER(RoundStats)]),
     "nnb_trajectory_samples": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, _P]),
+    "nnb_mx4_quantize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, _P]),
+    "nnb_mx4_dequantize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, _P, _P]),
+    "nnb_mx4_linear_workspace_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_size_t)]),
+    "nnb_mx4_linear": (C.c_int, [_P, C.POINTER(Mx4LinearArgs), _P, C.c_size_t]),
     "nnb_profile_enable": (C.c_int, [_P, C.c_int]),
     "nnb_profile_reset": (C.c_int, [_P]),
     "nnb_profile_get": (C.c_int, [_P, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_int64)]),

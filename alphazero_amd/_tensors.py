@@ -1,0 +1,36 @@
+"""What the operators that take torch tensors need to hand them to libnnb.so."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import NnbError
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # nnb_dtype
+
+
+def dtype_code(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in DTYPES:
+        raise ValueError(f"{name} is {t.dtype}: expected float32, float16 or bfloat16")
+    return DTYPES[t.dtype]
+
+
+def on_device(t: torch.Tensor):
+    """Makes the tensor's GPU current, which the library launches on."""
+    if t.device.type != "cuda":
+        raise NnbError(f"a tensor on {t.device}: the kernels run on an MI355X only (there is no CPU path)")
+    return torch.cuda.device(t.device)
+
+
+def stream_of(t: torch.Tensor) -> C.c_void_p:
+    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def ptr(t: torch.Tensor) -> C.c_void_p:
+    return C.c_void_p(t.data_ptr())
+
+
+def no_grad(what: str, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NnbError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")

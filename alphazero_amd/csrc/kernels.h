@@ -155,4 +155,22 @@ void launch_net_stage_split(hipStream_t st, int stage, const NetWeights &w, cons
                             const int32_t *count_ptr, int n_max);
 void launch_split_to_f32(hipStream_t st, const void *act, const float *inv_scale, int cells, int n, float *out);
 
+// mx4_kernels.hip: 4-bit floats with a power-of-two scale per 32, rows padded to whole k-steps of the matrix unit
+constexpr int kMx4Pad = 128;
+constexpr int mx4_padded(int cols) { return (cols + kMx4Pad - 1) / kMx4Pad * kMx4Pad; }
+struct Mx4Linear {                      // y [rows][n] = x * w^T (+ bias, ReLU)
+    const uint8_t *x_codes, *x_scales;  // [rows][kp/2], [rows][kp/32]
+    const uint8_t *w_codes, *w_scales;  // [n][kp/2], [n][kp/32]
+    const void *bias;                   // [n] or null
+    void *y;
+    const int32_t *row_count;           // live rows, read on the device, or null
+    long long rows, y_stride;
+    int kp, n, bias_type, y_type, relu;
+};
+void launch_mx4_quantize(hipStream_t st, int type, long long rows, int cols, const void *x, long long row_stride,
+                         long long col_stride, const int32_t *row_count, uint8_t *codes, uint8_t *scales);
+void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, const uint8_t *codes, const uint8_t *scales,
+                           void *out);
+void launch_mx4_linear(hipStream_t st, const Mx4Linear &a);
+
 }  // namespace nnb

@@ -772,6 +772,41 @@ int run_free_rounds(nnb_engine *e, hipStream_t st, const nnb_search_params &para
     return NNB_OK;
 }
 
+// ---- operators that need no engine ----
+int check_dtype(int type, const char *what) {
+    if (type != NNB_F32 && type != NNB_F16 && type != NNB_BF16) return fail(NNB_ERR_ARG, "%s %d is no nnb_dtype", what, type);
+    return NNB_OK;
+}
+
+int check_mx4_shape(int64_t rows, int64_t cols) {
+    if (rows < 0 || rows > 0x7fffffffLL) return fail(NNB_ERR_ARG, "%lld rows out of range [0, 2^31)", (long long)rows);
+    if (cols < 1 || cols > (1 << 24)) return fail(NNB_ERR_ARG, "%lld columns out of range [1, 2^24]", (long long)cols);
+    return NNB_OK;
+}
+
+int check_mx4_pointers(const uint8_t *codes, const uint8_t *scales) {
+    if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(scales) % 4)
+        return fail(NNB_ERR_ARG, "codes must be 16-byte, scales 4-byte aligned");
+    return NNB_OK;
+}
+
+int check_workspace(const void *workspace, size_t bytes, size_t need) {
+    if (need == 0) return NNB_OK;
+    if (!workspace || bytes < need)
+        return fail(NNB_ERR_WORKSPACE, "workspace has %zu bytes, %zu needed", workspace ? bytes : (size_t)0, need);
+    if (reinterpret_cast<uintptr_t>(workspace) % kAlign)
+        return fail(NNB_ERR_WORKSPACE, "workspace must be %zu-byte aligned", kAlign);
+    return NNB_OK;
+}
+
+// Workspace of nnb_mx4_linear: the quantised rows.
+void carve_mx4_rows(Carver &c, int64_t rows, int cols, bool x_quantized, uint8_t *&codes, uint8_t *&scales) {
+    codes = scales = nullptr;
+    if (x_quantized) return;
+    codes = c.take<uint8_t>((size_t)rows * (mx4_padded(cols) / 2));
+    scales = c.take<uint8_t>((size_t)rows * (mx4_padded(cols) / 32));
+}
+
 }  // namespace
 
 extern "C" {
@@ -1236,6 +1271,80 @@ int nnb_search_static(void *stream, const nnb_search_params *p, int32_t n, const
     launch_tree_init(st, d, sd, make_noise, 0);
     launch_tree_fused(st, d, sd, plan);
     launch_readout(st, d, sd, visits_out, action_out, root_value_out, nullptr);
+    HIP_TRY(hipGetLastError());
+    return NNB_OK;
+}
+
+int nnb_mx4_quantize(void *stream, int x_type, int64_t rows, int64_t cols, const void *x, int64_t row_stride,
+                     int64_t col_stride, uint8_t *codes_out, uint8_t *scales_out) {
+    if (int rc = check_dtype(x_type, "x_type")) return rc;
+    if (int rc = check_mx4_shape(rows, cols)) return rc;
+    if (rows == 0) return NNB_OK;
+    if (!x || !codes_out || !scales_out) return fail(NNB_ERR_ARG, "null pointer");
+    if (int rc = check_mx4_pointers(codes_out, scales_out)) return rc;
+    launch_mx4_quantize(static_cast<hipStream_t>(stream), x_type, rows, (int)cols, x, row_stride, col_stride, nullptr,
+                        codes_out, scales_out);
+    HIP_TRY(hipGetLastError());
+    return NNB_OK;
+}
+
+int nnb_mx4_dequantize(void *stream, int out_type, int64_t rows, int64_t cols, const uint8_t *codes,
+                       const uint8_t *scales, void *out) {
+    if (int rc = check_dtype(out_type, "out_type")) return rc;
+    if (int rc = check_mx4_shape(rows, cols)) return rc;
+    if (rows == 0) return NNB_OK;
+    if (!codes || !scales || !out) return fail(NNB_ERR_ARG, "null pointer");
+    if (int rc = check_mx4_pointers(codes, scales)) return rc;
+    launch_mx4_dequantize(static_cast<hipStream_t>(stream), out_type, rows, (int)cols, codes, scales, out);
+    HIP_TRY(hipGetLastError());
+    return NNB_OK;
+}
+
+int nnb_mx4_linear_workspace_bytes(int64_t rows, int64_t cols, int64_t out_features, int x_quantized, size_t *bytes_out) {
+    if (!bytes_out) return fail(NNB_ERR_ARG, "bytes_out is null");
+    if (int rc = check_mx4_shape(rows, cols)) return rc;
+    if (int rc = check_mx4_shape(out_features, cols)) return rc;
+    Carver c(nullptr);
+    uint8_t *codes, *scales;
+    carve_mx4_rows(c, rows, (int)cols, x_quantized != 0, codes, scales);
+    *bytes_out = c.off;
+    return NNB_OK;
+}
+
+int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *p, void *workspace, size_t workspace_bytes) {
+    if (!p) return fail(NNB_ERR_ARG, "args is null");
+    const bool quantized = p->x == nullptr;
+    size_t need = 0;
+    if (int rc = nnb_mx4_linear_workspace_bytes(p->rows, p->cols, p->out_features, quantized, &need)) return rc;
+    if (!quantized)
+        if (int rc = check_dtype(p->x_type, "x_type")) return rc;
+    if (p->bias)
+        if (int rc = check_dtype(p->bias_type, "bias_type")) return rc;
+    if (int rc = check_dtype(p->y_type, "y_type")) return rc;
+    if (p->rows == 0 || p->out_features == 0) return NNB_OK;
+    if (!p->w_codes || !p->w_scales || !p->y || (quantized && (!p->x_codes || !p->x_scales)))
+        return fail(NNB_ERR_ARG, "null pointer");
+    if (int rc = check_mx4_pointers(p->w_codes, p->w_scales)) return rc;
+    if (quantized)
+        if (int rc = check_mx4_pointers(p->x_codes, p->x_scales)) return rc;
+    if (p->y_row_stride < p->out_features)
+        return fail(NNB_ERR_ARG, "y_row_stride %lld is smaller than a row of %lld", (long long)p->y_row_stride,
+                    (long long)p->out_features);
+    if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    Mx4Linear a = {};
+    a.x_codes = p->x_codes; a.x_scales = p->x_scales; a.w_codes = p->w_codes; a.w_scales = p->w_scales;
+    a.bias = p->bias; a.bias_type = p->bias_type; a.y = p->y; a.y_type = p->y_type; a.y_stride = p->y_row_stride;
+    a.rows = p->rows; a.kp = mx4_padded((int)p->cols); a.n = (int)p->out_features; a.relu = p->relu != 0;
+    if (!quantized) {
+        Carver c(workspace);
+        uint8_t *codes, *scales;
+        carve_mx4_rows(c, p->rows, (int)p->cols, false, codes, scales);
+        launch_mx4_quantize(st, p->x_type, p->rows, (int)p->cols, p->x, p->x_row_stride, p->x_col_stride, nullptr, codes,
+                            scales);
+        a.x_codes = codes; a.x_scales = scales;
+    }
+    launch_mx4_linear(st, a);
     HIP_TRY(hipGetLastError());
     return NNB_OK;
 }

@@ -379,6 +379,47 @@ int nnb_dirichlet_noise(void *stream, int32_t n, uint64_t seed, const int32_t *g
                         const int32_t *move_indices, const uint8_t *legal_masks, double alpha,
                         float *noise_out);
 
+/* ---- operators on weight matrices and activations -------------------------- */
+/* They need no engine: the arrays, and a workspace where one is named, are device memory of the caller on the
+ * current device; work is enqueued on `stream`, nothing is allocated or waited for, so every call can be captured into
+ * a graph.  A workspace (256-byte aligned) is scratch of one call: calls that may overlap in time need one each.
+ * No counterparts in the reference (it trains with stock layers and optimisers, lightning_module.py:20-31). */
+enum nnb_dtype { NNB_F32 = 0, NNB_F16 = 1, NNB_BF16 = 2 };
+
+/* 4-bit floats with shared scales.  A row of `cols` numbers is cut into blocks of 32; a block shares the scale 2^e,
+ * e = floor(log2 max|x|) - 2 clamped to [-127, 127] and stored as the byte e + 127; an element is the e2m1 code of
+ * x / 2^e (values 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), to nearest with ties to the even code and beyond 6
+ * to 6.  A block that holds an infinity or a NaN gets the byte 255 and reads as NaN.  Rows are padded with zeros to
+ * Kp = the next multiple of 128: codes_out [rows][Kp/2], 16-byte aligned, element 2i in the low half of byte i;
+ * scales_out [rows][Kp/32], 4-byte aligned.
+ * x [rows][cols] of type x_type (nnb_dtype), element (r, c) at x[r*row_stride + c*col_stride] (strides in elements, may
+ * be 0 or negative).  rows = 0 is a no-op; cols in [1, 2^24], rows at most 2^31 - 1. */
+int nnb_mx4_quantize(void *stream, int x_type, int64_t rows, int64_t cols, const void *x, int64_t row_stride,
+                     int64_t col_stride, uint8_t *codes_out, uint8_t *scales_out);
+/* The values codes and scales stand for, out [rows][cols] (contiguous) of type out_type, rounded once. */
+int nnb_mx4_dequantize(void *stream, int out_type, int64_t rows, int64_t cols, const uint8_t *codes,
+                       const uint8_t *scales, void *out);
+
+/* y = x w^T (+ bias) (then ReLU): a linear layer on 4-bit weights.  x is given either as numbers (x, x_type, strides: it
+ * is quantised as nnb_mx4_quantize does, into the workspace) or already quantised (x = NULL, x_codes / x_scales);
+ * products of codes and scales are exact, sums, bias and ReLU in float32, one rounding to y_type at the end.
+ * y [rows][out_features], row r at y + r*y_row_stride, must not overlap the inputs. */
+typedef struct nnb_mx4_linear_args {
+    int64_t rows, cols, out_features;
+    const void *x;
+    int64_t x_row_stride, x_col_stride;
+    const uint8_t *x_codes, *x_scales;
+    const uint8_t *w_codes, *w_scales;   /* the weights [out_features][cols], quantised              */
+    const void *bias;                    /* [out_features] of type bias_type, or NULL                */
+    void *y;
+    int64_t y_row_stride;
+    int32_t x_type, bias_type, y_type;   /* nnb_dtype                                                */
+    int32_t relu;
+} nnb_mx4_linear_args;
+/* Bytes of workspace nnb_mx4_linear needs (0 is possible). */
+int nnb_mx4_linear_workspace_bytes(int64_t rows, int64_t cols, int64_t out_features, int x_quantized, size_t *bytes_out);
+int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *args, void *workspace, size_t workspace_bytes);
+
 /* Average device time, in milliseconds, of the `which`-th engine kernel class since
  * the last nnb_profile_reset, measured with HIP events on the launch stream when
  * profiling is enabled (nnb_profile_enable(engine, 1)).  Classes: 0 tree step,
