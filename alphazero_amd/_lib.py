@@ -55,6 +55,23 @@ class Mx4LinearArgs(C.Structure):
                 ("x_type", C.c_int32), ("bias_type", C.c_int32), ("y_type", C.c_int32), ("relu", C.c_int32)]
 
 
+NS_MAX_STEPS = 16
+
+
+class NewtonSchulz(C.Structure):
+    _fields_ = [("steps", C.c_int32), ("coefficients", (C.c_float * 3) * NS_MAX_STEPS), ("eps", C.c_double)]
+
+
+class MuonMatrix(C.Structure):
+    _fields_ = [("weight", C.c_void_p), ("grad", C.c_void_p), ("momentum", C.c_void_p), ("weight_out", C.c_void_p),
+                ("momentum_out", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64)]
+
+
+class MuonParams(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("nesterov", C.c_int32),
+                ("ns", NewtonSchulz)]
+
+
 TRAJECTORY_BYTES = 32 + 42 * 32
 PLY_BYTES = 32
 
@@ -87,6 +104,11 @@ SIGNATURES = {
     "nnb_mx4_dequantize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, _P, _P]),
     "nnb_mx4_linear_workspace_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_size_t)]),
     "nnb_mx4_linear": (C.c_int, [_P, C.POINTER(Mx4LinearArgs), _P, C.c_size_t]),
+    "nnb_orthogonalize_workspace_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
+    "nnb_orthogonalize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_int64, _P, C.POINTER(C.c_int64), _P,
+                                    C.POINTER(C.c_int64), C.POINTER(NewtonSchulz), _P, C.c_size_t]),
+    "nnb_muon_workspace_bytes": (C.c_int, [C.c_int32, C.POINTER(MuonMatrix), C.POINTER(C.c_size_t)]),
+    "nnb_muon_step": (C.c_int, [_P, C.c_int, C.c_int32, C.POINTER(MuonMatrix), C.POINTER(MuonParams), _P, C.c_size_t]),
     "nnb_profile_enable": (C.c_int, [_P, C.c_int]),
     "nnb_profile_reset": (C.c_int, [_P]),
     "nnb_profile_get": (C.c_int, [_P, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_int64)]),

@@ -17,6 +17,7 @@ SOURCES = [
     ("net_kernels_f16.hip", []),
     ("net_kernels_split.hip", []),
     ("mx4_kernels.hip", []),
+    ("ortho_kernels.hip", []),
     ("nnb_api.hip", []),
 ]
 # Packed float32 instructions are kept out of all kernels: some of their forms have been seen to give wrong results.

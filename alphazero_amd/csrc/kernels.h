@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include "engine_layout.h"
 #include "heads_math.h"
+#include "ortho_layout.h"
 
 namespace nnb {
 
@@ -172,5 +173,10 @@ void launch_mx4_quantize(hipStream_t st, int type, long long rows, int cols, con
 void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, const uint8_t *codes, const uint8_t *scales,
                            void *out);
 void launch_mx4_linear(hipStream_t st, const Mx4Linear &a);
+
+// ortho_kernels.hip: Newton-Schulz orthogonalisation and the optimiser step on it.  The group's workspace holds an area
+// per matrix (OrthoItem::ws); `first` is scratch of the launches.
+bool ortho_coefficients_ok(const OrthoParams &p);
+void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p);
 
 }  // namespace nnb

@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <new>
 #include <vector>
 
@@ -16,6 +17,7 @@
 #include "c4_bits.h"
 #include "engine_layout.h"
 #include "kernels.h"
+#include "numeric_types.h"
 
 using namespace nnb;
 
@@ -807,6 +809,67 @@ void carve_mx4_rows(Carver &c, int64_t rows, int cols, bool x_quantized, uint8_t
     scales = c.take<uint8_t>((size_t)rows * (mx4_padded(cols) / 32));
 }
 
+// Limits of the orthogonalisation kernels' indices.
+int check_matrix(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 0) return fail(NNB_ERR_ARG, "matrix of %lld x %lld", (long long)rows, (long long)cols);
+    const int64_t shorter = rows < cols ? rows : cols, longer = rows < cols ? cols : rows;
+    if (longer > 0x7fffffffLL || rows * cols > 0x7fffffffLL || shorter > 16384)
+        return fail(NNB_ERR_ARG, "matrix of %lld x %lld: more than 2^31 - 1 elements or a shorter side over 16384",
+                    (long long)rows, (long long)cols);
+    return NNB_OK;
+}
+
+int to_ortho_params(const nnb_newton_schulz *ns, OrthoParams &p) {
+    if (!ns) return fail(NNB_ERR_ARG, "Newton-Schulz parameters are null");
+    if (ns->steps < 1 || ns->steps > NNB_NS_MAX_STEPS)
+        return fail(NNB_ERR_ARG, "%d steps out of range [1, %d]", ns->steps, NNB_NS_MAX_STEPS);
+    if (!(ns->eps >= 0.0) || !std::isfinite(ns->eps)) return fail(NNB_ERR_ARG, "eps must be finite and >= 0");
+    static_assert(NNB_NS_MAX_STEPS == kOrthoMaxSteps, "steps the kernels take");
+    p.steps = ns->steps;
+    p.eps = ns->eps;
+    for (int i = 0; i < ns->steps; ++i)
+        for (int j = 0; j < 3; ++j) {
+            p.coef[i][j] = ns->coefficients[i][j];
+            if (!std::isfinite(p.coef[i][j])) return fail(NNB_ERR_ARG, "coefficient %d of step %d is not finite", j, i);
+        }
+    if (!ortho_coefficients_ok(p)) return fail(NNB_ERR_ARG, "these coefficients let the singular values grow without bound");
+    return NNB_OK;
+}
+
+// Calls emit(group) for groups of at most kOrthoItems items whose areas take kOrthoGroupBytes (or one matrix's, if that
+// is more); a large batch is cut.  Returns the bytes of the largest group.
+constexpr size_t kOrthoGroupBytes = (size_t)1 << 30;
+template <typename F> size_t ortho_groups(const OrthoItem *items, size_t count, F &&emit) {
+    OrthoGroup g = {};
+    size_t used = 0, most = 0;
+    auto flush = [&] {
+        if (g.count) emit(g);
+        most = used > most ? used : most;
+        g.count = 0;
+        used = 0;
+    };
+    for (size_t i = 0; i < count; ++i) {
+        const size_t each = ortho_area(items[i].rows, items[i].cols).bytes;
+        for (int done = 0; done < items[i].batch;) {
+            if (g.count == kOrthoItems || (g.count && used + each > kOrthoGroupBytes)) flush();
+            const size_t room = (kOrthoGroupBytes - (used < kOrthoGroupBytes ? used : kOrthoGroupBytes)) / each;
+            OrthoItem &it = g.item[g.count++];
+            it = items[i];
+            const size_t left = (size_t)(items[i].batch - done);
+            it.batch = (int)(room < 1 ? 1 : room < left ? room : left);
+            const size_t size = dtype_bytes(it.type);
+            if (it.x) it.x = static_cast<const char *>(it.x) + done * it.x_bs * (long long)size;
+            if (it.out) it.out = static_cast<char *>(it.out) + done * it.o_bs * (long long)size;
+            it.ws = used;
+            it.ws_stride = each;
+            used += it.batch * each;
+            done += it.batch;
+        }
+    }
+    flush();
+    return most;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1345,6 +1408,107 @@ int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *p, void *workspace, 
         a.x_codes = codes; a.x_scales = scales;
     }
     launch_mx4_linear(st, a);
+    HIP_TRY(hipGetLastError());
+    return NNB_OK;
+}
+
+int nnb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, size_t *bytes_out) {
+    if (!bytes_out) return fail(NNB_ERR_ARG, "bytes_out is null");
+    if (batch < 0 || batch > 0x7fffffffLL) return fail(NNB_ERR_ARG, "batch %lld out of range [0, 2^31)", (long long)batch);
+    if (int rc = check_matrix(rows, cols)) return rc;
+    *bytes_out = 0;
+    if (batch == 0 || rows == 0 || cols == 0) return NNB_OK;
+    OrthoItem it = {};
+    it.rows = (int)rows; it.cols = (int)cols; it.batch = (int)batch;
+    *bytes_out = ortho_groups(&it, 1, [](OrthoGroup &) {});
+    return NNB_OK;
+}
+
+int nnb_orthogonalize(void *stream, int type, int64_t batch, int64_t rows, int64_t cols, const void *x,
+                      const int64_t x_strides[3], void *out, const int64_t out_strides[3], const nnb_newton_schulz *ns,
+                      void *workspace, size_t workspace_bytes) {
+    if (int rc = check_dtype(type, "type")) return rc;
+    size_t need = 0;
+    if (int rc = nnb_orthogonalize_workspace_bytes(batch, rows, cols, &need)) return rc;
+    OrthoParams p = {};
+    if (int rc = to_ortho_params(ns, p)) return rc;
+    if (need == 0) return NNB_OK;
+    if (!x || !out || !x_strides || !out_strides) return fail(NNB_ERR_ARG, "null pointer");
+    if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
+    p.type = type;
+    OrthoItem it = {};
+    it.x = x; it.out = out; it.type = type;
+    it.x_bs = x_strides[0]; it.x_rs = x_strides[1]; it.x_cs = x_strides[2];
+    it.o_bs = out_strides[0]; it.o_rs = out_strides[1]; it.o_cs = out_strides[2];
+    it.rows = (int)rows; it.cols = (int)cols; it.batch = (int)batch;
+    ortho_groups(&it, 1, [&](OrthoGroup &g) {
+        g.ws = static_cast<unsigned char *>(workspace);
+        launch_orthogonalize(static_cast<hipStream_t>(stream), g, p);
+    });
+    HIP_TRY(hipGetLastError());
+    return NNB_OK;
+}
+
+// The matrices of an optimiser step that have elements, as items; a negative result is an error.
+static int muon_items(int type, int32_t count, const nnb_muon_matrix *matrices, const nnb_muon_params *params,
+                      OrthoItem *items) {
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+        const nnb_muon_matrix &m = matrices[i];
+        if (int rc = check_matrix(m.rows, m.cols)) return rc;
+        if (m.rows == 0 || m.cols == 0) continue;
+        OrthoItem it = {};
+        it.type = type;
+        it.rows = (int)m.rows; it.cols = (int)m.cols; it.batch = 1;
+        if (params) {
+            if (!m.weight || !m.grad || !m.momentum || !m.weight_out || !m.momentum_out)
+                return fail(NNB_ERR_ARG, "matrix %d: null pointer", i);
+            it.x = m.grad; it.weight = m.weight; it.out = m.weight_out;
+            it.momentum = m.momentum; it.momentum_out = m.momentum_out;
+            it.x_rs = it.o_rs = m.cols; it.x_cs = it.o_cs = 1;
+            it.scale = (float)((double)params->lr * std::sqrt(m.rows > m.cols ? (double)m.rows / (double)m.cols : 1.0));
+        }
+        items[n++] = it;
+    }
+    return n;
+}
+
+int nnb_muon_workspace_bytes(int32_t count, const nnb_muon_matrix *matrices, size_t *bytes_out) {
+    if (!bytes_out) return fail(NNB_ERR_ARG, "bytes_out is null");
+    if (count < 0 || count > (1 << 20)) return fail(NNB_ERR_ARG, "count %d out of range [0, 2^20]", count);
+    if (count && !matrices) return fail(NNB_ERR_ARG, "matrices is null");
+    std::unique_ptr<OrthoItem[]> items(new (std::nothrow) OrthoItem[count ? count : 1]);
+    if (!items) return fail(NNB_ERR_ARG, "out of host memory");
+    const int n = muon_items(NNB_F32, count, matrices, nullptr, items.get());
+    if (n < 0) return n;
+    *bytes_out = ortho_groups(items.get(), n, [](OrthoGroup &) {});
+    return NNB_OK;
+}
+
+int nnb_muon_step(void *stream, int type, int32_t count, const nnb_muon_matrix *matrices, const nnb_muon_params *params,
+                  void *workspace, size_t workspace_bytes) {
+    if (int rc = check_dtype(type, "type")) return rc;
+    if (!params) return fail(NNB_ERR_ARG, "params is null");
+    if (!std::isfinite(params->lr) || !std::isfinite(params->momentum) || !std::isfinite(params->weight_decay))
+        return fail(NNB_ERR_ARG, "lr, momentum and weight_decay must be finite");
+    OrthoParams p = {};
+    if (int rc = to_ortho_params(&params->ns, p)) return rc;
+    size_t need = 0;
+    if (int rc = nnb_muon_workspace_bytes(count, matrices, &need)) return rc;
+    std::unique_ptr<OrthoItem[]> items(new (std::nothrow) OrthoItem[count ? count : 1]);
+    if (!items) return fail(NNB_ERR_ARG, "out of host memory");
+    const int n = muon_items(type, count, matrices, params, items.get());
+    if (n <= 0) return n;
+    if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
+    p.type = type;
+    p.muon = 1;
+    p.mu = params->momentum;
+    p.nesterov = params->nesterov != 0;
+    p.decay = (float)(1.0 - (double)params->lr * (double)params->weight_decay);
+    ortho_groups(items.get(), n, [&](OrthoGroup &g) {
+        g.ws = static_cast<unsigned char *>(workspace);
+        launch_orthogonalize(static_cast<hipStream_t>(stream), g, p);
+    });
     HIP_TRY(hipGetLastError());
     return NNB_OK;
 }

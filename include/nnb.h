@@ -420,6 +420,48 @@ typedef struct nnb_mx4_linear_args {
 int nnb_mx4_linear_workspace_bytes(int64_t rows, int64_t cols, int64_t out_features, int x_quantized, size_t *bytes_out);
 int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *args, void *workspace, size_t workspace_bytes);
 
+/* Newton-Schulz orthogonalisation.  X = x / (|x|_F + eps), then `steps` times
+ *     X <- a X + b (X X^T) X + c (X X^T)^2 X      with step i's (a, b, c) = coefficients[i],
+ * which drives the singular values towards 1 and keeps the singular vectors.  Sums, the norm and the small matrices
+ * are float32-faithful (each operand 22 bits, sums in float32, the norm in double); one rounding to `type` at the end.
+ * Coefficients that let the singular values grow beyond what half-pair operands can hold are refused; any that keep
+ * them below about 10 are accepted.  A matrix with a NaN or an infinity gives NaN, a zero matrix zeros. */
+#define NNB_NS_MAX_STEPS 16
+typedef struct nnb_newton_schulz {
+    int32_t steps;                                 /* 1 .. NNB_NS_MAX_STEPS                                  */
+    float coefficients[NNB_NS_MAX_STEPS][3];
+    double eps;                                    /* >= 0; 0 makes a zero matrix NaN                         */
+} nnb_newton_schulz;
+/* x and out: `batch` matrices [rows][cols] of type `type`, element (b, r, c) at b*strides[0] + r*strides[1] +
+ * c*strides[2] (elements).  out's elements must not overlap each other or x, except out = x with equal strides.
+ * Limits: rows*cols < 2^31, the shorter side at most 16384.  batch, rows or cols = 0 is a no-op. */
+int nnb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, size_t *bytes_out);
+int nnb_orthogonalize(void *stream, int type, int64_t batch, int64_t rows, int64_t cols, const void *x,
+                      const int64_t x_strides[3], void *out, const int64_t out_strides[3], const nnb_newton_schulz *ns,
+                      void *workspace, size_t workspace_bytes);
+
+/* One step of the orthogonalised-momentum optimiser on `count` weight matrices [rows][cols], each
+ *     m' = momentum * m + g;   u = nesterov ? g + momentum * m' : m'
+ *     w' = w * (1 - lr * weight_decay) - lr * max(1, rows / cols)^(1/2) * orthogonalize(u)
+ * weight, grad and weight_out of type `type`, momentum and momentum_out float32, all contiguous; weight_out may be
+ * weight and momentum_out momentum, otherwise nothing may overlap.  `matrices` and `params` are host memory, read
+ * before the call returns (a captured call keeps their values).  A matrix with rows or cols = 0 is skipped. */
+typedef struct nnb_muon_matrix {
+    const void *weight, *grad;
+    const float *momentum;
+    void *weight_out;
+    float *momentum_out;
+    int64_t rows, cols;
+} nnb_muon_matrix;
+typedef struct nnb_muon_params {
+    float lr, momentum, weight_decay;
+    int32_t nesterov;
+    nnb_newton_schulz ns;
+} nnb_muon_params;
+int nnb_muon_workspace_bytes(int32_t count, const nnb_muon_matrix *matrices, size_t *bytes_out);
+int nnb_muon_step(void *stream, int type, int32_t count, const nnb_muon_matrix *matrices, const nnb_muon_params *params,
+                  void *workspace, size_t workspace_bytes);
+
 /* Average device time, in milliseconds, of the `which`-th engine kernel class since
  * the last nnb_profile_reset, measured with HIP events on the launch stream when
  * profiling is enabled (nnb_profile_enable(engine, 1)).  Classes: 0 tree step,

@@ -98,3 +98,99 @@ def test_mx4_python_refusals():
         mx4.linear(x.clone().requires_grad_(), w)
     with pytest.raises(NnbError, match="backward"):
         mx4.quantize(x.clone().requires_grad_())
+
+
+def test_optimiser_structs_match_the_header(tmp_path):
+    import os
+    import subprocess
+    from alphazero_amd import _lib
+    from conftest import ROOT
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include "nnb.h"\nint main(void){printf("%zu %zu %zu\\n",sizeof(nnb_newton_schulz),'
+                   "sizeof(nnb_muon_matrix),sizeof(nnb_muon_params));return 0;}\n")
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")])
+    sizes = [int(v) for v in subprocess.check_output([str(tmp_path / "s")]).split()]
+    assert sizes == [C.sizeof(_lib.NewtonSchulz), C.sizeof(_lib.MuonMatrix), C.sizeof(_lib.MuonParams)]
+
+
+def _ns(steps=5, abc=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    from alphazero_amd._lib import NewtonSchulz
+    ns = NewtonSchulz(steps=steps, eps=eps)
+    for i in range(16):
+        for j in range(3):
+            ns.coefficients[i][j] = abc[j]
+    return ns
+
+
+def test_orthogonalize_refuses_bad_arguments(lib):
+    p, s = C.c_void_p(4096), (C.c_int64 * 3)(0, 64, 1)
+    def call(t=0, batch=1, rows=32, cols=64, x=p, xs=s, out=p, os_=s, ns=None, ws=p, nbytes=1 << 30):
+        ns = _ns() if ns is None else ns
+        return lib.nnb_orthogonalize(None, t, batch, rows, cols, x, xs, out, os_, C.byref(ns), ws, nbytes)
+    for kw, word in ((dict(t=4), "dtype"), (dict(batch=-1), "batch"), (dict(rows=-1), "matrix"), (dict(rows=20000, cols=20000), "16384"),
+                     (dict(rows=1 << 16, cols=1 << 15), "16384"), (dict(cols=1 << 31), "2^31"), (dict(x=None), "null"),
+                     (dict(out=None), "null"), (dict(xs=None), "null"), (dict(os_=None), "null"), (dict(ns=_ns(steps=0)), "steps"),
+                     (dict(ns=_ns(steps=17)), "steps"), (dict(ns=_ns(eps=-1.0)), "eps"), (dict(ns=_ns(eps=float("nan"))), "eps"),
+                     (dict(ns=_ns(abc=(float("inf"), 0.0, 0.0))), "finite"), (dict(ns=_ns(abc=(30.0, 0.0, 5.0))), "grow")):
+        assert call(**kw) == -1 and word in _message(lib), kw
+    assert call(ws=None) == -4 and call(nbytes=100) == -4 and call(ws=C.c_void_p(4100)) == -4
+    assert call(batch=0, x=None) == 0 and call(rows=0) == 0 and call(cols=0) == 0
+    assert lib.nnb_orthogonalize(None, 0, 1, 4, 4, p, s, p, s, None, p, 1 << 30) == -1
+    n = C.c_size_t()
+    assert lib.nnb_orthogonalize_workspace_bytes(1, 4, 4, None) == -1
+    # a large batch is worked off in parts: its workspace stays bounded
+    assert lib.nnb_orthogonalize_workspace_bytes(1 << 20, 64, 64, C.byref(n)) == 0 and 0 < n.value <= 1 << 30
+
+
+def test_muon_step_refuses_bad_arguments(lib):
+    from alphazero_amd._lib import MuonMatrix, MuonParams
+    p = C.c_void_p(4096)
+    def call(t=0, count=1, ws=p, nbytes=1 << 30, lr=0.1, momentum=0.9, wd=0.0, ns=None, **kw):
+        items = (MuonMatrix * 2)()
+        for it in items:
+            for k, v in {**dict(weight=4096, grad=4096, momentum=4096, weight_out=4096, momentum_out=4096, rows=4, cols=8), **kw}.items():
+                setattr(it, k, v)
+        params = MuonParams(lr=lr, momentum=momentum, weight_decay=wd, nesterov=1, ns=_ns() if ns is None else ns)
+        return lib.nnb_muon_step(None, t, count, items, C.byref(params), ws, nbytes)
+    nan = float("nan")
+    for kw, word in ((dict(t=-2), "dtype"), (dict(count=-1), "count"), (dict(lr=nan), "finite"), (dict(momentum=nan), "finite"),
+                     (dict(wd=nan), "finite"), (dict(weight=None), "null"), (dict(grad=None), "null"), (dict(momentum_out=None), "null"),
+                     (dict(rows=-3), "matrix"), (dict(ns=_ns(steps=40)), "steps")):
+        assert call(**kw) == -1 and word in _message(lib), kw
+    assert call(ws=None) == -4
+    assert call(count=0, ws=None) == 0
+    assert call(rows=0, ws=None, weight=None) == 0
+    assert lib.nnb_muon_step(None, 0, 1, None, C.byref(MuonParams(ns=_ns())), p, 1) == -1
+    assert lib.nnb_muon_step(None, 0, 1, None, None, p, 1) == -1
+
+
+def test_optimiser_python_refusals():
+    import torch
+    from alphazero_amd import optim
+    from alphazero_amd._lib import NnbError
+    x = torch.randn(8, 9)
+    with pytest.raises(NnbError):                                       # no CPU path
+        optim.orthogonalize(x)
+    for bad in (x[0], x.double(), x.int()):
+        with pytest.raises(ValueError):
+            optim.orthogonalize(bad)
+    for kw in (dict(steps=0), dict(steps=17), dict(coefficients=(1.0, 2.0)), dict(coefficients=[(1, 0, 0)] * 4), dict(out=x.half()),
+               dict(out=torch.zeros(9, 8))):
+        with pytest.raises(ValueError):
+            optim.orthogonalize(x, **kw)
+    with pytest.raises(NnbError, match="backward"):
+        optim.orthogonalize(x.clone().requires_grad_())
+    w, g, m = x.clone(), x.clone(), x.clone()
+    for args in (([w], [g], []), ([w], [g[:4]], [m]), ([w], [g.half()], [m]), ([w], [g], [m.half()]), ([w.double()], [g.double()], [m]),
+                 ([w, w], [g, g], [m, m.clone()])):
+        with pytest.raises(ValueError):
+            optim.muon_update(*args, lr=0.1)
+    with pytest.raises(NnbError):
+        optim.muon_update([w], [g], [m], lr=0.1)
+    for kw in (dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1), dict(steps=0)):
+        with pytest.raises(ValueError):
+            optim.Muon([torch.nn.Parameter(x)], **kw)
+    with pytest.raises(ValueError):
+        optim.Muon([torch.nn.Parameter(x[0])])
+    with pytest.raises(ValueError):
+        optim.Muon([torch.nn.Parameter(x.t())])
