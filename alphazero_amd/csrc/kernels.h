@@ -158,21 +158,36 @@ void launch_split_to_f32(hipStream_t st, const void *act, const float *inv_scale
 
 // mx4_kernels.hip: 4-bit floats with a power-of-two scale per 32, rows padded to whole k-steps of the matrix unit
 constexpr int kMx4Pad = 128;
-constexpr int mx4_padded(int cols) { return (cols + kMx4Pad - 1) / kMx4Pad * kMx4Pad; }
+__host__ __device__ constexpr int mx4_padded(int cols) { return (cols + kMx4Pad - 1) / kMx4Pad * kMx4Pad; }
+// Scales lie in word blocks of 256 bytes: 16 rows x four k-steps of 128
+__host__ __device__ constexpr int mx4_scale_words(int kp) { return (kp + 511) / 512; }
+__host__ __device__ constexpr size_t mx4_scale_bytes(long long rows, int cols) {
+    return (size_t)((rows + 15) / 16) * mx4_scale_words(mx4_padded(cols)) * 256;
+}
+__host__ __device__ constexpr size_t mx4_scale_at(long long row, int block, int kp) {
+    return ((size_t)(row / 16) * mx4_scale_words(kp) + block / 16) * 256 + ((block % 4) * 16 + row % 16) * 4 + block / 4 % 4;
+}
 struct Mx4Linear {                      // y [rows][n] = x * w^T (+ bias, ReLU)
-    const uint8_t *x_codes, *x_scales;  // [rows][kp/2], [rows][kp/32]
-    const uint8_t *w_codes, *w_scales;  // [n][kp/2], [n][kp/32]
+    const uint8_t *x_codes, *x_scales;
+    const uint8_t *w_codes, *w_scales;
     const void *bias;                   // [n] or null
     void *y;
     const int32_t *row_count;           // live rows, read on the device, or null
     long long rows, y_stride;
-    int kp, n, bias_type, y_type, relu;
+    int kp, n, bias_type, y_type, relu, wide;
+};
+struct Mx4Rows {                        // rows that are still numbers
+    const void *x;
+    long long row_stride, col_stride;
+    int type, cols;
 };
 void launch_mx4_quantize(hipStream_t st, int type, long long rows, int cols, const void *x, long long row_stride,
                          long long col_stride, const int32_t *row_count, uint8_t *codes, uint8_t *scales);
 void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, const uint8_t *codes, const uint8_t *scales,
                            void *out);
-void launch_mx4_linear(hipStream_t st, const Mx4Linear &a);
+// Few rows are quantised inside the product's own launch: then launch_mx4_linear takes them as `x`, not as codes.
+bool mx4_linear_fuses(long long rows, int cols);
+void launch_mx4_linear(hipStream_t st, Mx4Linear a, const Mx4Rows *x);
 
 // ortho_kernels.hip: Newton-Schulz orthogonalisation and the optimiser step on it.  The group's workspace holds an area
 // per matrix (OrthoItem::ws); `first` is scratch of the launches.

@@ -787,8 +787,8 @@ int check_mx4_shape(int64_t rows, int64_t cols) {
 }
 
 int check_mx4_pointers(const uint8_t *codes, const uint8_t *scales) {
-    if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(scales) % 4)
-        return fail(NNB_ERR_ARG, "codes must be 16-byte, scales 4-byte aligned");
+    if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(scales) % 16)
+        return fail(NNB_ERR_ARG, "codes and scales must be 16-byte aligned");
     return NNB_OK;
 }
 
@@ -801,12 +801,12 @@ int check_workspace(const void *workspace, size_t bytes, size_t need) {
     return NNB_OK;
 }
 
-// Workspace of nnb_mx4_linear: the quantised rows.
+// Workspace of nnb_mx4_linear: the quantised rows, unless they come quantised or the product quantises them itself.
 void carve_mx4_rows(Carver &c, int64_t rows, int cols, bool x_quantized, uint8_t *&codes, uint8_t *&scales) {
     codes = scales = nullptr;
-    if (x_quantized) return;
+    if (x_quantized || mx4_linear_fuses(rows, cols)) return;
     codes = c.take<uint8_t>((size_t)rows * (mx4_padded(cols) / 2));
-    scales = c.take<uint8_t>((size_t)rows * (mx4_padded(cols) / 32));
+    scales = c.take<uint8_t>(mx4_scale_bytes(rows, cols));
 }
 
 // Limits of the orthogonalisation kernels' indices.
@@ -1399,6 +1399,12 @@ int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *p, void *workspace, 
     a.x_codes = p->x_codes; a.x_scales = p->x_scales; a.w_codes = p->w_codes; a.w_scales = p->w_scales;
     a.bias = p->bias; a.bias_type = p->bias_type; a.y = p->y; a.y_type = p->y_type; a.y_stride = p->y_row_stride;
     a.rows = p->rows; a.kp = mx4_padded((int)p->cols); a.n = (int)p->out_features; a.relu = p->relu != 0;
+    if (!quantized && mx4_linear_fuses(p->rows, (int)p->cols)) {
+        const Mx4Rows x = {p->x, p->x_row_stride, p->x_col_stride, p->x_type, (int)p->cols};
+        launch_mx4_linear(st, a, &x);
+        HIP_TRY(hipGetLastError());
+        return NNB_OK;
+    }
     if (!quantized) {
         Carver c(workspace);
         uint8_t *codes, *scales;
@@ -1407,7 +1413,7 @@ int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *p, void *workspace, 
                             scales);
         a.x_codes = codes; a.x_scales = scales;
     }
-    launch_mx4_linear(st, a);
+    launch_mx4_linear(st, a, nullptr);
     HIP_TRY(hipGetLastError());
     return NNB_OK;
 }

@@ -31,11 +31,18 @@ def _padded(cols: int) -> int:
     return -(-cols // PAD) * PAD
 
 
+def _scale_shape(rows: int, cols: int) -> tuple:
+    """Blocks of 256 bytes, one per 16 rows and 512 elements (see nnb_mx4_quantize for the order within)."""
+    return (-(-rows // 16), -(-cols // 512), 256)
+
+
 class MX4Tensor:
     """Quantised numbers of shape `shape`, blocks along the last dimension.
 
     codes   uint8 [rows, Kp/2], Kp = the last dimension rounded up to 128: two elements a byte, the even one low
-    scales  uint8 [rows, Kp/32]: exponent + 127 of each block's scale, 255 = not a number
+    scales  uint8 [ceil(rows/16), ceil(Kp/512), 256]: exponent + 127 of each block's scale, 255 = not a number, in the
+            order in which the matrix instruction takes them: the scale of row r, block b is byte
+            ((b % 4) * 16 + r % 16) * 4 + (b // 4) % 4 of [r // 16, b // 16]
     """
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
@@ -43,9 +50,9 @@ class MX4Tensor:
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError(f"shape {tuple(shape)} has no last dimension to cut into blocks")
         rows, kp = shape[:-1].numel(), _padded(shape[-1])
-        for name, t, width in (("codes", codes, kp // 2), ("scales", scales, kp // 32)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != (rows, width) or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous uint8 of shape {(rows, width)}, got {t.dtype} {tuple(t.shape)}")
+        for name, t, want in (("codes", codes, (rows, kp // 2)), ("scales", scales, _scale_shape(rows, kp))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous uint8 of shape {want}, got {t.dtype} {tuple(t.shape)}")
         if codes.device != scales.device:
             raise ValueError("codes and scales are on different devices")
         self.codes, self.scales, self.shape = codes, scales, shape
@@ -96,7 +103,7 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
         rows, cols = v.shape
         kp = _padded(cols)
         codes = torch.empty((rows, kp // 2), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((rows, kp // 32), dtype=torch.uint8, device=x.device)
+        scales = torch.empty(_scale_shape(rows, kp), dtype=torch.uint8, device=x.device)
         check(_lib.load().nnb_mx4_quantize(stream_of(x), code, rows, cols, ptr(v), v.stride(0), v.stride(1), ptr(codes),
                                            ptr(scales)), "nnb_mx4_quantize")
     return MX4Tensor(codes, scales, x.shape)

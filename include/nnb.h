@@ -390,8 +390,10 @@ enum nnb_dtype { NNB_F32 = 0, NNB_F16 = 1, NNB_BF16 = 2 };
  * e = floor(log2 max|x|) - 2 clamped to [-127, 127] and stored as the byte e + 127; an element is the e2m1 code of
  * x / 2^e (values 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), to nearest with ties to the even code and beyond 6
  * to 6.  A block that holds an infinity or a NaN gets the byte 255 and reads as NaN.  Rows are padded with zeros to
- * Kp = the next multiple of 128: codes_out [rows][Kp/2], 16-byte aligned, element 2i in the low half of byte i;
- * scales_out [rows][Kp/32], 4-byte aligned.
+ * Kp = the next multiple of 128: codes_out [rows][Kp/2], 16-byte aligned, element 2i in the low half of byte i.
+ * scales_out, 16-byte aligned, holds ceil(rows/16) * ceil(Kp/512) blocks of 256 bytes: the scale of row r, block b is
+ * byte ((b % 4) * 16 + r % 16) * 4 + (b / 4) % 4 of block (r / 16) * ceil(Kp/512) + b / 16 (the order in which the matrix
+ * instruction takes them; bytes that belong to no row or block are written too).
  * x [rows][cols] of type x_type (nnb_dtype), element (r, c) at x[r*row_stride + c*col_stride] (strides in elements, may
  * be 0 or negative).  rows = 0 is a no-op; cols in [1, 2^24], rows at most 2^31 - 1. */
 int nnb_mx4_quantize(void *stream, int x_type, int64_t rows, int64_t cols, const void *x, int64_t row_stride,

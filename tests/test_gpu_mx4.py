@@ -57,7 +57,7 @@ def test_quantize_equals_its_definition(shape, dtype):
     q = mx4.quantize(x.cuda())
     _same(q.dequantize().cpu(), quantized(x.double().numpy()))
     kp = -(-shape[1] // 128) * 128
-    assert q.codes.shape == (shape[0], kp // 2) and q.scales.shape == (shape[0], kp // 32)
+    assert q.codes.shape == (shape[0], kp // 2) and q.scales.shape == (-(-shape[0] // 16), -(-kp // 512), 256)
     blocks = -(-shape[1] // 32)
     assert not q.codes[:, blocks * 16:].any()                          # padding multiplies as zero
 

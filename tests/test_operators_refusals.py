@@ -55,24 +55,25 @@ def test_mx4_linear_refuses_bad_arguments(lib):
                      (dict(x=None), "null"), (dict(w_codes=4104), "aligned"), (dict(y_row_stride=7), "y_row_stride"),
                      (dict(out_features=-2), "rows")):
         assert call(**kw) == -1 and word in _message(lib), kw
-    assert call(ws=None) == -4 and "needed" in _message(lib)
-    assert call(ws_bytes=16) == -4
-    assert call(ws=C.c_void_p(4097)) == -4 and "aligned" in _message(lib)
+    assert call(rows=40, ws=None) == -4 and "needed" in _message(lib)
+    assert call(rows=40, ws_bytes=16) == -4
+    assert call(rows=40, ws=C.c_void_p(4097)) == -4 and "aligned" in _message(lib)
     assert call(rows=0, x=None) == 0 and call(out_features=0) == 0
     assert lib.nnb_mx4_linear(None, None, None, 0) == -1
     n = C.c_size_t()
     assert lib.nnb_mx4_linear_workspace_bytes(4, 64, 8, 0, None) == -1
-    assert lib.nnb_mx4_linear_workspace_bytes(4, 64, 8, 0, C.byref(n)) == 0 and n.value >= 4 * (64 + 4)
+    assert lib.nnb_mx4_linear_workspace_bytes(4, 64, 8, 0, C.byref(n)) == 0 and n.value == 0
+    assert lib.nnb_mx4_linear_workspace_bytes(40, 11520, 8, 0, C.byref(n)) == 0 and n.value >= 40 * (5760 + 360)
 
 
 def test_mx4_python_refusals():
     import torch
     from alphazero_amd import mx4
     from alphazero_amd._lib import NnbError
-    codes, scales = torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.uint8)
+    codes, scales = torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(1, 1, 256, dtype=torch.uint8)
     w = mx4.MX4Tensor(codes, scales, (8, 100))
     for bad in ((codes, scales, (8, 300)), (codes, scales, (7, 100)), (codes.int(), scales, (8, 100)), (codes, scales, ()),
-                (codes, scales, (8, 0)), (codes[:, ::2], scales, (8, 60))):
+                (codes, scales, (8, 0)), (codes.t().contiguous().t(), scales, (8, 100)), (codes, scales[:, :, :128], (8, 100))):
         with pytest.raises(ValueError):
             mx4.MX4Tensor(*bad)
     with pytest.raises(ValueError):
