@@ -45,63 +45,59 @@ __device__ __forceinline__ uint32_t encode8(const float (&v)[8], uint32_t byte) 
     return r;
 }
 
-template <typename T> struct alignas(16) Pack8 { T v[8]; };
+// Eight elements in one or two wide accesses; global memory takes them at any element's alignment.
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Pack8 { T v[8]; };
 
-// x [rows][cols] (any strides) -> codes, scales.  A wave takes 16 rows x 512 elements: eight per lane and row, so that
-// four lanes share a block, all sixteen loads in flight; the sixteen rows' scale bytes meet in LDS and leave as one
-// word block.  `wide`: a lane's eight elements are 16 / 32 aligned bytes.  row_count (may be null): live rows, read on
-// the device.
+// x [rows][cols] (any strides) -> codes, scales.  A block takes 16 rows x 512 elements, a wave four of the rows, a lane
+// eight elements of each, so that four lanes share a scale; the sixteen rows' scale bytes meet in LDS and leave as one
+// word block.  row_count (may be null): live rows, read on the device.
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__ x, long long rows, int cols, int kp,
-                                                           long long row_stride, long long col_stride, bool wide,
+                                                           long long row_stride, long long col_stride,
                                                            const int32_t *__restrict__ row_count,
                                                            uint32_t *__restrict__ codes, uint32_t *__restrict__ scales) {
-    __shared__ uint8_t bytes[4][256];
+    __shared__ uint32_t bytes[64];
     if (row_count) rows = *row_count < rows ? *row_count : rows;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int words = mx4_scale_words(kp);
     const long long tasks = (rows + 15) / 16 * words;
-    const long long waves = (long long)gridDim.x * 4;
-    for (long long t = (long long)blockIdx.x * 4 + wave; t < tasks; t += waves) {
-        const long long row0 = t / words * 16;
+    for (long long t = blockIdx.x; t < tasks; t += gridDim.x) {
+        const long long row0 = t / words * 16 + wave * 4;
         const int k = (int)(t % words) * 512 + lane * 8;
         const T *p = x + row0 * row_stride + k * col_stride;
-        const int n_rows = rows - row0 < 16 ? (int)(rows - row0) : 16;
-        const bool whole = wide && k + 8 <= cols;
+        Pack8<T> q[4];
+        if (col_stride == 1 && k + 8 <= cols) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            Pack8<T> q[8];
+            for (int i = 0; i < 4; ++i)
+                if (row0 + i < rows) q[i] = *reinterpret_cast<const Pack8<T> *>(p + i * row_stride);
+                else q[i] = {};
+        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = half * 8 + i;
-                if (r < n_rows && whole) {
-                    q[i] = *reinterpret_cast<const Pack8<T> *>(p + r * row_stride);
-                } else {
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        q[i].v[j] = r < n_rows && k + j < cols ? p[r * row_stride + j * col_stride] : T(0.f);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = half * 8 + i;
-                float v[8];
-                uint32_t top = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[j] = to_f32(q[i].v[j]);
-                    const uint32_t m = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;   // magnitudes order as integers
-                    top = m > top ? m : top;
-                }
-                top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-                top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-                const uint32_t byte = scale_byte(top);
-                if (r < n_rows && k < kp) codes[((row0 + r) * kp + k) >> 3] = byte == 255 ? 0 : encode8(v, byte);
-                if ((lane & 3) == (i & 3)) bytes[wave][((lane >> 2 & 3) * 16 + r) * 4 + (lane >> 4)] = (uint8_t)byte;
-            }
+                for (int j = 0; j < 8; ++j)
+                    q[i].v[j] = row0 + i < rows && k + j < cols ? p[i * row_stride + j * col_stride] : T(0.f);
         }
-        // the wave's own LDS accesses complete in order
-        scales[t * 64 + lane] = reinterpret_cast<const uint32_t *>(bytes[wave])[lane];
+        uint8_t *b = reinterpret_cast<uint8_t *>(bytes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v[8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = to_f32(q[i].v[j]);
+                const uint32_t m = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;       // magnitudes order as integers
+                top = m > top ? m : top;
+            }
+            top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+            const uint32_t byte = scale_byte(top);
+            if (row0 + i < rows && k < kp) codes[((row0 + i) * kp + k) >> 3] = byte == 255 ? 0 : encode8(v, byte);
+            if ((lane & 3) == i) b[((lane >> 2 & 3) * 16 + wave * 4 + i) * 4 + (lane >> 4)] = (uint8_t)byte;
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) scales[t * 64 + lane] = bytes[lane];
+        __syncthreads();
     }
 }
 
@@ -114,7 +110,7 @@ __device__ __forceinline__ float mx4_value(uint32_t code, float scale) {
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ scales, long long rows, int cols,
-                                                             int kp, bool wide, T *__restrict__ out) {
+                                                             int kp, T *__restrict__ out) {
     const int groups = kp >> 3;
     const long long total = rows * groups, stride = (long long)gridDim.x * 256;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
@@ -127,7 +123,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t *__r
 #pragma unroll
         for (int j = 0; j < 8; ++j) q.v[j] = from_f32<T>(mx4_value(c >> (4 * j), scale));
         T *p = out + row * cols + k;
-        if (wide && k + 8 <= cols) {
+        if (k + 8 <= cols) {
             *reinterpret_cast<Pack8<T> *>(p) = q;
         } else {
 #pragma unroll
@@ -254,7 +250,20 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
     const int read0 = (lane & 15) * 8 + ((lane >> 4) ^ (lane & 7));
 
     f32x4 acc[TX][TW] = {};
-    int sx[TX], sw[TW];
+    int sx[TX], sw[TW], sx_next[TX], sw_next[TW];
+    auto load_scales = [&](int word) {
+#pragma unroll
+        for (int i = 0; i < TX; ++i) sx_next[i] = (int)xs[i][word * 64];
+#pragma unroll
+        for (int i = 0; i < TW; ++i) sw_next[i] = (int)ws[i][word * 64];
+    };
+    // Every load this wave has issued has landed, and after the barrier everybody's; nobody reads the other buffer any
+    // more.  The wait is the builtin so that the compiler knows of it and adds none between the next stage's loads and
+    // the products.
+    auto meet = [&] {
+        __builtin_amdgcn_s_waitcnt(0x0070);                  // vmcnt(0) lgkmcnt(0)
+        asm volatile("s_barrier" ::: "memory");
+    };
     auto compute = [&](int t, int s, int step_of_word) {
         i32x4 xf[TX], wf[TW];
         const i32x4 *base = lds[t & 1];
@@ -268,19 +277,22 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
             for (int j = 0; j < TW; ++j) acc[i][j] = mfma_mx4(wf[j], xf[i], acc[i][j], sw[j], sx[i], step_of_word);
     };
     issue(0);
+    load_scales(0);
     for (int t = 0; t < stages; t += 2) {
+        meet();
 #pragma unroll
-        for (int i = 0; i < TX; ++i) sx[i] = xs[i][t / 2 * 64];
+        for (int i = 0; i < TX; ++i) sx[i] = sx_next[i];
 #pragma unroll
-        for (int i = 0; i < TW; ++i) sw[i] = ws[i][t / 2 * 64];
-        // this stage's loads have landed everywhere, and nobody reads the other buffer any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int i = 0; i < TW; ++i) sw[i] = sw_next[i];
         if (t + 1 < stages) issue(t + 1);
         compute(t, 0, 0);
         if (2 * t + 1 < steps) compute(t, 1, 1);
         if (t + 1 < stages) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (t + 2 < stages) issue(t + 2);
+            meet();
+            if (t + 2 < stages) {
+                issue(t + 2);
+                load_scales(t / 2 + 1);
+            }
             compute(t + 1, 0, 2);
             if (2 * t + 3 < steps) compute(t + 1, 1, 3);
         }
@@ -307,7 +319,7 @@ constexpr int kRowsWaves = 8;
 
 template <typename T, int RT, typename X, bool FUSED>
 __global__ __launch_bounds__(kRowsWaves * 64) void mx4_rows_kernel(Mx4Linear a, const X *__restrict__ x, int cols,
-                                                                  long long row_stride, long long col_stride, bool wide_x) {
+                                                                  long long row_stride, long long col_stride) {
     __shared__ f32x4 part[kRowsWaves][RT][64];
     __shared__ uint32_t xcodes[FUSED ? kMx4FusedElements / 8 : 1];
     __shared__ uint8_t xbytes[FUSED ? kMx4FusedElements / 32 : 1];
@@ -351,7 +363,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mx4_rows_kernel(Mx4Linear a, 
             const int r = i / per_row, k = (i - r * per_row) * 8;
             const X *p = x + r * row_stride + k * col_stride;
             float v[8];
-            if (wide_x && k + 8 <= cols) {
+            if (col_stride == 1 && k + 8 <= cols) {
                 const Pack8<X> q = *reinterpret_cast<const Pack8<X> *>(p);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = to_f32(q.v[j]);
@@ -421,12 +433,10 @@ void launch_mx4_quantize(hipStream_t st, int type, long long rows, int cols, con
                          long long col_stride, const int32_t *row_count, uint8_t *codes, uint8_t *scales) {
     const int kp = mx4_padded(cols);
     const long long tasks = (rows + 15) / 16 * mx4_scale_words(kp);
-    const long long blocks = (tasks + 3) / 4;
     with_dtype(type, [&](auto t) {
         typedef decltype(t) T;
-        const bool wide = col_stride == 1 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && row_stride * sizeof(T) % 16 == 0;
-        mx4_quantize_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(
-            static_cast<const T *>(x), rows, cols, kp, row_stride, col_stride, wide, row_count,
+        mx4_quantize_kernel<T><<<(int)(tasks < 16384 ? tasks : 16384), 256, 0, st>>>(
+            static_cast<const T *>(x), rows, cols, kp, row_stride, col_stride, row_count,
             reinterpret_cast<uint32_t *>(codes), reinterpret_cast<uint32_t *>(scales));
     });
 }
@@ -437,9 +447,8 @@ void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, c
     const long long blocks = (rows * (kp / 8) + 255) / 256;
     with_dtype(type, [&](auto t) {
         typedef decltype(t) T;
-        const bool wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && cols * sizeof(T) % 16 == 0;
         mx4_dequantize_kernel<T><<<(int)(blocks < 16384 ? blocks : 16384), 256, 0, st>>>(
-            reinterpret_cast<const uint32_t *>(codes), scales, rows, cols, kp, wide, static_cast<T *>(out));
+            reinterpret_cast<const uint32_t *>(codes), scales, rows, cols, kp, static_cast<T *>(out));
     });
 }
 
@@ -453,16 +462,14 @@ void launch_mx4_linear(hipStream_t st, Mx4Linear a, const Mx4Rows *x) {
         if (x) {
             with_dtype(x->type, [&](auto u) {
                 typedef decltype(u) X;
-                const bool wide = x->col_stride == 1 && reinterpret_cast<uintptr_t>(x->x) % 16 == 0 &&
-                                  x->row_stride * sizeof(X) % 16 == 0;
                 mx4_rows_kernel<T, 1, X, true><<<dim3(features, 1), kRowsWaves * 64, 0, st>>>(
-                    a, static_cast<const X *>(x->x), x->cols, x->row_stride, x->col_stride, wide);
+                    a, static_cast<const X *>(x->x), x->cols, x->row_stride, x->col_stride);
             });
         } else if (a.rows <= 16) {
-            mx4_rows_kernel<T, 1, float, false><<<dim3(features, 1), kRowsWaves * 64, 0, st>>>(a, nullptr, 0, 0, 0, false);
+            mx4_rows_kernel<T, 1, float, false><<<dim3(features, 1), kRowsWaves * 64, 0, st>>>(a, nullptr, 0, 0, 0);
         } else if (a.rows <= 256) {
             mx4_rows_kernel<T, 4, float, false><<<dim3(features, (unsigned)((a.rows + 63) / 64)), kRowsWaves * 64, 0, st>>>(
-                a, nullptr, 0, 0, 0, false);
+                a, nullptr, 0, 0, 0);
         } else {
             auto tiles = [&](int r, int f) { return (a.rows + r - 1) / r * ((a.n + f - 1) / f); };
             if (tiles(256, 256) >= 256)
