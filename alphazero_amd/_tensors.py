@@ -1,6 +1,7 @@
 """What the operators that take torch tensors need to hand them to libnnb.so."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -16,15 +17,19 @@ def dtype_code(t: torch.Tensor, name: str) -> int:
     return DTYPES[t.dtype]
 
 
+_STAY = contextlib.nullcontext()
+
+
 def on_device(t: torch.Tensor):
     """Makes the tensor's GPU current, which the library launches on."""
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise NnbError(f"a tensor on {t.device}: the kernels run on an MI355X only (there is no CPU path)")
-    return torch.cuda.device(t.device)
+    # switching devices costs more than a small launch: only where it changes something
+    return _STAY if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def stream_of(t: torch.Tensor) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(t.get_device()))
 
 
 def ptr(t: torch.Tensor) -> C.c_void_p:

@@ -156,16 +156,11 @@ void launch_net_stage_split(hipStream_t st, int stage, const NetWeights &w, cons
                             const int32_t *count_ptr, int n_max);
 void launch_split_to_f32(hipStream_t st, const void *act, const float *inv_scale, int cells, int n, float *out);
 
-// mx4_kernels.hip: 4-bit floats with a power-of-two scale per 32, rows padded to whole k-steps of the matrix unit
-constexpr int kMx4Pad = 128;
+// mx4_kernels.hip: 4-bit floats with a power-of-two scale per block of 32, in units of 32 rows x 256 elements
+constexpr int kMx4Pad = 256;
 __host__ __device__ constexpr int mx4_padded(int cols) { return (cols + kMx4Pad - 1) / kMx4Pad * kMx4Pad; }
-// Scales lie in word blocks of 256 bytes: 16 rows x four k-steps of 128
-__host__ __device__ constexpr int mx4_scale_words(int kp) { return (kp + 511) / 512; }
-__host__ __device__ constexpr size_t mx4_scale_bytes(long long rows, int cols) {
-    return (size_t)((rows + 15) / 16) * mx4_scale_words(mx4_padded(cols)) * 256;
-}
-__host__ __device__ constexpr size_t mx4_scale_at(long long row, int block, int kp) {
-    return ((size_t)(row / 16) * mx4_scale_words(kp) + block / 16) * 256 + ((block % 4) * 16 + row % 16) * 4 + block / 4 % 4;
+__host__ __device__ constexpr size_t mx4_units(long long rows, int cols) {
+    return (size_t)((rows + 31) / 32) * (mx4_padded(cols) / 256);
 }
 struct Mx4Linear {                      // y [rows][n] = x * w^T (+ bias, ReLU)
     const uint8_t *x_codes, *x_scales;

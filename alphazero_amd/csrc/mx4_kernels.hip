@@ -5,11 +5,12 @@
 // for codes 0..7, to nearest with ties to the even code, beyond 6 to 6.  A block that holds an infinity or a NaN gets
 // the scale byte 255 and reads as NaN.
 //
-// Codes: [rows][Kp/2] bytes, Kp = K padded with zeros to k-steps of 128, element 2i in the low half of byte i.
-// Scales: one 256-byte word block per 16 rows and four k-steps, in the order the matrix instruction wants them: lane
-// l = 16 * (k-block within the step) + (row within the 16) holds four bytes, one per k-step, so a fragment's scales
-// for 512 elements are one coalesced load and the instruction picks the byte itself.  (Scales in row order cost a cache
-// line per row and fetch; the codes' own traffic is what the large product waits for.)
+// Layout: units of 32 rows x 256 elements (rows and K are padded with zeros), 4096 bytes of codes and 256 of scales each,
+// [row / 32][k / 256], in the order in which v_mfma_scale_f32_32x32x64_f8f6f4 takes them: lane l = 32 * half + row of k-step s
+// holds the 32 elements (one block) 64 s + 32 half of its row, 16 bytes at (64 s + l) * 16 (element 2i in the low half of
+// byte i), and their scale is byte s of word l.  A unit is contiguous, so whole kilobytes move between memory and LDS
+// whatever K is (rows of a power-of-two length would all start on the same memory channels), a fragment is one
+// conflict-free LDS read, and its four k-steps' scales one word.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -45,40 +46,41 @@ __device__ __forceinline__ uint32_t encode8(const float (&v)[8], uint32_t byte) 
     return r;
 }
 
+template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) PackN { T v[N]; };
 // Eight elements in one or two wide accesses; global memory takes them at any element's alignment.
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Pack8 { T v[8]; };
 
-// x [rows][cols] (any strides) -> codes, scales.  A block takes 16 rows x 512 elements, a wave four of the rows, a lane
-// eight elements of each, so that four lanes share a scale; the sixteen rows' scale bytes meet in LDS and leave as one
-// word block.  row_count (may be null): live rows, read on the device.
+// x [rows][cols] (any strides) -> codes, scales.  A block makes one unit: a thread eight elements of four rows, so that
+// four lanes share a scale; codes and scales meet in LDS and leave in whole lines.  row_count (may be null): live rows,
+// read on the device.
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__ x, long long rows, int cols, int kp,
                                                            long long row_stride, long long col_stride,
                                                            const int32_t *__restrict__ row_count,
-                                                           uint32_t *__restrict__ codes, uint32_t *__restrict__ scales) {
+                                                           uint4 *__restrict__ codes, uint32_t *__restrict__ scales) {
+    __shared__ uint4 unit[256];
     __shared__ uint32_t bytes[64];
     if (row_count) rows = *row_count < rows ? *row_count : rows;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int words = mx4_scale_words(kp);
-    const long long tasks = (rows + 15) / 16 * words;
+    const int units = kp / 256;
+    const long long tasks = (rows + 31) / 32 * units;
+    const int group = threadIdx.x & 31, r0 = threadIdx.x >> 5;  // eight elements of the 256, rows r0, r0 + 8, + 16, + 24
     for (long long t = blockIdx.x; t < tasks; t += gridDim.x) {
-        const long long row0 = t / words * 16 + wave * 4;
-        const int k = (int)(t % words) * 512 + lane * 8;
+        const long long row0 = t / units * 32 + r0;
+        const int k = (int)(t % units) * 256 + group * 8;
         const T *p = x + row0 * row_stride + k * col_stride;
         Pack8<T> q[4];
         if (col_stride == 1 && k + 8 <= cols) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (row0 + i < rows) q[i] = *reinterpret_cast<const Pack8<T> *>(p + i * row_stride);
+                if (row0 + 8 * i < rows) q[i] = *reinterpret_cast<const Pack8<T> *>(p + 8 * i * row_stride);
                 else q[i] = {};
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    q[i].v[j] = row0 + i < rows && k + j < cols ? p[i * row_stride + j * col_stride] : T(0.f);
+                    q[i].v[j] = row0 + 8 * i < rows && k + j < cols ? p[8 * i * row_stride + j * col_stride] : T(0.f);
         }
-        uint8_t *b = reinterpret_cast<uint8_t *>(bytes);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float v[8];
@@ -92,102 +94,128 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__
             top = max(top, (uint32_t)__shfl_xor((int)top, 1));
             top = max(top, (uint32_t)__shfl_xor((int)top, 2));
             const uint32_t byte = scale_byte(top);
-            if (row0 + i < rows && k < kp) codes[((row0 + i) * kp + k) >> 3] = byte == 255 ? 0 : encode8(v, byte);
-            if ((lane & 3) == i) b[((lane >> 2 & 3) * 16 + wave * 4 + i) * 4 + (lane >> 4)] = (uint8_t)byte;
+            const int lane = (group >> 2 & 1) * 32 + r0 + 8 * i, step = group >> 3;
+            reinterpret_cast<uint32_t *>(unit)[(step * 64 + lane) * 4 + (group & 3)] = byte == 255 ? 0 : encode8(v, byte);
+            if ((group & 3) == i) reinterpret_cast<uint8_t *>(bytes)[lane * 4 + step] = (uint8_t)byte;
         }
         __syncthreads();
-        if (threadIdx.x < 64) scales[t * 64 + lane] = bytes[lane];
+        codes[t * 256 + threadIdx.x] = unit[threadIdx.x];
+        if (threadIdx.x < 64) scales[t * 64 + threadIdx.x] = bytes[threadIdx.x];
         __syncthreads();
     }
 }
 
-__device__ __forceinline__ float mx4_value(uint32_t code, float scale) {
-    const uint32_t m = code & 7;
-    const float size = m < 2 ? 0.5f * (float)m : __builtin_ldexpf(1.f + 0.5f * (float)(m & 1), (int)(m >> 1) - 1);
-    return (code & 8 ? -size : size) * scale;
-}
-
+// A block turns one unit back into numbers: its 16-byte blocks meet in LDS row by row, then every lane writes 16 bytes of
+// a row's 256 columns.
 template <typename T>
-__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t *__restrict__ codes,
-                                                             const uint8_t *__restrict__ scales, long long rows, int cols,
-                                                             int kp, T *__restrict__ out) {
-    const int groups = kp >> 3;
-    const long long total = rows * groups, stride = (long long)gridDim.x * 256;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-        const long long row = i / groups;
-        const int k = (int)(i - row * groups) * 8;
-        if (k >= cols) continue;
-        const uint32_t c = codes[i], byte = scales[mx4_scale_at(row, k >> 5, kp)];
-        const float scale = __builtin_bit_cast(float, byte == 255 ? 0x7fc00000u : byte ? byte << 23 : 0x00400000u);
-        Pack8<T> q;
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint4 *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                                             long long rows, int cols, int kp, bool aligned, T *__restrict__ out) {
+    constexpr int kPack = 16 / sizeof(T), kRowLanes = 256 / kPack;
+    __shared__ uint4 blocks[32][9];
+    __shared__ uint8_t bytes[256];
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const int units = kp / 256, tid = threadIdx.x;
+    const long long tasks = (rows + 31) / 32 * units;
+    for (long long t = blockIdx.x; t < tasks; t += gridDim.x) {
+        const long long row0 = t / units * 32;
+        const int k0 = (int)(t % units) * 256;
+        blocks[tid & 31][tid >> 5] = codes[t * 256 + tid];           // piece (k-step, half) = tid / 32 of row tid % 32
+        bytes[tid] = scales[t * 256 + tid];
+        __syncthreads();
+        const int k = tid % kRowLanes * kPack, block = k >> 5;
+#pragma unroll 4
+        for (int r = tid / kRowLanes; r < 32; r += 256 / kRowLanes) {
+            if (row0 + r >= rows || k0 + k >= cols) continue;
+            const uint32_t byte = bytes[((block & 1) * 32 + r) * 4 + (block >> 1)];
+            const float scale = __builtin_bit_cast(float, byte ? byte << 23 : 0x00400000u);
+            const uint8_t *c = reinterpret_cast<const uint8_t *>(&blocks[r][block]) + (k & 31) / 2;
+            PackN<T, kPack> q;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q.v[j] = from_f32<T>(mx4_value(c >> (4 * j), scale));
-        T *p = out + row * cols + k;
-        if (k + 8 <= cols) {
-            *reinterpret_cast<Pack8<T> *>(p) = q;
-        } else {
+            for (int e = 0; e < kPack; e += 4) {
+                const uint32_t pair = *reinterpret_cast<const uint16_t *>(c + e / 2);
+                const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(pair, scale, 0);
+                const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(pair, scale, 1);
+                const float v[4] = {a[0], a[1], b[0], b[1]};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k + j < cols) p[j] = q.v[j];
+                for (int j = 0; j < 4; ++j) q.v[e + j] = from_f32<T>(byte == 255 ? __builtin_nanf("") : v[j]);
+            }
+            T *p = out + (row0 + r) * cols + k0 + k;
+            if (aligned) {
+                *reinterpret_cast<PackN<T, kPack> *>(p) = q;
+            } else {
+#pragma unroll
+                for (int j = 0; j < kPack; ++j)
+                    if (k0 + k + j < cols) p[j] = q.v[j];
+            }
         }
+        __syncthreads();
     }
 }
 
 // ----------------------------------------------------------------------------------------------- linear layer
 //
-// y [rows][n] = x [rows][K] * w [n][K]^T (+ bias, ReLU), both in MX4, on v_mfma_scale_f32_16x16x128_f8f6f4: lane l of a
-// 16 x 128 fragment holds the 32 elements (one scale block) l/16 of row l%16.  The weights are the instruction's first
+// y [rows][n] = x [rows][K] * w [n][K]^T (+ bias, ReLU), both in MX4.  The weights are the matrix instructions' first
 // operand, so a lane ends up with four consecutive features of one row: one store.
 
-__device__ __forceinline__ f32x4 mfma_mx4(i32x4 w, i32x4 x, f32x4 acc, int w_scale, int x_scale, int step) {
-    const i32x8 w8 = __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
-    const i32x8 x8 = __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
-    // 4 = e2m1; the byte of the scale word is part of the instruction
-    switch (step) {
-    case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc, 4, 4, 0, w_scale, 0, x_scale);
-    case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc, 4, 4, 1, w_scale, 1, x_scale);
-    case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc, 4, 4, 2, w_scale, 2, x_scale);
-    default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc, 4, 4, 3, w_scale, 3, x_scale);
-    }
+__device__ __forceinline__ i32x8 operand(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
+
+// 32 x 32 x 64: lane l holds the 32 elements (one block) l/32 of row l%32; 4 = e2m1; the byte of the scale words is
+// part of the instruction.
+template <int BYTE>
+__device__ __forceinline__ f32x16 mfma_mx4_32(i32x4 w, i32x4 x, f32x16 acc, int w_scale, int x_scale) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w), operand(x), acc, 4, 4, BYTE, w_scale, BYTE, x_scale);
+}
+// 16 x 16 x 128: block l/16 of row l%16.
+template <int W_BYTE, int X_BYTE>
+__device__ __forceinline__ f32x4 mfma_mx4_16(i32x4 w, i32x4 x, f32x4 acc, int w_scale, int x_scale) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(x), acc, 4, 4, W_BYTE, w_scale, X_BYTE, x_scale);
 }
 
-// Bias, ReLU, rounding and store of the four features c .. c + 3 of row r.
-template <typename T> struct alignas(4 * sizeof(T)) Pack4 { T v[4]; };
-template <typename T>
-__device__ __forceinline__ void store_features(const Mx4Linear &a, long long r, int c, f32x4 acc, const float (&bias)[4]) {
-    Pack4<T> q;
+// Bias, ReLU, rounding and store of the N features c .. c + N - 1 of row r.
+template <typename T, int N>
+__device__ __forceinline__ void store_features(const Mx4Linear &a, long long r, int c, const float *sum, const float (&bias)[N]) {
+    const float least = a.relu ? 0.f : -__builtin_inff();
+    PackN<T, N> q;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float v = acc[e] + bias[e];
-        if (a.relu) v = v < 0.f ? 0.f : v;                   // NaN stays NaN
-        q.v[e] = from_f32<T>(v);
+    for (int e = 0; e < N; ++e) {
+        const float v = sum[e] + bias[e];
+        q.v[e] = from_f32<T>(v < least ? least : v);         // NaN stays NaN
     }
     T *p = static_cast<T *>(a.y) + r * a.y_stride + c;
-    if (a.wide && c + 4 <= a.n) {
-        *reinterpret_cast<Pack4<T> *>(p) = q;
+    if (a.wide && c + N <= a.n) {
+        *reinterpret_cast<PackN<T, N> *>(p) = q;
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < N; ++e)
             if (c + e < a.n) p[e] = q.v[e];
     }
 }
-__device__ __forceinline__ void load_bias(const Mx4Linear &a, int c, float (&bias)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) bias[e] = a.bias && c + e < a.n ? load_as_f32(a.bias, a.bias_type, c + e) : 0.f;
+
+// Large products on 32 x 32 x 64 tiles (measured alone: 6.5 PFLOP/s with one wave per SIMD, 16 x 16 x 128 3.6).  A block
+// of 2 x 2 waves computes (TX * 64) rows x (TW * 64) features.  A stage is 256 elements of every row, one unit per 32
+// rows, brought to LDS by the loads themselves into a ring of RING stages.  Operands are read from LDS AHEAD k-steps
+// before they multiply; all waves meet once per stage, when its last operands are in registers: from then on its place in
+// the ring is free for the stage RING further on, and the next one's operands are read while the last AHEAD k-steps
+// multiply.
+
+// 16 bytes a lane from base + offset to 1 KB of LDS at `to` (both uniform).  In assembly because the compiler, which
+// cannot tell the ring's stages apart, would wait for every load in flight before every read of LDS; the kernel's own
+// wait in front of its barrier is the only one needed.
+__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t offset, void *to) {
+    const uint32_t m0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)to;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
 }
 
-// Large products.  A block computes (WX * TX * 16) rows x (WW * TW * 16) features with WX x WW waves; a stage is 256
-// elements (128 bytes) of every row, brought to LDS by the loads themselves, two stages in turn.  A row's eight 16-byte
-// chunks lie at chunk ^ (row & 7): a fragment read then touches every bank group once.
-#define LDS_PTR(p) (__attribute__((address_space(3))) uint32_t *)(p)
-#define GLOBAL_PTR(p) (const __attribute__((address_space(1))) uint32_t *)(p)
-
-template <typename T, int WX, int WW, int TX, int TW>
-__global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
-    constexpr int kRows = WX * TX * 16, kFeatures = WW * TW * 16, kWaves = WX * WW;
-    constexpr int kLoads = (kRows + kFeatures) / 8 / kWaves;         // 1 KB (8 rows x 128 bytes) each, per wave and stage
-    static_assert((kRows + kFeatures) % (8 * kWaves) == 0, "whole loads per wave");
-    __shared__ i32x4 lds[2][(kRows + kFeatures) * 8];
+template <typename T, int TX, int TW, int RING, int AHEAD>
+__global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
+    constexpr int kWaves = 4, kRows = 2 * TX * 32, kFeatures = 2 * TW * 32;
+    constexpr int kXUnits = 2 * TX, kUnits = 2 * TX + 2 * TW;        // per stage; a wave loads kUnits of 4 * kUnits kilobytes
+    constexpr int kScaleLoads = kUnits / 4;                          // 1 KB: the scales of four units
+    constexpr int kInFlight = (RING - 2) * (kUnits + 1);             // a wave's loads behind the stage it waits for
+    static_assert(kXUnits % 4 == 0 && kUnits % 4 == 0 && kScaleLoads <= kWaves && kInFlight < 64, "");
+    __shared__ i32x4 lds[RING][kUnits][256];
+    __shared__ i32x4 lds_scales[RING][kUnits][16];
     const long long rows = a.row_count && *a.row_count < a.rows ? *a.row_count : a.rows;
 
     // Tiles in groups of eight row tiles walked feature tile by feature tile; consecutive tiles of the walk on one
@@ -205,115 +233,141 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
     if (row0 >= rows) return;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int steps = a.kp / 128, stages = (steps + 1) / 2;
-    const uint32_t cs = a.kp / 2;
-    const int chunk = (lane & 7) ^ (lane >> 3);
-    const uint8_t *xbase = a.x_codes + row0 * cs, *wbase = a.w_codes + (size_t)col0 * cs;
-    uint32_t offset[kLoads];
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-        int r = (wave * kLoads + j) * 8 + (lane >> 3);
-        const bool is_x = r < kRows;
-        // rows and features past the end repeat the last one; their results are not stored
-        const long long left = is_x ? rows - row0 : (long long)(a.n - col0);
-        if (!is_x) r -= kRows;
-        r = r < left ? r : (int)left - 1;
-        offset[j] = (uint32_t)r * cs + chunk * 16;
-    }
-    auto issue = [&](int t) {
-        // an odd number of k-steps: the last stage's second half would lie behind the row; it fetches the first half again
-        const uint32_t k = t * 128 - (2 * t + 2 > steps && chunk >= 4 ? 64 : 0);
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const uint8_t *base = (wave * kLoads + j) * 8 < kRows ? xbase : wbase;
-            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(base + (size_t)(offset[j] + k)),
-                                             LDS_PTR(&lds[t & 1][(wave * kLoads + j) * 64]), 16, 0, 0);
-        }
+    const int stages = a.kp / 256;
+    // Unit u of the tile: kXUnits of x, then the weights'.  Rows and features past the end repeat the last unit; their
+    // results are not stored.
+    const long long x_unit0 = row0 / 32, w_unit0 = col0 / 32;
+    const int x_left = (int)((rows + 31) / 32 - x_unit0 < kXUnits ? (rows + 31) / 32 - x_unit0 : kXUnits) - 1;
+    const int w_left = ((a.n + 31) / 32 - (int)w_unit0 < kUnits - kXUnits ? (a.n + 31) / 32 - (int)w_unit0 : kUnits - kXUnits) - 1;
+    auto unit_at = [&](int u) {                                      // units of its tensor before it
+        const int i = u < kXUnits ? u : u - kXUnits, left = u < kXUnits ? x_left : w_left;
+        return ((u < kXUnits ? x_unit0 : w_unit0) + (i < left ? i : left)) * stages;
     };
-    const int wx = wave % WX * TX * 16, ww = wave / WX * TW * 16;    // this wave's first row and feature in the tile
-    const int words = mx4_scale_words(a.kp);
-    const uint32_t *xs[TX], *ws[TW];
+    const uint8_t *codes[kUnits / 4];                                // this wave's units: wave * kUnits / 4 + i
 #pragma unroll
-    for (int i = 0; i < TX; ++i) {
-        long long r = row0 + wx + i * 16;
-        r = r < rows ? r : rows - 1;
-        xs[i] = reinterpret_cast<const uint32_t *>(a.x_scales) + (r / 16 * words) * 64 + lane;
+    for (int i = 0; i < kUnits / 4; ++i) {
+        const int u = wave * (kUnits / 4) + i;
+        codes[i] = (u < kXUnits ? a.x_codes : a.w_codes) + unit_at(u) * 4096;
     }
+    const int sload = wave % kScaleLoads;                            // a spare wave repeats another one's load
+    const uint8_t *scales = (sload * 4 < kXUnits ? a.x_scales : a.w_scales) + unit_at(sload * 4) * 256;
+    const uint32_t soffset = (uint32_t)(unit_at(sload * 4 + (lane >> 4)) - unit_at(sload * 4)) * 256 + (lane & 15) * 16;
+    auto issue = [&](int t, int slot) {
 #pragma unroll
-    for (int i = 0; i < TW; ++i) {
-        int c = col0 + ww + i * 16;
-        c = c < a.n ? c : a.n - 1;
-        ws[i] = reinterpret_cast<const uint32_t *>(a.w_scales) + ((size_t)(c / 16) * words) * 64 + lane;
-    }
-    // where this lane finds chunk l/16 (first step of a stage; the second one's is the same with bit 6 of the byte address
-    // flipped) of row l%16 of a fragment
-    const int read0 = (lane & 15) * 8 + ((lane >> 4) ^ (lane & 7));
+        for (int i = 0; i < kUnits / 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                load_to_lds(codes[i] + (size_t)t * 4096 + j * 1024, lane * 16, &lds[slot][wave * (kUnits / 4) + i][j * 64]);
+        load_to_lds(scales + (size_t)t * 256, soffset, &lds_scales[slot][sload * 4][0]);
+    };
+    const int ux = wave % 2 * TX, uw = kXUnits + wave / 2 * TW;      // this wave's first units in the tile
 
-    f32x4 acc[TX][TW] = {};
-    int sx[TX], sw[TW], sx_next[TX], sw_next[TW];
-    auto load_scales = [&](int word) {
+    constexpr int kBuffers = AHEAD == 1 ? 2 : 4;                     // of operands, by k-step
+    f32x16 acc[TX][TW] = {};
+    i32x4 xf[kBuffers][TX], wf[kBuffers][TW];
+    int sx[2][TX], sw[2][TW];
+    auto fragments = [&](int slot, auto s) {
+        constexpr int S = s;
 #pragma unroll
-        for (int i = 0; i < TX; ++i) sx_next[i] = (int)xs[i][word * 64];
+        for (int i = 0; i < TW; ++i) wf[S % kBuffers][i] = lds[slot][uw + i][S * 64 + lane];
 #pragma unroll
-        for (int i = 0; i < TW; ++i) sw_next[i] = (int)ws[i][word * 64];
+        for (int i = 0; i < TX; ++i) xf[S % kBuffers][i] = lds[slot][ux + i][S * 64 + lane];
     };
-    // Every load this wave has issued has landed, and after the barrier everybody's; nobody reads the other buffer any
-    // more.  The wait is the builtin so that the compiler knows of it and adds none between the next stage's loads and
-    // the products.
-    auto meet = [&] {
-        __builtin_amdgcn_s_waitcnt(0x0070);                  // vmcnt(0) lgkmcnt(0)
-        asm volatile("s_barrier" ::: "memory");
+    auto fragment_scales = [&](int slot, int to) {
+#pragma unroll
+        for (int i = 0; i < TW; ++i) sw[to][i] = reinterpret_cast<const int *>(lds_scales[slot][uw + i])[lane];
+#pragma unroll
+        for (int i = 0; i < TX; ++i) sx[to][i] = reinterpret_cast<const int *>(lds_scales[slot][ux + i])[lane];
     };
-    auto compute = [&](int t, int s, int step_of_word) {
-        i32x4 xf[TX], wf[TW];
-        const i32x4 *base = lds[t & 1];
-#pragma unroll
-        for (int i = 0; i < TX; ++i) xf[i] = base[(wx + i * 16) * 8 + (read0 ^ (s * 4))];
-#pragma unroll
-        for (int i = 0; i < TW; ++i) wf[i] = base[(kRows + ww + i * 16) * 8 + (read0 ^ (s * 4))];
+    // The loads of the stage to come have landed (those of later ones may be on their way), this wave has read what it
+    // needs of the present one, and after the barrier so have all.
+    auto meet = [&](bool all_issued) {
+        if (all_issued) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kInFlight) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto multiply = [&](auto s) {
+        constexpr int S = s;
 #pragma unroll
         for (int i = 0; i < TX; ++i)
 #pragma unroll
-            for (int j = 0; j < TW; ++j) acc[i][j] = mfma_mx4(wf[j], xf[i], acc[i][j], sw[j], sx[i], step_of_word);
+            for (int j = 0; j < TW; ++j)
+                acc[i][j] = mfma_mx4_32<S>(wf[S % kBuffers][j], xf[S % kBuffers][i], acc[i][j], sw[0][j], sx[0][i]);
+        __builtin_amdgcn_sched_barrier(0);                           // the products stay between the reads they hide
     };
-    issue(0);
-    load_scales(0);
-    for (int t = 0; t < stages; t += 2) {
-        meet();
 #pragma unroll
-        for (int i = 0; i < TX; ++i) sx[i] = sx_next[i];
-#pragma unroll
-        for (int i = 0; i < TW; ++i) sw[i] = sw_next[i];
-        if (t + 1 < stages) issue(t + 1);
-        compute(t, 0, 0);
-        if (2 * t + 1 < steps) compute(t, 1, 1);
-        if (t + 1 < stages) {
-            meet();
-            if (t + 2 < stages) {
-                issue(t + 2);
-                load_scales(t / 2 + 1);
+    for (int t = 0; t < RING - 1; ++t)
+        if (t < stages) issue(t, t);
+    meet(RING - 1 <= stages);
+    if (RING - 1 < stages) issue(RING - 1, RING - 1);
+    static_for<AHEAD>([&](auto s) { fragments(0, s); });
+    fragment_scales(0, 0);
+    int slot = 0;
+    for (int t = 0; t + 1 < stages; ++t) {
+        const int next = slot + 1 == RING ? 0 : slot + 1;
+        static_for<4>([&](auto s) {
+            constexpr int S = s;
+            if constexpr (S == 4 - AHEAD) {
+                meet(t + RING <= stages);
+                fragment_scales(next, 1);
             }
-            compute(t + 1, 0, 2);
-            if (2 * t + 3 < steps) compute(t + 1, 1, 3);
-        }
+            if constexpr (S + AHEAD < 4) fragments(slot, std::integral_constant<int, S + AHEAD>{});
+            else fragments(next, std::integral_constant<int, S + AHEAD - 4>{});
+            if constexpr (S == 4 - AHEAD)
+                if (t + RING < stages) issue(t + RING, slot);
+            multiply(s);
+        });
+#pragma unroll
+        for (int i = 0; i < TX; ++i) sx[0][i] = sx[1][i];
+#pragma unroll
+        for (int i = 0; i < TW; ++i) sw[0][i] = sw[1][i];
+        slot = next;
     }
+    static_for<4>([&](auto s) {
+        constexpr int S = s;
+        if constexpr (S + AHEAD < 4) fragments(slot, std::integral_constant<int, S + AHEAD>{});
+        multiply(s);
+    });
+
+    // Results leave through LDS (free once all waves are past their last fragment; every wave has its own part), 32 rows
+    // at a time, so that a row's features are stored in whole cache lines: straight from the accumulators a lane would
+    // write four features of its own row (measured on 8192 x 8192 outputs in bfloat16: 140 us for the stores alone).
+    // Loops stay rolled where they can: this code runs once per tile, and what it costs is fetching its instructions.
+    constexpr int kWidth = TW * 32, kStride = kWidth + 4, kPack = 16 / sizeof(T), kRowLanes = kWidth / kPack;
+    static_assert((kWaves * 32 * kStride + kFeatures) * 4 <= sizeof(lds), "the waves' parts and the bias fit");
+    __syncthreads();
+    float *mine = reinterpret_cast<float *>(lds) + wave * 32 * kStride;
+    float *bias = reinterpret_cast<float *>(lds) + kWaves * 32 * kStride;
+    if ((int)threadIdx.x < kFeatures) {
+        const int c = col0 + threadIdx.x;
+        bias[threadIdx.x] = a.bias && c < a.n ? load_as_f32(a.bias, a.bias_type, c) : 0.f;
+    }
+    __syncthreads();
+    const int f0 = lane % kRowLanes * kPack, c = col0 + wave / 2 * kWidth + f0;
+    float b[kPack];
 #pragma unroll
-    for (int j = 0; j < TW; ++j) {
-        const int c = col0 + ww + j * 16 + (lane >> 4) * 4;
-        if (c >= a.n) continue;
-        float bias[4];
-        load_bias(a, c, bias);
+    for (int e = 0; e < kPack; ++e) b[e] = bias[wave / 2 * kWidth + f0 + e];
 #pragma unroll
-        for (int i = 0; i < TX; ++i) {
-            const long long r = row0 + wx + i * 16 + (lane & 15);
-            if (r < rows) store_features<T>(a, r, c, acc[i][j], bias);
+    for (int i = 0; i < TX; ++i) {
+#pragma unroll
+        for (int j = 0; j < TW; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f32x4 v = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+                *reinterpret_cast<f32x4 *>(&mine[(lane & 31) * kStride + j * 32 + e * 8 + (lane >> 5) * 4]) = v;
+            }
+#pragma unroll 2
+        for (int q = 0; q < 32 * kRowLanes / 64; ++q) {
+            const int in_tile = q * (64 / kRowLanes) + lane / kRowLanes;
+            const long long r = row0 + (ux + i) * 32 + in_tile;
+            if (r < rows) store_features<T, kPack>(a, r, c, &mine[in_tile * kStride + f0], b);
         }
     }
 }
 
-// Few rows: a block computes RT * 16 rows x 16 features, its eight waves take every eighth word (512 elements) of K
-// with fragments straight from memory and add up in LDS in a fixed order.  FUSED (at most 16 rows, kMx4FusedElements
-// elements): x comes as numbers and every block quantises them into LDS for itself, which saves a launch.
+// Few rows, on 16 x 16 x 128 tiles: a block computes RT * 16 rows x 16 features, its eight waves take every eighth 512
+// elements of K with fragments straight from memory and add up in LDS in a fixed order.  FUSED (at most 16 rows,
+// kMx4FusedElements elements): x comes as numbers and every block quantises them into LDS for itself, which saves a
+// launch.
 constexpr int kMx4FusedElements = 65536;
 constexpr int kRowsWaves = 8;
 
@@ -324,39 +378,43 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mx4_rows_kernel(Mx4Linear a, 
     __shared__ uint32_t xcodes[FUSED ? kMx4FusedElements / 8 : 1];
     __shared__ uint8_t xbytes[FUSED ? kMx4FusedElements / 32 : 1];
     const long long rows = a.row_count && *a.row_count < a.rows ? *a.row_count : a.rows;
-    const long long row0 = (long long)blockIdx.y * (RT * 16);
+    const int feature_tiles = (a.n + 15) / 16;
+    const long long row0 = (long long)(blockIdx.x / feature_tiles) * (RT * 16);
     if (row0 >= rows) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kb = lane >> 4;
-    const int col0 = blockIdx.x * 16;
-    const int steps = a.kp / 128, words = mx4_scale_words(a.kp);
-    const size_t cs = a.kp / 2;
-    const int c = col0 + r16 < a.n ? col0 + r16 : a.n - 1;
-    const uint8_t *wc = a.w_codes + c * cs + kb * 16;
-    const uint32_t *ws = reinterpret_cast<const uint32_t *>(a.w_scales) + (size_t)blockIdx.x * words * 64 + lane;
+    // A wave's loop bounds have to be scalar values: matrix instructions ignore the lane mask, so a branch around one must
+    // be a real branch.
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kb = lane >> 4;
+    const int col0 = blockIdx.x % feature_tiles * 16;
+    const int words = a.kp / 256, chunks = (words + 1) / 2;
+    // This lane's block of a k-step of 128 within a unit: k-step kb / 2 (of 64) of its half of the unit, half kb % 2, so
+    // 16 bytes at `at` (+ 2048 for the unit's second half) and scale bytes kb / 2 and 2 + kb / 2 of one word.
+    auto at = [&](int first) { return (kb >> 1) * 1024 + ((kb & 1) * 32 + (first & 16) + r16) * 16; };
+    auto word_at = [&](int first) { return (kb & 1) * 32 + (first & 16) + r16; };
+    const int shift = 8 * (kb >> 1);
+    const uint8_t *wc = a.w_codes + (size_t)(col0 / 32) * words * 4096 + at(col0);
+    const uint32_t *ws = reinterpret_cast<const uint32_t *>(a.w_scales) + (size_t)(col0 / 32) * words * 64 + word_at(col0);
     const uint8_t *xc[RT];
     const uint32_t *xs[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const long long r = row0 + i * 16 + r16 < rows ? row0 + i * 16 + r16 : rows - 1;
-        const long long tile = row0 + i * 16 < rows ? row0 / 16 + i : (rows - 1) / 16;
         if (FUSED) {
-            xc[i] = reinterpret_cast<const uint8_t *>(xcodes) + r * cs + kb * 16;
+            xc[i] = reinterpret_cast<const uint8_t *>(xcodes) + (r16 < rows ? r16 : rows - 1) * (a.kp / 2) + kb * 16;
         } else {
-            xc[i] = a.x_codes + r * cs + kb * 16;
-            xs[i] = reinterpret_cast<const uint32_t *>(a.x_scales) + tile * words * 64 + lane;
+            const long long first = row0 + i * 16 < rows ? row0 + i * 16 : (rows - 1) / 16 * 16;
+            xc[i] = a.x_codes + first / 32 * words * 4096 + at((int)(first & 16));
+            xs[i] = reinterpret_cast<const uint32_t *>(a.x_scales) + first / 32 * words * 64 + word_at((int)(first & 16));
         }
     }
     i32x4 wf[4];
-    int wsc = 0;
-    auto load_w = [&](int word) {
+    int wsc[2] = {};
+    auto unit_of = [&](int chunk, int s) { return (size_t)(chunk * 2 + s / 2 < words ? chunk * 2 + s / 2 : words - 1); };
+    auto load_w = [&](int chunk) {                   // two units; behind the last one the last again, unused
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int step = word * 4 + s < steps ? word * 4 + s : steps - 1;        // the tail repeats the last step, unused
-            wf[s] = *reinterpret_cast<const i32x4 *>(wc + (size_t)step * 64);
-        }
-        wsc = (int)ws[(size_t)word * 64];
+        for (int s = 0; s < 4; ++s) wf[s] = *reinterpret_cast<const i32x4 *>(wc + unit_of(chunk, s) * 4096 + (s & 1) * 2048);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) wsc[s] = (int)ws[unit_of(chunk, 2 * s) * 64];
     };
-    if (wave < words) load_w(wave);
+    if (wave < chunks) load_w(wave);
     if (FUSED) {
         const int per_row = a.kp / 8, total = (int)rows * per_row;
         for (int i = threadIdx.x; i < (total + 3) / 4 * 4; i += kRowsWaves * 64) {
@@ -383,29 +441,37 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mx4_rows_kernel(Mx4Linear a, 
         __syncthreads();
     }
     f32x4 acc[RT] = {};
-    for (int word = wave; word < words; word += kRowsWaves) {
+    for (int chunk = wave; chunk < chunks; chunk += kRowsWaves) {
         i32x4 w4[4], xf[RT][4];
         int sx[RT][4];
-        const int sw = wsc;
+        const int sw[2] = {wsc[0] >> shift, wsc[1] >> shift};
 #pragma unroll
         for (int s = 0; s < 4; ++s) w4[s] = wf[s];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
+            if (FUSED) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int step = word * 4 + s < steps ? word * 4 + s : steps - 1;
-                xf[i][s] = *reinterpret_cast<const i32x4 *>(xc[i] + (size_t)step * 64);
-                if (FUSED) sx[i][s] = (int)xbytes[(int)(r16 < rows ? r16 : rows - 1) * (a.kp / 32) + step * 4 + kb];
+                for (int s = 0; s < 4; ++s) {
+                    const int step = (int)unit_of(chunk, s) * 2 + (s & 1);
+                    xf[i][s] = *reinterpret_cast<const i32x4 *>(xc[i] + step * 64);
+                    sx[i][s] = (int)xbytes[(int)(r16 < rows ? r16 : rows - 1) * (a.kp / 32) + step * 4 + kb];
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    xf[i][s] = *reinterpret_cast<const i32x4 *>(xc[i] + unit_of(chunk, s) * 4096 + (s & 1) * 2048);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) sx[i][s] = (int)xs[i][unit_of(chunk, 2 * s) * 64] >> shift;
             }
-            if (!FUSED) sx[i][0] = (int)xs[i][(size_t)word * 64];
         }
-        if (word + kRowsWaves < words) load_w(word + kRowsWaves);
+        if (chunk + kRowsWaves < chunks) load_w(chunk + kRowsWaves);
         static_for<4>([&](auto s) {
-            if (word * 4 + s < steps) {
+            constexpr int S = s, BYTE = 2 * (S & 1);
+            if (chunk * 2 + S / 2 < words) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    if (FUSED) acc[i] = mfma_mx4(w4[s], xf[i][s], acc[i], sw >> (8 * s), sx[i][s], 0);
-                    else acc[i] = mfma_mx4(w4[s], xf[i][s], acc[i], sw, sx[i][0], s);
+                    if (FUSED) acc[i] = mfma_mx4_16<BYTE, 0>(w4[S], xf[i][S], acc[i], sw[S / 2], sx[i][S]);
+                    else acc[i] = mfma_mx4_16<BYTE, BYTE>(w4[S], xf[i][S], acc[i], sw[S / 2], sx[i][S / 2]);
                 }
             }
         });
@@ -420,9 +486,13 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mx4_rows_kernel(Mx4Linear a, 
         const long long r = row0 + wave * 16 + r16;
         const int cf = col0 + kb * 4;
         if (r < rows && cf < a.n) {
-            float bias[4];
-            load_bias(a, cf, bias);
-            store_features<T>(a, r, cf, sum, bias);
+            float v[4], bias[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = sum[e];
+                bias[e] = a.bias && cf + e < a.n ? load_as_f32(a.bias, a.bias_type, cf + e) : 0.f;
+            }
+            store_features<T, 4>(a, r, cf, v, bias);
         }
     }
 }
@@ -432,50 +502,80 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mx4_rows_kernel(Mx4Linear a, 
 void launch_mx4_quantize(hipStream_t st, int type, long long rows, int cols, const void *x, long long row_stride,
                          long long col_stride, const int32_t *row_count, uint8_t *codes, uint8_t *scales) {
     const int kp = mx4_padded(cols);
-    const long long tasks = (rows + 15) / 16 * mx4_scale_words(kp);
+    const long long tasks = (rows + 31) / 32 * (kp / 256);
     with_dtype(type, [&](auto t) {
         typedef decltype(t) T;
         mx4_quantize_kernel<T><<<(int)(tasks < 16384 ? tasks : 16384), 256, 0, st>>>(
             static_cast<const T *>(x), rows, cols, kp, row_stride, col_stride, row_count,
-            reinterpret_cast<uint32_t *>(codes), reinterpret_cast<uint32_t *>(scales));
+            reinterpret_cast<uint4 *>(codes), reinterpret_cast<uint32_t *>(scales));
     });
 }
 
 void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, const uint8_t *codes, const uint8_t *scales,
                            void *out) {
     const int kp = mx4_padded(cols);
-    const long long blocks = (rows * (kp / 8) + 255) / 256;
+    const long long tasks = (rows + 31) / 32 * (kp / 256);
     with_dtype(type, [&](auto t) {
         typedef decltype(t) T;
-        mx4_dequantize_kernel<T><<<(int)(blocks < 16384 ? blocks : 16384), 256, 0, st>>>(
-            reinterpret_cast<const uint32_t *>(codes), scales, rows, cols, kp, static_cast<T *>(out));
+        mx4_dequantize_kernel<T><<<(int)(tasks < 16384 ? tasks : 16384), 256, 0, st>>>(
+            reinterpret_cast<const uint4 *>(codes), scales, rows, cols, kp,
+            cols * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0, static_cast<T *>(out));
     });
 }
 
 bool mx4_linear_fuses(long long rows, int cols) { return rows <= 16 && rows * mx4_padded(cols) <= kMx4FusedElements; }
 
+namespace {
+
+// Which kernel multiplies: the cheapest by these costs in microseconds (256 CUs; measured at rows 1 .. 2048 of 1024 x 11520,
+// 4096 x 4096, 8192 x 1024, 512 x 512 and 300 x 16384 layers and at 8192^3, within 20 %):
+//   rows kernel     3 + (1.2 + K / 2300) per 256 blocks of (64 rows x 16 features)
+//   128 x 128, one block per CU (four stages in flight)     3.5 + 0.64 per stage of 256 elements and 256 tiles
+//   128 x 128, two blocks per CU (two stages each)          3.5 + 0.9 per stage and 512 tiles
+//   256 x 256       8 + 1.65 per stage and 256 tiles
+// For example 1024 rows of 11520 -> 1024: 26 / 31 / 35 / 86 us in this order, 2048 rows of 1024 -> 8192: 95 / 30 / 23 / 25.
+template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
+    auto tiles = [&](int r, int f) { return (a.rows + r - 1) / r * ((a.n + f - 1) / f); };
+    auto rounds = [](long long blocks, int at_once) { return (double)((blocks + at_once - 1) / at_once); };
+    const double stages = a.kp / 256;
+    const double rows_cost = 3.0 + rounds(tiles(64, 16), 256) * (1.2 + a.kp / 2300.0);
+    const double one_cost = 3.5 + rounds(tiles(128, 128), 256) * stages * 0.64;
+    const double two_cost = 3.5 + rounds(tiles(128, 128), 512) * stages * 0.9;
+    const double large_cost = 8.0 + rounds(tiles(256, 256), 256) * stages * 1.65;
+    const double tile_cost = one_cost < two_cost ? one_cost : two_cost;
+    if (a.rows <= 16 || rows_cost <= (tile_cost < large_cost ? tile_cost : large_cost)) {
+        auto rows_form = [&](auto rt) {
+            constexpr int RT = rt;
+            mx4_rows_kernel<T, RT, float, false><<<(unsigned)tiles(RT * 16, 16), kRowsWaves * 64, 0, st>>>(a, nullptr, 0, 0, 0);
+        };
+        // as few rows per block as still leave at most a block per CU (128 rows of 11520 -> 1024: 7.2 / 6.2 / 7.6 us with
+        // 16 / 32 / 64 rows, 64 rows 4.8 / 5.6 / 7.3)
+        if (a.rows <= 16 || tiles(16, 16) <= 256) rows_form(std::integral_constant<int, 1>{});
+        else if (a.rows <= 32 || tiles(32, 16) <= 256) rows_form(std::integral_constant<int, 2>{});
+        else rows_form(std::integral_constant<int, 4>{});
+    } else if (large_cost <= tile_cost) {
+        mx4_tile_kernel<T, 4, 4, 2, 1><<<(unsigned)tiles(256, 256), 256, 0, st>>>(a);
+    } else if (two_cost < one_cost) {
+        mx4_tile_kernel<T, 2, 2, 2, 2><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
+    } else {
+        mx4_tile_kernel<T, 2, 2, 4, 3><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
+    }
+}
+
+}  // namespace
+
 void launch_mx4_linear(hipStream_t st, Mx4Linear a, const Mx4Rows *x) {
     with_dtype(a.y_type, [&](auto t) {
         typedef decltype(t) T;
-        a.wide = reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(T)) == 0 && a.y_stride % 4 == 0;
-        const unsigned features = (unsigned)((a.n + 15) / 16);
+        a.wide = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * sizeof(T) % 16 == 0;
         if (x) {
             with_dtype(x->type, [&](auto u) {
                 typedef decltype(u) X;
-                mx4_rows_kernel<T, 1, X, true><<<dim3(features, 1), kRowsWaves * 64, 0, st>>>(
+                mx4_rows_kernel<T, 1, X, true><<<(unsigned)((a.n + 15) / 16), kRowsWaves * 64, 0, st>>>(
                     a, static_cast<const X *>(x->x), x->cols, x->row_stride, x->col_stride);
             });
-        } else if (a.rows <= 16) {
-            mx4_rows_kernel<T, 1, float, false><<<dim3(features, 1), kRowsWaves * 64, 0, st>>>(a, nullptr, 0, 0, 0);
-        } else if (a.rows <= 256) {
-            mx4_rows_kernel<T, 4, float, false><<<dim3(features, (unsigned)((a.rows + 63) / 64)), kRowsWaves * 64, 0, st>>>(
-                a, nullptr, 0, 0, 0);
         } else {
-            auto tiles = [&](int r, int f) { return (a.rows + r - 1) / r * ((a.n + f - 1) / f); };
-            if (tiles(256, 256) >= 256)
-                mx4_tile_kernel<T, 2, 2, 8, 8><<<(unsigned)tiles(256, 256), 256, 0, st>>>(a);
-            else
-                mx4_tile_kernel<T, 2, 2, 4, 4><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
+            launch_product<T>(st, a);
         }
     });
 }

@@ -805,8 +805,8 @@ int check_workspace(const void *workspace, size_t bytes, size_t need) {
 void carve_mx4_rows(Carver &c, int64_t rows, int cols, bool x_quantized, uint8_t *&codes, uint8_t *&scales) {
     codes = scales = nullptr;
     if (x_quantized || mx4_linear_fuses(rows, cols)) return;
-    codes = c.take<uint8_t>((size_t)rows * (mx4_padded(cols) / 2));
-    scales = c.take<uint8_t>(mx4_scale_bytes(rows, cols));
+    codes = c.take<uint8_t>(mx4_units(rows, cols) * 4096);
+    scales = c.take<uint8_t>(mx4_units(rows, cols) * 256);
 }
 
 // Limits of the orthogonalisation kernels' indices.

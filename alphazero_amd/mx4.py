@@ -23,34 +23,28 @@ from . import _lib
 from ._lib import Mx4LinearArgs, check
 from ._tensors import dtype_code, no_grad, on_device, ptr, stream_of
 
-BLOCK = 32      # elements that share a scale
-PAD = 128       # rows are padded with zeros to a multiple of this
+BLOCK = 32                              # elements that share a scale
+UNIT_ROWS, UNIT_COLS = 32, 256          # rows and columns are padded with zeros to whole units
 
 
-def _padded(cols: int) -> int:
-    return -(-cols // PAD) * PAD
-
-
-def _scale_shape(rows: int, cols: int) -> tuple:
-    """Blocks of 256 bytes, one per 16 rows and 512 elements (see nnb_mx4_quantize for the order within)."""
-    return (-(-rows // 16), -(-cols // 512), 256)
+def _units(rows: int, cols: int) -> tuple:
+    return -(-rows // UNIT_ROWS), -(-cols // UNIT_COLS)
 
 
 class MX4Tensor:
     """Quantised numbers of shape `shape`, blocks along the last dimension.
 
-    codes   uint8 [rows, Kp/2], Kp = the last dimension rounded up to 128: two elements a byte, the even one low
-    scales  uint8 [ceil(rows/16), ceil(Kp/512), 256]: exponent + 127 of each block's scale, 255 = not a number, in the
-            order in which the matrix instruction takes them: the scale of row r, block b is byte
-            ((b % 4) * 16 + r % 16) * 4 + (b // 4) % 4 of [r // 16, b // 16]
+    Units of 32 rows x 256 columns (include/nnb.h gives the order within, the matrix instructions'):
+    codes   uint8 [ceil(rows/32), ceil(cols/256), 4096]
+    scales  uint8 [ceil(rows/32), ceil(cols/256), 256], exponent + 127, 255 = not a number
     """
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
         shape = torch.Size(shape)
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError(f"shape {tuple(shape)} has no last dimension to cut into blocks")
-        rows, kp = shape[:-1].numel(), _padded(shape[-1])
-        for name, t, want in (("codes", codes, (rows, kp // 2)), ("scales", scales, _scale_shape(rows, kp))):
+        units = _units(shape[:-1].numel(), shape[-1])
+        for name, t, want in (("codes", codes, units + (4096,)), ("scales", scales, units + (256,))):
             if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous uint8 of shape {want}, got {t.dtype} {tuple(t.shape)}")
         if codes.device != scales.device:
@@ -66,7 +60,7 @@ class MX4Tensor:
         with on_device(self.codes):
             out = torch.empty(self.shape, dtype=dtype, device=self.device)
             code = dtype_code(out, "dtype")
-            check(_lib.load().nnb_mx4_dequantize(stream_of(self.codes), code, self.codes.shape[0], self.shape[-1],
+            check(_lib.load().nnb_mx4_dequantize(stream_of(self.codes), code, self.shape[:-1].numel(), self.shape[-1],
                                                  ptr(self.codes), ptr(self.scales), ptr(out)), "nnb_mx4_dequantize")
         return out
 
@@ -99,11 +93,11 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x of shape {tuple(x.shape)} has no last dimension to cut into blocks")
     with on_device(x):
-        v = _rows_view(x.detach())
+        v = _rows_view(x)
         rows, cols = v.shape
-        kp = _padded(cols)
-        codes = torch.empty((rows, kp // 2), dtype=torch.uint8, device=x.device)
-        scales = torch.empty(_scale_shape(rows, kp), dtype=torch.uint8, device=x.device)
+        units = _units(rows, cols)
+        codes = torch.empty(units + (4096,), dtype=torch.uint8, device=x.device)
+        scales = torch.empty(units + (256,), dtype=torch.uint8, device=x.device)
         check(_lib.load().nnb_mx4_quantize(stream_of(x), code, rows, cols, ptr(v), v.stride(0), v.stride(1), ptr(codes),
                                            ptr(scales)), "nnb_mx4_quantize")
     return MX4Tensor(codes, scales, x.shape)
@@ -142,16 +136,16 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
         elif tuple(out.shape) != y_shape or out.dtype != out_dtype:
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, expected {out_dtype} {y_shape}")
         no_grad("mx4.linear", out)
-        y_stride = _row_stride(out, n)
+        y_stride = n if out.is_contiguous() else _row_stride(out, n)
         args = Mx4LinearArgs()
         args.rows, args.cols, args.out_features = torch.Size(y_shape[:-1]).numel(), cols, n
         if quantized:
             args.x_codes, args.x_scales = ptr(x.codes), ptr(x.scales)
         else:
-            v = _rows_view(x.detach())
+            v = _rows_view(x)
             args.x, args.x_row_stride, args.x_col_stride = ptr(v), v.stride(0), v.stride(1)
         args.w_codes, args.w_scales = ptr(weight.codes), ptr(weight.scales)
-        b = bias.detach().contiguous() if bias is not None else None
+        b = bias.contiguous() if bias is not None else None
         args.bias = ptr(b) if b is not None else None
         args.y, args.y_row_stride = ptr(out), y_stride
         args.x_type, args.y_type, args.relu = x_type, dtype_code(out, "out"), int(bool(relu))
@@ -160,6 +154,7 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
         nbytes = C.c_size_t()
         check(lib.nnb_mx4_linear_workspace_bytes(args.rows, cols, n, int(quantized), C.byref(nbytes)),
               "nnb_mx4_linear_workspace_bytes")
-        workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
-        check(lib.nnb_mx4_linear(stream_of(out), C.byref(args), ptr(workspace), nbytes.value), "nnb_mx4_linear")
+        workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=device) if nbytes.value else None
+        check(lib.nnb_mx4_linear(stream_of(out), C.byref(args), ptr(workspace) if workspace is not None else None, nbytes.value),
+              "nnb_mx4_linear")
     return out

@@ -389,12 +389,16 @@ enum nnb_dtype { NNB_F32 = 0, NNB_F16 = 1, NNB_BF16 = 2 };
 /* 4-bit floats with shared scales.  A row of `cols` numbers is cut into blocks of 32; a block shares the scale 2^e,
  * e = floor(log2 max|x|) - 2 clamped to [-127, 127] and stored as the byte e + 127; an element is the e2m1 code of
  * x / 2^e (values 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), to nearest with ties to the even code and beyond 6
- * to 6.  A block that holds an infinity or a NaN gets the byte 255 and reads as NaN.  Rows are padded with zeros to
- * Kp = the next multiple of 128: codes_out [rows][Kp/2], 16-byte aligned, element 2i in the low half of byte i.
- * scales_out, 16-byte aligned, holds ceil(rows/16) * ceil(Kp/512) blocks of 256 bytes: the scale of row r, block b is
- * byte ((b % 4) * 16 + r % 16) * 4 + (b / 4) % 4 of block (r / 16) * ceil(Kp/512) + b / 16 (the order in which the matrix
- * instruction takes them; bytes that belong to no row or block are written too).
- * x [rows][cols] of type x_type (nnb_dtype), element (r, c) at x[r*row_stride + c*col_stride] (strides in elements, may
+ * to 6.  A block that holds an infinity or a NaN gets the byte 255 and reads as NaN.
+ * Layout: units of 32 rows x 256 columns (both padded with zeros), [ceil(rows/32)][ceil(cols/256)], codes_out 4096 bytes
+ * and scales_out 256 bytes each, 16-byte aligned.  Block b (of 32) of row r lies in unit (r/32, b/8): its codes at byte
+ * ((b/2 % 4) * 64 + (b % 2) * 32 + r % 32) * 16, element 2i in the low half of byte i, its scale at byte
+ * ((b % 2) * 32 + r % 32) * 4 + b/2 % 4 (the order in which the matrix instructions take them). */
+/* NNB_MX4_UNITS(rows, cols) * NNB_MX4_CODE_BYTES and * NNB_MX4_SCALE_BYTES are the two arrays' sizes. */
+#define NNB_MX4_UNITS(rows, cols) ((((rows) + 31) / 32) * (((cols) + 255) / 256))
+#define NNB_MX4_CODE_BYTES 4096
+#define NNB_MX4_SCALE_BYTES 256
+/* x [rows][cols] of type x_type (nnb_dtype), element (r, c) at x[r*row_stride + c*col_stride] (strides in elements, may
  * be 0 or negative).  rows = 0 is a no-op; cols in [1, 2^24], rows at most 2^31 - 1. */
 int nnb_mx4_quantize(void *stream, int x_type, int64_t rows, int64_t cols, const void *x, int64_t row_stride,
                      int64_t col_stride, uint8_t *codes_out, uint8_t *scales_out);

@@ -56,10 +56,11 @@ def test_quantize_equals_its_definition(shape, dtype):
     x = (torch.randn(shape, generator=g) * torch.exp(3 * torch.randn(shape[0], 1, generator=g))).to(getattr(torch, dtype))
     q = mx4.quantize(x.cuda())
     _same(q.dequantize().cpu(), quantized(x.double().numpy()))
-    kp = -(-shape[1] // 128) * 128
-    assert q.codes.shape == (shape[0], kp // 2) and q.scales.shape == (-(-shape[0] // 16), -(-kp // 512), 256)
-    blocks = -(-shape[1] // 32)
-    assert not q.codes[:, blocks * 16:].any()                          # padding multiplies as zero
+    units = (-(-shape[0] // 32), -(-shape[1] // 256))
+    assert q.codes.shape == units + (4096,) and q.scales.shape == units + (256,)
+    # padding multiplies as zero: [unit, 2 k-steps of 64.., half, row, 16 bytes] back to rows
+    full = q.codes.reshape(units + (4, 2, 32, 16)).permute(0, 4, 1, 2, 3, 5).reshape(units[0] * 32, units[1] * 128).cpu()
+    assert not full[shape[0]:].any() and not full[:, -(-shape[1] // 32) * 16:].any()
 
 
 def test_quantize_every_half_and_every_bfloat16():

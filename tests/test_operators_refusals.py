@@ -70,10 +70,10 @@ def test_mx4_python_refusals():
     import torch
     from alphazero_amd import mx4
     from alphazero_amd._lib import NnbError
-    codes, scales = torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(1, 1, 256, dtype=torch.uint8)
+    codes, scales = torch.zeros(1, 1, 4096, dtype=torch.uint8), torch.zeros(1, 1, 256, dtype=torch.uint8)
     w = mx4.MX4Tensor(codes, scales, (8, 100))
-    for bad in ((codes, scales, (8, 300)), (codes, scales, (7, 100)), (codes.int(), scales, (8, 100)), (codes, scales, ()),
-                (codes, scales, (8, 0)), (codes.t().contiguous().t(), scales, (8, 100)), (codes, scales[:, :, :128], (8, 100))):
+    for bad in ((codes, scales, (8, 300)), (codes, scales, (33, 100)), (codes.int(), scales, (8, 100)), (codes, scales, ()),
+                (codes, scales, (8, 0)), (codes.expand(2, 1, 4096), scales.expand(2, 1, 256), (40, 100)), (codes, scales[:, :, :128], (8, 100))):
         with pytest.raises(ValueError):
             mx4.MX4Tensor(*bad)
     with pytest.raises(ValueError):
