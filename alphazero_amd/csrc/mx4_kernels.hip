@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include "kernels.h"
+#include "lds_loads.h"
 #include "mfma_tiles.h"
 #include "numeric_types.h"
 
@@ -198,15 +199,6 @@ __device__ __forceinline__ void store_features(const Mx4Linear &a, long long r, 
 // the ring is free for the stage RING further on, and the next one's operands are read while the last AHEAD k-steps
 // multiply.
 
-// 16 bytes a lane from base + offset to 1 KB of LDS at `to` (both uniform).  In assembly because the compiler, which
-// cannot tell the ring's stages apart, would wait for every load in flight before every read of LDS; the kernel's own
-// wait in front of its barrier is the only one needed.
-__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t offset, void *to) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)to;
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :: "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
-}
-
 template <typename T, int TX, int TW, int RING, int AHEAD>
 __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
     constexpr int kWaves = 4, kRows = 2 * TX * 32, kFeatures = 2 * TW * 32;
@@ -282,8 +274,8 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
     // The loads of the stage to come have landed (those of later ones may be on their way), this wave has read what it
     // needs of the present one, and after the barrier so have all.
     auto meet = [&](bool all_issued) {
-        if (all_issued) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kInFlight) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (all_issued) wait_and_meet<kInFlight>();
+        else wait_and_meet<0>();
     };
     auto multiply = [&](auto s) {
         constexpr int S = s;

@@ -11,6 +11,7 @@
 #include <cstring>
 #include <memory>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "../../include/nnb.h"
@@ -1447,6 +1448,12 @@ int nnb_orthogonalize(void *stream, int type, int64_t batch, int64_t rows, int64
     it.x_bs = x_strides[0]; it.x_rs = x_strides[1]; it.x_cs = x_strides[2];
     it.o_bs = out_strides[0]; it.o_rs = out_strides[1]; it.o_cs = out_strides[2];
     it.rows = (int)rows; it.cols = (int)cols; it.batch = (int)batch;
+    // orthogonalising the transpose is the same thing: the columns get the smaller stride, as the kernels like it
+    if (std::llabs(it.x_rs) < std::llabs(it.x_cs)) {
+        std::swap(it.rows, it.cols);
+        std::swap(it.x_rs, it.x_cs);
+        std::swap(it.o_rs, it.o_cs);
+    }
     ortho_groups(&it, 1, [&](OrthoGroup &g) {
         g.ws = static_cast<unsigned char *>(workspace);
         launch_orthogonalize(static_cast<hipStream_t>(stream), g, p);

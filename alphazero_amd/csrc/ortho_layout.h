@@ -5,15 +5,17 @@
 
 namespace nnb {
 
-constexpr int kOrthoTile = 64;           // matrices are padded with zeros to whole tiles
+constexpr int kOrthoPad = 64;            // matrices are padded with zeros to a multiple of this
 constexpr int kOrthoItems = 20;          // matrices (or equal batches of them) per group of launches
 constexpr int kOrthoMaxSteps = 16;
 constexpr int kOrthoSegment = 3;         // Newton-Schulz steps between two looks at the matrix itself
-constexpr int kOrthoNormParts = 256;     // partial sums of squares per matrix
+constexpr int kOrthoNormParts = 1024;    // partial sums of squares per matrix at most
 
-constexpr int ortho_padded(int v) { return (v + kOrthoTile - 1) / kOrthoTile * kOrthoTile; }
+__host__ __device__ constexpr int ortho_padded(int v) { return (v + kOrthoPad - 1) / kOrthoPad * kOrthoPad; }
+__host__ __device__ constexpr int ortho_min(int a, int b) { return a < b ? a : b; }
+__host__ __device__ constexpr int ortho_max(int a, int b) { return a > b ? a : b; }
 
-// One matrix, or `batch` equal ones.  X is the matrix laid on its long side: m <= n, transposed if rows > cols.
+// One matrix, or `batch` equal ones.
 struct OrthoItem {
     const void *x;               // the matrix, or the gradient of an optimiser step
     void *out;                   // the result, or the new weights
@@ -28,19 +30,38 @@ struct OrthoItem {
     float scale;                 // optimiser step: lr * max(1, rows / cols)^(1/2)
 };
 
-struct OrthoGroup {
-    OrthoItem item[kOrthoItems];
+// What the products need of an item.
+struct OrthoShape {
+    size_t ws, ws_stride;
+    int rows, cols, batch;
+};
+
+template <typename Item> struct OrthoGroupOf {
+    Item item[kOrthoItems];
     int first[kOrthoItems + 1];  // first block of every item in the launch at hand
     int count;
     unsigned char *ws;
 };
+typedef OrthoGroupOf<OrthoItem> OrthoGroup;
+typedef OrthoGroupOf<OrthoShape> OrthoShapes;
 
-// Areas of one matrix's workspace.  "Planes" are a hi and a lo half per value: value * 2^k = hi + lo.
+// Areas of one matrix's workspace.  X is the matrix laid on its long side (m <= n, transposed if rows > cols).  A matrix
+// [R][K] of float32-faithful operands (value * 2^k = hi + lo, two halves) takes 4 R K bytes: units of 16 rows x 32 k,
+// [R / 16][K / 32], 1 KB of hi and 1 KB of lo halves, each in the order in which a 16 x 16 x 32 matrix instruction takes
+// them: lane l holds k 8 (l / 16) .. + 7 of row l % 16.
 struct OrthoArea {
     int m, n, mp, np;
-    size_t parts, x, xt[2], sq[6], bytes;
+    int tile;                    // side of the Gram product's tiles
+    int splits;                  // parts that the long side is cut into for it
+    int parts_used;              // partial sums of squares
+    size_t parts, x, xt0, sq0, partial, bytes;
+    size_t wide, square;         // bytes of an m x n and of an m x m matrix
+    __host__ __device__ size_t xt(int i) const { return xt0 + i * wide; }
+    __host__ __device__ size_t sq(int i) const { return sq0 + i * square; }
 };
 enum OrthoSquare { SQ_A0 = 0, SQ_A1 = 1, SQ_T = 2, SQ_P = 3, SQ_Q0 = 4, SQ_Q1 = 5 };
+
+__host__ __device__ constexpr int ortho_triangle(int t) { return t * (t + 1) / 2; }
 
 __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     OrthoArea a;
@@ -48,12 +69,21 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     a.n = rows < cols ? cols : rows;
     a.mp = ortho_padded(a.m);
     a.np = ortho_padded(a.n);
-    const size_t wide = (size_t)a.mp * a.np * 4, square = (size_t)a.mp * a.mp * 4;
+    a.tile = a.mp > 256 ? 128 : 64;
+    // enough blocks for two per CU, at least 256 of the long side each
+    const int tiles = ortho_triangle((a.mp + a.tile - 1) / a.tile);
+    a.splits = ortho_max(1, ortho_min(512 / tiles, a.np / 256));
+    const long long count = (long long)rows * cols;
+    a.parts_used = (int)(count / 4096 < 1 ? 1 : count / 4096 < kOrthoNormParts ? count / 4096 : kOrthoNormParts);
+    a.wide = (size_t)a.mp * a.np * 4;
+    a.square = (size_t)a.mp * a.mp * 4;
     size_t o = 0;
-    a.parts = o; o += kOrthoNormParts * sizeof(double);
-    a.x = o; o += wide;
-    for (int i = 0; i < 2; ++i) { a.xt[i] = o; o += wide; }
-    for (int i = 0; i < 6; ++i) { a.sq[i] = o; o += square; }
+    a.parts = o; o += (size_t)kOrthoNormParts * sizeof(double);
+    a.x = o; o += a.wide;
+    a.xt0 = o; o += 2 * a.wide;
+    a.sq0 = o; o += 6 * a.square;
+    a.partial = o;
+    if (a.splits > 1) o += (size_t)a.splits * tiles * a.tile * a.tile * sizeof(float);
     a.bytes = o;
     return a;
 }
