@@ -422,15 +422,267 @@ __global__ __launch_bounds__(256, 2) void ortho_finish_kernel(OrthoShapes g, Ort
     product<T, STAGE_FINISH, TB, RING>(g, p, s, &items);
 }
 
-// Largest magnitudes on [0, rho]: of p, of l p(l) and of l p(l)^2.
+// ------------------------------------------------------------------------------------- matrices in one block's LDS
+//
+// A square's results come four rows of one column to a lane: eight bytes of hi and of lo halves of the transposed
+// matrix's units, which for a symmetric matrix is the matrix.
+
+// Address of lane (row r, k .. k + 3) in units of a matrix with K columns.
+__device__ __forceinline__ int unit_bytes(int r, int k, int kdim) {
+    return ((r / 16) * (kdim / 32) + k / 32) * 2048 + ((k % 32 / 8) * 16 + r % 16) * 16 + k % 8 * 2;
+}
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void put4(unsigned char *unit, f32x4 v) {
+    half4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = (f16_t)v[e];
+        lo[e] = (f16_t)(v[e] - (float)hi[e]);
+    }
+    *reinterpret_cast<half4 *>(unit) = hi;
+    *reinterpret_cast<half4 *>(unit + 1024) = lo;
+}
+__device__ __forceinline__ f32x4 get4(const unsigned char *unit) {
+    const half4 hi = *reinterpret_cast<const half4 *>(unit), lo = *reinterpret_cast<const half4 *>(unit + 1024);
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
+    return v;
+}
+// acc += rows rb of F times rows cb .. cb + N - 1 (blocks of 16) of G, both units with K columns; G may lie in global memory.
+template <int N>
+__device__ __forceinline__ void multiply_units(const unsigned char *f, const unsigned char *g, int rb, int cb, int kdim, f32x4 (&acc)[N]) {
+    const int lane = threadIdx.x & 63, ku = kdim / 32;
+    for (int k = 0; k < ku; ++k) {
+        const unsigned char *fu = f + (rb * ku + k) * 2048 + lane * 16;
+        const half8 fh = *reinterpret_cast<const half8 *>(fu), fl = *reinterpret_cast<const half8 *>(fu + 1024);
+        half8 gh[N], gl[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const unsigned char *gu = g + ((cb + j) * ku + k) * 2048 + lane * 16;
+            gh[j] = *reinterpret_cast<const half8 *>(gu);
+            gl[j] = *reinterpret_cast<const half8 *>(gu + 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, gh[j], acc[j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, gl[j], acc[j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, gh[j], acc[j], 0, 0, 0);
+    }
+}
+
+// A whole matrix (m <= 64, n <= NP) in one block of eight waves: the twenty launches of the long way would cost a small
+// matrix several times what it computes.
+template <typename T, int NP>
+__global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoParams p, OrthoSmallSteps steps) {
+    constexpr int M = kOrthoSmallRows, kWide = M * NP * 4, kSquare = M * M * 4, TN = NP / 32;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kWide + 2 * kSquare];
+    unsigned char *x = lds, *xt = lds + kWide, *sq_a = lds + 2 * kWide, *sq_b = sq_a + kSquare;
+    int batch;
+    const OrthoItem &it = g.item[find_item(g, blockIdx.x, batch)];
+    const bool tall = it.rows > it.cols;
+    const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const T *src = static_cast<const T *>(it.x) + batch * it.x_bs;
+    const long long rs = tall ? it.x_cs : it.x_rs, cs = tall ? it.x_rs : it.x_cs;
+    // X is u or its transpose; a thread takes eight columns of a row
+    constexpr int kPer = M * NP / 8 / 512;
+    float u[kPer][8];
+    double sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int at = q * 512 + tid, i = at / (NP / 8), j = at % (NP / 8) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v = 0.f;
+            if (i < m && j + e < n) {
+                v = to_f32(src[i * rs + (j + e) * cs]);
+                if (p.muon) {
+                    const size_t o = tall ? (size_t)(j + e) * it.cols + i : (size_t)i * it.cols + j + e;
+                    const float m_new = p.mu * it.momentum[o] + v;
+                    it.momentum_out[o] = m_new;
+                    v = update_of(p, v, m_new);
+                }
+            }
+            u[q][e] = v;
+            sum += (double)v * (double)v;
+        }
+    }
+    double *wave_sum = reinterpret_cast<double *>(sq_a);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) wave_sum[wave] = sum;
+    __syncthreads();
+    double norm = 0.0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) norm += wave_sum[w];
+    const double scale = (double)steps.pow_kx / (sqrt(norm) + p.eps);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int at = q * 512 + tid, i = at / (NP / 8), j = at % (NP / 8) * 8;
+        float v[8];
+        half8 lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)((double)u[q][e] * scale);
+        const half8 hi = pack_hi(v, lo);
+        unsigned char *row = x + unit_bytes(i, j, NP);
+        *reinterpret_cast<half8 *>(row) = hi;
+        *reinterpret_cast<half8 *>(row + 1024) = lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            unsigned char *turned = xt + unit_bytes(j + e, i, M);
+            *reinterpret_cast<f16_t *>(turned) = hi[e];
+            *reinterpret_cast<f16_t *>(turned + 1024) = lo[e];
+        }
+    }
+    __syncthreads();
+    const int rb = wave / 2, cb = wave % 2 * 2, nb = wave % 2 * TN;     // 16-row block; first 16-column block of a square, of X
+    const int row = rb * 16 + (lane >> 4) * 4, col = lane & 15;         // a lane's four rows and its column in a block
+    for (int s = 0; s < p.steps; ++s) {
+        const OrthoSmallStep st = steps.step[s];
+        f32x4 a[2] = {};
+        multiply_units<2>(x, x, rb, cb, NP, a);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) put4(sq_a + unit_bytes((cb + j) * 16 + col, row, M), a[j] * st.a_scale);
+        __syncthreads();
+        f32x4 b[2] = {};
+        multiply_units<2>(sq_a, sq_a, rb, cb, M, b);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int o = unit_bytes((cb + j) * 16 + col, row, M);
+            put4(sq_b + o, get4(sq_a + o) * st.b + b[j] * st.c);
+        }
+        __syncthreads();
+        f32x4 y[TN] = {};
+        multiply_units<TN>(sq_b, xt, rb, nb, M, y);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) y[j] = get4(xt + unit_bytes((nb + j) * 16 + col, row, M)) * st.ax + y[j] * st.y_scale;
+        if (s + 1 < p.steps) {
+            __syncthreads();                                            // everybody has read the old X
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int c = (nb + j) * 16 + col;
+                unsigned char *turned = xt + unit_bytes(c, row, M);
+                put4(turned, y[j]);
+                const half4 hi = *reinterpret_cast<half4 *>(turned), lo = *reinterpret_cast<half4 *>(turned + 1024);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unsigned char *straight = x + unit_bytes(row + e, c, NP);
+                    *reinterpret_cast<f16_t *>(straight) = hi[e];
+                    *reinterpret_cast<f16_t *>(straight + 1024) = lo[e];
+                }
+            }
+            __syncthreads();
+            continue;
+        }
+        T *out = static_cast<T *>(it.out) + batch * it.o_bs;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = row + e, c = (nb + j) * 16 + col;
+                if (i >= m || c >= n) continue;
+                const int ur = tall ? c : i, uc = tall ? i : c;
+                float v = y[j][e];
+                if (p.muon) v = to_f32(static_cast<const T *>(it.weight)[(size_t)ur * it.cols + uc]) * p.decay - it.scale * v;
+                out[ur * it.o_rs + uc * it.o_cs] = from_f32<T>(v);
+            }
+    }
+}
+
+// All products of a segment for a matrix with m <= 128: A comes from memory, Q goes there, a block of eight waves each;
+// A (then T, then the next A) and P stay in LDS, Q is read back from memory where it is multiplied.
+template <int MP>
+__global__ __launch_bounds__(512) void ortho_segment_kernel(OrthoShapes g, OrthoSegmentSteps steps, int a_from, int q_to) {
+    constexpr int kSquare = MP * MP * 4, RB = MP / 64, CB = MP / 32;     // a wave's blocks of 16: RB rows x CB columns
+    __shared__ __attribute__((aligned(16))) unsigned char sq_a[kSquare], sq_p[kSquare];
+    int batch;
+    const OrthoShape &it = g.item[find_item(g, blockIdx.x, batch)];
+    const OrthoArea area = ortho_area(it.rows, it.cols);
+    if (area.mp != MP) return;                                           // the other size's launch takes it
+    unsigned char *ws = g.ws + it.ws + batch * it.ws_stride;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rb = wave / 2 * RB, cb = wave % 2 * CB;
+    const int row = (lane >> 4) * 4, col = lane & 15;
+    for (int i = tid * 16; i < kSquare; i += 512 * 16)
+        *reinterpret_cast<u32x4 *>(sq_a + i) = *reinterpret_cast<const u32x4 *>(ws + area.sq(a_from) + i);
+    __syncthreads();
+    // Q alternates between two places so that the last one is q_to
+    int q = (steps.count & 1) ? q_to : (q_to == SQ_Q0 ? SQ_Q1 : SQ_Q0);
+    f32x4 acc[RB][CB];
+    auto product = [&](const unsigned char *f, const unsigned char *h) {
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+#pragma unroll
+            for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            multiply_units<CB>(f, h, rb + i, cb, MP, acc[i]);
+        }
+    };
+    auto store = [&](unsigned char *to, float scale) {
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+#pragma unroll
+            for (int j = 0; j < CB; ++j) put4(to + unit_bytes((cb + j) * 16 + col, (rb + i) * 16 + row, MP), acc[i][j] * scale);
+    };
+    for (int s = 0; s < steps.count; ++s) {
+        const OrthoSegmentStep &st = steps.step[s];
+        product(sq_a, sq_a);
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+#pragma unroll
+            for (int j = 0; j < CB; ++j) {
+                const int r = (rb + i) * 16 + row, c = (cb + j) * 16 + col, o = unit_bytes(c, r, MP);
+                f32x4 v = get4(sq_a + o) * st.b + acc[i][j] * st.c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += r + e == c ? st.a : 0.f;
+                put4(sq_p + o, v);
+                if (s == 0) put4(ws + area.sq(q) + o, v);                // the first step's P is Q
+            }
+        __syncthreads();
+        if (s > 0) {
+            const int next = q == SQ_Q0 ? SQ_Q1 : SQ_Q0;
+            product(sq_p, ws + area.sq(q));
+            store(ws + area.sq(next), st.q_scale);
+            q = next;
+        }
+        if (s + 1 < steps.count) {
+            product(sq_p, sq_a);
+            __syncthreads();                                             // everybody has read A
+            store(sq_a, st.t_scale);
+            __syncthreads();
+            product(sq_a, sq_p);
+            __syncthreads();                                             // everybody has read T
+            store(sq_a, st.a_scale);
+        }
+        __syncthreads();
+    }
+}
+
+// Largest magnitudes on [0, rho]: of p, of l p(l) and of l p(l)^2, p(l) = c0 + c1 l + c2 l^2.  They lie at the ends or where a
+// derivative vanishes: p', p + l p' = c0 + 2 c1 l + 3 c2 l^2, and p + 2 l p' = c0 + 3 c1 l + 5 c2 l^2 (or p itself, a zero).
 void polynomial_bounds(const float *c, double rho, double &p_max, double &lp_max, double &lpp_max) {
     p_max = lp_max = lpp_max = 0.0;
-    for (int i = 0; i <= 4096; ++i) {
-        const double l = rho * i / 4096.0, v = std::fabs(c[0] + c[1] * l + c[2] * l * l);
+    auto at = [&](double l) {
+        if (!(l >= 0.0 && l <= rho)) return;
+        const double v = std::fabs(c[0] + c[1] * l + c[2] * l * l);
         p_max = std::fmax(p_max, v);
         lp_max = std::fmax(lp_max, l * v);
         lpp_max = std::fmax(lpp_max, l * v * v);
-    }
+    };
+    auto roots = [&](double q0, double q1, double q2) {          // of q0 + q1 l + q2 l^2
+        if (q2 == 0.0) { if (q1 != 0.0) at(-q0 / q1); return; }
+        const double d = q1 * q1 - 4.0 * q2 * q0;
+        if (d < 0.0) return;
+        at((-q1 + std::sqrt(d)) / (2.0 * q2));
+        at((-q1 - std::sqrt(d)) / (2.0 * q2));
+    };
+    at(0.0);
+    at(rho);
+    roots(c[1], 2.0 * c[2], 0.0);
+    roots(c[0], 2.0 * c[1], 3.0 * c[2]);
+    roots(c[0], 3.0 * c[1], 5.0 * c[2]);
 }
 
 // Largest k <= 14 with bound * 2^k <= 2^15 (halves reach 2^16: the rest is room for rounding).
@@ -456,12 +708,60 @@ bool ortho_coefficients_ok(const OrthoParams &p) {
     return true;
 }
 
+namespace {
+
+void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
+    OrthoSmallSteps steps = {};
+    double rho = 1.0;
+    int kx = exponent_for(1.0), blocks = 0, widest = 0;
+    steps.pow_kx = (float)std::ldexp(1.0, kx);
+    for (int i = 0; i < p.steps; ++i) {
+        const float *c = p.coef[i];
+        double p_max, lp_max, lpp_max;
+        polynomial_bounds(c, rho * 1.001, p_max, lp_max, lpp_max);
+        // |b l + c l^2| <= |p| + |a|
+        const int ka = exponent_for(rho), kb = exponent_for(p_max + std::fabs(c[0]));
+        const int kn = i + 1 < p.steps ? exponent_for(std::sqrt(std::fmax(lpp_max, 1e-6))) : 0;
+        OrthoSmallStep &s = steps.step[i];
+        s.a_scale = (float)std::ldexp(1.0, ka - 2 * kx);
+        s.b = (float)std::ldexp(c[1], kb - ka);
+        s.c = (float)std::ldexp(c[2], kb - 2 * ka);
+        s.ax = (float)std::ldexp(c[0], kn - kx);
+        s.y_scale = (float)std::ldexp(1.0, kn - kb - kx);
+        kx = kn;
+        rho = std::fmax(lpp_max, 1e-6);
+    }
+    for (int i = 0; i < g.count; ++i) {
+        g.first[i] = blocks;
+        blocks += g.item[i].batch;
+        widest = ortho_max(widest, ortho_max(g.item[i].rows, g.item[i].cols));
+    }
+    g.first[g.count] = blocks;
+    with_dtype(p.type, [&](auto type) {
+        typedef decltype(type) T;
+        if (widest <= 64) ortho_small_kernel<T, 64><<<blocks, 512, 0, st>>>(g, p, steps);
+        else if (widest <= 128) ortho_small_kernel<T, 128><<<blocks, 512, 0, st>>>(g, p, steps);
+        else ortho_small_kernel<T, 256><<<blocks, 512, 0, st>>>(g, p, steps);
+    });
+}
+
+}  // namespace
+
 void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
+    bool small = true, segments = true;
+    for (int i = 0; i < g.count; ++i) {
+        small &= ortho_is_small(g.item[i].rows, g.item[i].cols);
+        segments &= ortho_min(g.item[i].rows, g.item[i].cols) <= kOrthoSegmentRows;
+    }
+    if (small) {
+        launch_small(st, g, p);
+        return;
+    }
     OrthoShapes shapes = {};
     shapes.count = g.count;
     shapes.ws = g.ws;
     long long symmetric128 = 0, full128 = 0;
-    bool reduce = false, large_gram = false;
+    bool any64 = false, any128 = false, gram_of[2] = {}, reduce_of[2] = {};
     for (int i = 0; i < g.count; ++i) {
         const OrthoItem &it = g.item[i];
         const OrthoArea a = ortho_area(it.rows, it.cols);
@@ -469,8 +769,10 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         const int mt = (a.mp + 127) / 128, nt = (a.np + 127) / 128;
         symmetric128 += (long long)it.batch * ortho_triangle(mt);
         full128 += (long long)it.batch * mt * nt;
-        reduce |= a.splits > 1;
-        large_gram |= a.tile == 128;
+        any64 |= a.mp == 64;
+        any128 |= a.mp == 128;
+        gram_of[a.tile == 128] = true;
+        reduce_of[a.tile == 128] |= a.splits > 1;
     }
     // Tiles of 128 need half the LDS traffic, tiles of 64 give four times the blocks: 128 where they fill the chip.
     const int symmetric_tile = symmetric128 >= 200 ? 128 : 64, full_tile = full128 >= 200 ? 128 : 64;
@@ -491,16 +793,17 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     };
     auto launch = [&](auto stage, bool large, dim3 grid, const StageArgs &s) {
         constexpr int STAGE = stage;
-        if (grid.x == 0) return;
         if (large) ortho_product_kernel<STAGE, 4, 2><<<grid, 256, 0, st>>>(shapes, p, s);
         else ortho_product_kernel<STAGE, 2, 4><<<grid, 256, 0, st>>>(shapes, p, s);
     };
     auto gram = [&](const StageArgs &s) {
         for (int large = 0; large < 2; ++large) {
+            if (!gram_of[large]) continue;
             auto mine = [&](const OrthoArea &a) { return (a.tile == 128) == (large == 1); };
             int n = blocks(shapes, [&](const OrthoArea &a, const OrthoItem &) {
                 return mine(a) ? ortho_triangle((a.mp + a.tile - 1) / a.tile) * a.splits : 0; });
             launch(std::integral_constant<int, STAGE_GRAM>{}, large, n, s);
+            if (!reduce_of[large]) continue;
             n = blocks(shapes, [&](const OrthoArea &a, const OrthoItem &) {
                 return mine(a) && a.splits > 1 ? ortho_triangle((a.mp + a.tile - 1) / a.tile) : 0; });
             launch(std::integral_constant<int, STAGE_REDUCE>{}, large, n, s);
@@ -523,6 +826,9 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
             gram(s);
             n = squares();
             double q_max = 1.0;
+            OrthoSegmentSteps all = {};
+            all.count = len;
+            const int a_from = cur;
             for (int i = 0; i < len; ++i) {
                 const float *c = p.coef[s0 + i];
                 double p_max, lp_max, lpp_max;
@@ -531,7 +837,8 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 const int kp = exponent_for(p_max), pout = i == 0 ? SQ_Q0 : SQ_P;
                 s.f = cur; s.out[0] = pout;
                 s.a = (float)std::ldexp(c[0], kp); s.b = (float)std::ldexp(c[1], kp - ka); s.c = (float)std::ldexp(c[2], kp - 2 * ka);
-                launch(std::integral_constant<int, STAGE_POLY>{}, symmetric_tile == 128, n, s);
+                all.step[i].a = s.a; all.step[i].b = s.b; all.step[i].c = s.c;
+                if (!segments) launch(std::integral_constant<int, STAGE_POLY>{}, symmetric_tile == 128, n, s);
                 q_max *= p_max;
                 // T = P A and Q <- P Q in one launch, then A <- T P
                 int pair = 0;
@@ -539,25 +846,30 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 const int kt = exponent_for(lp_max);
                 if (i + 1 < len) {
                     s.g[pair] = cur; s.out[pair] = SQ_T;
-                    s.out_scale[pair++] = (float)std::ldexp(1.0, kt - kp - ka);
+                    s.out_scale[pair++] = all.step[i].t_scale = (float)std::ldexp(1.0, kt - kp - ka);
                 }
                 if (i == 0) {
                     q = SQ_Q0; kq = kp;
                 } else {
                     const int kn = exponent_for(q_max), next = q == SQ_Q0 ? SQ_Q1 : SQ_Q0;
                     s.g[pair] = q; s.out[pair] = next;
-                    s.out_scale[pair++] = (float)std::ldexp(1.0, kn - kp - kq);
+                    s.out_scale[pair++] = all.step[i].q_scale = (float)std::ldexp(1.0, kn - kp - kq);
                     q = next; kq = kn;
                 }
-                if (pair) launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 128, dim3(n, pair), s);
+                if (pair && !segments) launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 128, dim3(n, pair), s);
                 if (i + 1 < len) {
                     const int kn = exponent_for(lpp_max), next = cur == SQ_A0 ? SQ_A1 : SQ_A0;
                     s.f = SQ_T; s.g[0] = pout; s.out[0] = next;
-                    s.out_scale[0] = (float)std::ldexp(1.0, kn - kt - kp);
-                    launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 128, dim3(n, 1), s);
+                    s.out_scale[0] = all.step[i].a_scale = (float)std::ldexp(1.0, kn - kt - kp);
+                    if (!segments) launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 128, dim3(n, 1), s);
                     cur = next; ka = kn;
                 }
                 rho = std::fmax(lpp_max, 1e-6);
+            }
+            if (segments) {
+                n = blocks(shapes, [](const OrthoArea &, const OrthoItem &) { return 1; });
+                if (any64) ortho_segment_kernel<64><<<n, 512, 0, st>>>(shapes, all, a_from, q);
+                if (any128) ortho_segment_kernel<128><<<n, 512, 0, st>>>(shapes, all, a_from, q);
             }
             s.f = q; s.xt = xt;
             n = whole();

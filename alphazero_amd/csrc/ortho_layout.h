@@ -88,6 +88,32 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     return a;
 }
 
+// A small matrix stays in one block's LDS from its first to its last step: X <- a X + (b A + c A^2) X as it is written.
+constexpr int kOrthoSmallRows = 64, kOrthoSmallCols = 256;
+struct OrthoSmallStep {
+    float a_scale;               // 2^(k_A - 2 k_X)
+    float b, c;                  // b 2^(k_B - k_A), c 2^(k_B - 2 k_A)
+    float ax, y_scale;           // a 2^(k_X' - k_X), 2^(k_X' - k_B - k_X); the last step's k_X' is 0
+};
+struct OrthoSmallSteps {
+    float pow_kx;                // 2^(k_X) at the start
+    OrthoSmallStep step[kOrthoMaxSteps];
+};
+inline bool ortho_is_small(int rows, int cols) {
+    return ortho_min(rows, cols) <= kOrthoSmallRows && ortho_max(rows, cols) <= kOrthoSmallCols;
+}
+// Matrices up to this side take all products of a segment in one launch, a block each.
+constexpr int kOrthoSegmentRows = 128;
+struct OrthoSegmentStep {
+    float a, b, c;               // P = a I + b A + c A^2, times 2^(k_P), 2^(k_P - k_A), 2^(k_P - 2 k_A)
+    float t_scale, a_scale;      // T = P A, A <- T P: 2^(k_out - k_f - k_g)
+    float q_scale;               // Q <- P Q
+};
+struct OrthoSegmentSteps {
+    int count;
+    OrthoSegmentStep step[kOrthoSegment];
+};
+
 struct OrthoParams {
     int type;                    // nnb_dtype of x, out and weight
     int muon;                    // 1: optimiser step
