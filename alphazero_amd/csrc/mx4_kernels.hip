@@ -193,19 +193,20 @@ __device__ __forceinline__ void store_features(const Mx4Linear &a, long long r, 
 }
 
 // Large products on 32 x 32 x 64 tiles (measured alone: 6.5 PFLOP/s with one wave per SIMD, 16 x 16 x 128 3.6).  A block
-// of 2 x 2 waves computes (TX * 64) rows x (TW * 64) features.  A stage is 256 elements of every row, one unit per 32
+// of WX x WW waves computes (WX * TX * 32) rows x (WW * TW * 32) features.  A stage is 256 elements of every row, one unit per 32
 // rows, brought to LDS by the loads themselves into a ring of RING stages.  Operands are read from LDS AHEAD k-steps
 // before they multiply; all waves meet once per stage, when its last operands are in registers: from then on its place in
 // the ring is free for the stage RING further on, and the next one's operands are read while the last AHEAD k-steps
 // multiply.
 
-template <typename T, int TX, int TW, int RING, int AHEAD>
-__global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
-    constexpr int kWaves = 4, kRows = 2 * TX * 32, kFeatures = 2 * TW * 32;
-    constexpr int kXUnits = 2 * TX, kUnits = 2 * TX + 2 * TW;        // per stage; a wave loads kUnits of 4 * kUnits kilobytes
+template <typename T, int WX, int WW, int TX, int TW, int RING, int AHEAD>
+__global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
+    constexpr int kWaves = WX * WW, kRows = WX * TX * 32, kFeatures = WW * TW * 32;
+    constexpr int kXUnits = WX * TX, kUnits = kXUnits + WW * TW;     // per stage, of 4 KB; a wave loads kPerWave of them
+    constexpr int kPerWave = kUnits / kWaves;
     constexpr int kScaleLoads = kUnits / 4;                          // 1 KB: the scales of four units
-    constexpr int kInFlight = (RING - 2) * (kUnits + 1);             // a wave's loads behind the stage it waits for
-    static_assert(kXUnits % 4 == 0 && kUnits % 4 == 0 && kScaleLoads <= kWaves && kInFlight < 64, "");
+    constexpr int kInFlight = (RING - 2) * 4 * kPerWave;             // a wave's loads of codes behind the stage it waits for
+    static_assert(kXUnits % 4 == 0 && kUnits % 4 == 0 && kUnits % kWaves == 0 && kScaleLoads <= kWaves, "");
     __shared__ i32x4 lds[RING][kUnits][256];
     __shared__ i32x4 lds_scales[RING][kUnits][16];
     const long long rows = a.row_count && *a.row_count < a.rows ? *a.row_count : a.rows;
@@ -235,24 +236,25 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
         const int i = u < kXUnits ? u : u - kXUnits, left = u < kXUnits ? x_left : w_left;
         return ((u < kXUnits ? x_unit0 : w_unit0) + (i < left ? i : left)) * stages;
     };
-    const uint8_t *codes[kUnits / 4];                                // this wave's units: wave * kUnits / 4 + i
+    const uint8_t *codes[kPerWave];                                  // this wave's units: wave * kPerWave + i
 #pragma unroll
-    for (int i = 0; i < kUnits / 4; ++i) {
-        const int u = wave * (kUnits / 4) + i;
+    for (int i = 0; i < kPerWave; ++i) {
+        const int u = wave * kPerWave + i;
         codes[i] = (u < kXUnits ? a.x_codes : a.w_codes) + unit_at(u) * 4096;
     }
-    const int sload = wave % kScaleLoads;                            // a spare wave repeats another one's load
+    const bool loads_scales = wave < kScaleLoads;                    // one load more for the first waves
+    const int sload = loads_scales ? wave : 0;
     const uint8_t *scales = (sload * 4 < kXUnits ? a.x_scales : a.w_scales) + unit_at(sload * 4) * 256;
     const uint32_t soffset = (uint32_t)(unit_at(sload * 4 + (lane >> 4)) - unit_at(sload * 4)) * 256 + (lane & 15) * 16;
     auto issue = [&](int t, int slot) {
 #pragma unroll
-        for (int i = 0; i < kUnits / 4; ++i)
+        for (int i = 0; i < kPerWave; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                load_to_lds(codes[i] + (size_t)t * 4096 + j * 1024, lane * 16, &lds[slot][wave * (kUnits / 4) + i][j * 64]);
-        load_to_lds(scales + (size_t)t * 256, soffset, &lds_scales[slot][sload * 4][0]);
+                load_to_lds(codes[i] + (size_t)t * 4096 + j * 1024, lane * 16, &lds[slot][wave * kPerWave + i][j * 64]);
+        if (loads_scales) load_to_lds(scales + (size_t)t * 256, soffset, &lds_scales[slot][sload * 4][0]);
     };
-    const int ux = wave % 2 * TX, uw = kXUnits + wave / 2 * TW;      // this wave's first units in the tile
+    const int ux = wave % WX * TX, uw = kXUnits + wave / WX * TW;    // this wave's first units in the tile
 
     constexpr int kBuffers = AHEAD == 1 ? 2 : 4;                     // of operands, by k-step
     f32x16 acc[TX][TW] = {};
@@ -274,8 +276,9 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
     // The loads of the stage to come have landed (those of later ones may be on their way), this wave has read what it
     // needs of the present one, and after the barrier so have all.
     auto meet = [&](bool all_issued) {
-        if (all_issued) wait_and_meet<kInFlight>();
-        else wait_and_meet<0>();
+        if (!all_issued) wait_and_meet<0>();
+        else if (loads_scales) wait_and_meet<kInFlight + RING - 2>();
+        else wait_and_meet<kInFlight>();
     };
     auto multiply = [&](auto s) {
         constexpr int S = s;
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
     // write four features of its own row (measured on 8192 x 8192 outputs in bfloat16: 140 us for the stores alone).
     // Loops stay rolled where they can: this code runs once per tile, and what it costs is fetching its instructions.
     constexpr int kWidth = TW * 32, kStride = kWidth + 4, kPack = 16 / sizeof(T), kRowLanes = kWidth / kPack;
-    static_assert((kWaves * 32 * kStride + kFeatures) * 4 <= sizeof(lds), "the waves' parts and the bias fit");
+    static_assert((kWaves * 32 * kStride + kFeatures) * 4 <= (int)sizeof(lds), "the waves' parts and the bias fit");
     __syncthreads();
     float *mine = reinterpret_cast<float *>(lds) + wave * 32 * kStride;
     float *bias = reinterpret_cast<float *>(lds) + kWaves * 32 * kStride;
@@ -334,10 +337,10 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(Mx4Linear a) {
         bias[threadIdx.x] = a.bias && c < a.n ? load_as_f32(a.bias, a.bias_type, c) : 0.f;
     }
     __syncthreads();
-    const int f0 = lane % kRowLanes * kPack, c = col0 + wave / 2 * kWidth + f0;
+    const int f0 = lane % kRowLanes * kPack, c = col0 + wave / WX * kWidth + f0;
     float b[kPack];
 #pragma unroll
-    for (int e = 0; e < kPack; ++e) b[e] = bias[wave / 2 * kWidth + f0 + e];
+    for (int e = 0; e < kPack; ++e) b[e] = bias[wave / WX * kWidth + f0 + e];
 #pragma unroll
     for (int i = 0; i < TX; ++i) {
 #pragma unroll
@@ -522,8 +525,8 @@ namespace {
 // Which kernel multiplies: the cheapest by these costs in microseconds (256 CUs; measured at rows 1 .. 2048 of 1024 x 11520,
 // 4096 x 4096, 8192 x 1024, 512 x 512 and 300 x 16384 layers and at 8192^3, within 20 %):
 //   rows kernel     3 + (1.2 + K / 2300) per 256 blocks of (64 rows x 16 features)
-//   128 x 128, one block per CU (four stages in flight)     3.5 + 0.64 per stage of 256 elements and 256 tiles
-//   128 x 128, two blocks per CU (two stages each)          3.5 + 0.9 per stage and 512 tiles
+//   128 x 128, one block of eight waves per CU (a ring of four stages)   3.5 + 0.6 per stage of 256 elements and 256 tiles
+//   128 x 128, two blocks of four waves per CU (two stages each)         3.5 + 0.9 per stage and 512 tiles
 //   256 x 256       8 + 1.65 per stage and 256 tiles
 // For example 1024 rows of 11520 -> 1024: 26 / 31 / 35 / 86 us in this order, 2048 rows of 1024 -> 8192: 95 / 30 / 23 / 25.
 template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
@@ -531,7 +534,7 @@ template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
     auto rounds = [](long long blocks, int at_once) { return (double)((blocks + at_once - 1) / at_once); };
     const double stages = a.kp / 256;
     const double rows_cost = 3.0 + rounds(tiles(64, 16), 256) * (1.2 + a.kp / 2300.0);
-    const double one_cost = 3.5 + rounds(tiles(128, 128), 256) * stages * 0.64;
+    const double one_cost = 3.5 + rounds(tiles(128, 128), 256) * stages * 0.6;
     const double two_cost = 3.5 + rounds(tiles(128, 128), 512) * stages * 0.9;
     const double large_cost = 8.0 + rounds(tiles(256, 256), 256) * stages * 1.65;
     const double tile_cost = one_cost < two_cost ? one_cost : two_cost;
@@ -546,11 +549,11 @@ template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
         else if (a.rows <= 32 || tiles(32, 16) <= 256) rows_form(std::integral_constant<int, 2>{});
         else rows_form(std::integral_constant<int, 4>{});
     } else if (large_cost <= tile_cost) {
-        mx4_tile_kernel<T, 4, 4, 2, 1><<<(unsigned)tiles(256, 256), 256, 0, st>>>(a);
+        mx4_tile_kernel<T, 2, 2, 4, 4, 2, 1><<<(unsigned)tiles(256, 256), 256, 0, st>>>(a);
     } else if (two_cost < one_cost) {
-        mx4_tile_kernel<T, 2, 2, 2, 2><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
+        mx4_tile_kernel<T, 2, 2, 2, 2, 2, 2><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
     } else {
-        mx4_tile_kernel<T, 2, 2, 4, 3><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
+        mx4_tile_kernel<T, 4, 2, 1, 2, 4, 3><<<(unsigned)tiles(128, 128), 512, 0, st>>>(a);
     }
 }
 

@@ -208,7 +208,10 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroup g, OrthoPar
     emit_units<32, true>(q, kStride, area + (tall ? a.x : a.xt(0)), r0 + qr, c0 + qc, tall ? a.np : a.mp, Unchanged{});
 }
 
-enum OrthoStage { STAGE_GRAM, STAGE_REDUCE, STAGE_POLY, STAGE_MUL, STAGE_APPLY, STAGE_FINISH };
+enum OrthoStage { STAGE_GRAM, STAGE_POLY, STAGE_MUL, STAGE_APPLY, STAGE_FINISH };
+
+// Index of sub-tile (i, j), i <= j, of a symmetric matrix of `side` sub-tiles a side.
+__device__ __forceinline__ int sub_tile(int i, int j, int side) { return i * side - i * (i - 1) / 2 + j - i; }
 
 struct StageArgs {
     int f, g[2], out[2];         // squares: factors and result (MUL: up to two with the same first factor, by blockIdx.y;
@@ -218,88 +221,101 @@ struct StageArgs {
     float a, b, c;               // POLY: coefficients, times 2^(k_out), 2^(k_out - k_A), 2^(k_out - 2 k_A)
 };
 
-// C = F G^T over K, both factors in units.  A block computes a tile of 32 * TB squared with 2 x 2 waves; a stage is 32 of K,
-// brought to LDS by the loads themselves into a ring of RING stages; a wave reads a stage's operands into registers
-// while it multiplies the one before, and all waves meet once per stage.  48 matrix instructions (TB = 4) stand against
-// 16 LDS reads.
-template <typename T, int STAGE, int TB, int RING>
+// C = F G^T over K, both factors in units.  A block computes a tile of WR x WC sub-tiles (16 TB squared, one wave each)
+// with KG groups of such waves that share K; a stage is 32 of K per group, brought to LDS by the loads themselves into a
+// ring of RING stages; a wave reads a stage's operands into registers while it multiplies the one before, and all waves
+// meet once per stage.
+//
+// What bounds it: a CU takes in at most 64 bytes a clock (54 measured from L2, 18 to 24 from behind it), a 128 x 128
+// tile loads 32 KB a stage for 768 clocks of products, and the two overlap only where several blocks share a CU: of 1024 x
+// 1024 x 11520, loads alone take 50 us, products alone 46, both 73 with two blocks of four waves per CU.  One block per
+// CU is slower whatever it gains in reuse or depth (97 us with a ring of five stages, 85 with 128 x 256 tiles on eight
+// waves), and so is one load or read behind every few products (78).
+template <int TB_, int WR_, int WC_, int KG_, int RING_> struct Shape {
+    static constexpr int TB = TB_, WR = WR_, WC = WC_, KG = KG_, RING = RING_, kSub = 16 * TB, kRows = WR * kSub, kCols = WC * kSub,
+                         kWaves = WR * WC * KG, kThreads = 64 * kWaves, kUnits = (WR + WC) * TB;
+};
+typedef Shape<4, 2, 2, 1, 2> LargeTile;                          // 128 x 128
+typedef Shape<2, 2, 2, 1, 4> SmallTile;                          // 64 x 64, two blocks per CU
+typedef Shape<2, 2, 2, 2, 4> LoneTile;                           // 64 x 64, two groups of waves, one block per CU
+
+// Tiles of rows x cols that hold anything on or above the diagonal of an m x m matrix, and the tile of index `tile`.
+template <typename S> __host__ __device__ inline int upper_tiles_of_row(int ti, int mp) {
+    return (mp + S::kCols - 1) / S::kCols - ti * S::kRows / S::kCols;
+}
+template <typename S> __host__ __device__ inline int upper_tiles(int mp) {
+    int n = 0;
+    for (int ti = 0; ti * S::kRows < mp; ++ti) n += upper_tiles_of_row<S>(ti, mp);
+    return n;
+}
+
+template <typename T, int STAGE, typename S>
 __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams &p, const StageArgs &s, const OrthoGroup *items) {
-    constexpr int kTile = 32 * TB, kSub = 16 * TB, kStride = kSub + 4, kUnits = 4 * TB;
-    constexpr bool symmetric = STAGE == STAGE_GRAM || STAGE == STAGE_REDUCE || STAGE == STAGE_POLY || STAGE == STAGE_MUL;
-    constexpr int kRingBytes = STAGE == STAGE_REDUCE ? 0 : RING * kUnits * 2048, kOutBytes = 4 * kSub * kStride * 4;
+    constexpr int TB = S::TB, RING = S::RING, kSub = S::kSub, kStride = kSub + 4, kUnits = S::kUnits, kGroup = S::WR * S::WC;
+    constexpr bool symmetric = STAGE == STAGE_GRAM || STAGE == STAGE_POLY || STAGE == STAGE_MUL;
+    constexpr int kStageBytes = S::KG * kUnits * 2048, kRingBytes = RING * kStageBytes, kOutBytes = kGroup * kSub * kStride * 4;
+    constexpr int kPerWave = 2 * kUnits / kGroup;                // loads of 1 KB per stage: its group's, for its k
+    static_assert(2 * kUnits % kGroup == 0, "whole loads");
     __shared__ __attribute__((aligned(16))) unsigned char lds[kRingBytes > kOutBytes ? kRingBytes : kOutBytes];
     int local;
     const int index = find_item(g, xcd_block(), local);
     const OrthoShape &it = g.item[index];
     const OrthoArea a = ortho_area(it.rows, it.cols);
-    const int mt = (a.mp + kTile - 1) / kTile, nt = (a.np + kTile - 1) / kTile;
-    const int tiles = symmetric ? ortho_triangle(mt) : mt * nt;
+    const int mt = (a.mp + S::kRows - 1) / S::kRows, nt = (a.np + S::kCols - 1) / S::kCols;
+    const int tiles = symmetric ? upper_tiles<S>(a.mp) : mt * nt;
     int part = 0;
     if (STAGE == STAGE_GRAM) { part = local / tiles % a.splits; local = local / (tiles * a.splits) * tiles + local % tiles; }
-    const int batch = local / tiles, tile = local % tiles;
-    int ti = 0, tj;
+    const int batch = local / tiles;
+    int ti = 0, tj = local % tiles;
     if (symmetric) {
-        int t = tile;
-        while (t >= mt - ti) { t -= mt - ti; ++ti; }
-        tj = ti + t;
+        while (tj >= upper_tiles_of_row<S>(ti, a.mp)) tj -= upper_tiles_of_row<S>(ti++, a.mp);
+        tj += ti * S::kRows / S::kCols;
     } else {
-        ti = tile % mt;
-        tj = tile / mt;
+        ti = tj % mt;
+        tj /= mt;
     }
     unsigned char *area = g.ws + it.ws + batch * it.ws_stride;
     const int which = STAGE == STAGE_MUL ? blockIdx.y : 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wr = wave / 2 * kSub, wc = wave % 2 * kSub;
+    const int kg = wave / kGroup, in_group = wave % kGroup, wr = in_group / S::WC, wc = in_group % S::WC;
     f32x4 acc[TB][TB] = {};
-    f32x4 *partials = reinterpret_cast<f32x4 *>(area + a.partial) + ((size_t)tile * 4 + wave) * TB * TB * 64 + lane;
-    const size_t partial_stride = (size_t)tiles * 4 * TB * TB * 64;
-
-    if constexpr (STAGE == STAGE_REDUCE) {
-        for (int k = 0; k < a.splits; ++k)
-#pragma unroll
-            for (int i = 0; i < TB * TB; ++i) acc[i / TB][i % TB] += partials[k * partial_stride + i * 64];
-    } else {
+    {
         const int kdim = STAGE == STAGE_GRAM ? a.np : a.mp, k_units = kdim / 32;
-        int k0 = 0, k1 = k_units;                                // an even number of k-steps
+        int k0 = 0, k1 = k_units;                                // a multiple of 64: whole stages, an even number of 32s
         if (STAGE == STAGE_GRAM) {
-            k0 = (int)((long long)(k_units / 2) * part / a.splits) * 2;
-            k1 = (int)((long long)(k_units / 2) * (part + 1) / a.splits) * 2;
+            k0 = (int)((long long)(k_units / 4) * part / a.splits) * 4;
+            k1 = part + 1 == a.splits ? k_units : (int)((long long)(k_units / 4) * (part + 1) / a.splits) * 4;
         }
         const unsigned char *f = area + (STAGE == STAGE_GRAM ? a.x : a.sq(s.f));
         const unsigned char *h = STAGE == STAGE_GRAM ? f : STAGE == STAGE_POLY ? f : STAGE == STAGE_MUL ? area + a.sq(s.g[which])
                                                                                             : area + a.xt(s.xt);
         const int f_rows = a.mp / 16 - 1, h_rows = (symmetric ? a.mp : a.np) / 16 - 1;
-        const unsigned char *source[TB];                         // this wave's units of a stage; past the end the last again
+        const unsigned char *source[kPerWave];                   // this wave's kilobytes of a stage; past the end the last rows again
 #pragma unroll
-        for (int i = 0; i < TB; ++i) {
-            const int u = wave * TB + i;
-            source[i] = uniform(u < 2 * TB ? f + unit_offset(ortho_min(ti * 2 * TB + u, f_rows), k0, kdim)
-                                           : h + unit_offset(ortho_min(tj * 2 * TB + u - 2 * TB, h_rows), k0, kdim));
+        for (int i = 0; i < kPerWave; ++i) {
+            const int d = in_group * kPerWave + i, u = d / 2;
+            source[i] = uniform((u < S::WR * TB ? f + unit_offset(ortho_min(ti * S::WR * TB + u, f_rows), k0 + kg, kdim)
+                                                : h + unit_offset(ortho_min(tj * S::WC * TB + u - S::WR * TB, h_rows), k0 + kg, kdim)) +
+                                d % 2 * 1024);
         }
-        const int stages = k1 - k0;
-        auto issue = [&](int t, int slot) {
-#pragma unroll
-            for (int i = 0; i < TB; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    load_to_lds(source[i] + (size_t)t * 2048 + j * 1024, lane * 16, lds + (slot * kUnits + wave * TB + i) * 2048 + j * 1024);
+        const int stages = (k1 - k0) / S::KG;
+        auto issue = [&](int t, int slot, int i) {
+            load_to_lds(source[i] + (size_t)t * (S::KG * 2048), lane * 16,
+                        lds + slot * kStageBytes + kg * kUnits * 2048 + (in_group * kPerWave + i) * 1024);
         };
         half8 fh[2][TB], fl[2][TB], hh[2][TB], hl[2][TB];
-        auto fragments = [&](int slot, auto to) {
-            constexpr int B = to;
-            const unsigned char *base = lds + slot * kUnits * 2048 + lane * 16;
-#pragma unroll
-            for (int i = 0; i < TB; ++i) {
-                const unsigned char *fu = base + (wave / 2 * TB + i) * 2048, *hu = base + (2 * TB + wave % 2 * TB + i) * 2048;
-                fh[B][i] = *reinterpret_cast<const half8 *>(fu);
-                fl[B][i] = *reinterpret_cast<const half8 *>(fu + 1024);
-                hh[B][i] = *reinterpret_cast<const half8 *>(hu);
-                hl[B][i] = *reinterpret_cast<const half8 *>(hu + 1024);
-            }
+        auto fragment = [&](int slot, auto to, auto which_read) {     // read r of 4 * TB
+            constexpr int B = to, R = which_read, I = R / 4;
+            const unsigned char *base = lds + slot * kStageBytes + kg * kUnits * 2048 + lane * 16;
+            const unsigned char *fu = base + (wr * TB + I) * 2048, *hu = base + ((S::WR + wc) * TB + I) * 2048;
+            if constexpr (R % 4 == 0) fl[B][I] = *reinterpret_cast<const half8 *>(fu + 1024);
+            if constexpr (R % 4 == 1) hh[B][I] = *reinterpret_cast<const half8 *>(hu);
+            if constexpr (R % 4 == 2) fh[B][I] = *reinterpret_cast<const half8 *>(fu);
+            if constexpr (R % 4 == 3) hl[B][I] = *reinterpret_cast<const half8 *>(hu + 1024);
         };
+        // The three products of an entry stand TB * TB instructions apart: none waits for the one before.
         auto multiply = [&](auto from) {
             constexpr int B = from;
-            // the three products of an entry stand TB * TB instructions apart: none waits for the one before
 #pragma unroll
             for (int i = 0; i < TB; ++i)
 #pragma unroll
@@ -314,7 +330,7 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
                 for (int j = 0; j < TB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[B][i], hh[B][j], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         };
-        constexpr int kInFlight = (RING - 2) * 2 * TB;           // a wave's loads behind the stage it waits for
+        constexpr int kInFlight = (RING - 2) * kPerWave;         // a wave's loads behind the stage it waits for
         auto meet = [&](bool all_issued) {
             if (all_issued) wait_and_meet<kInFlight>();
             else wait_and_meet<0>();
@@ -323,36 +339,65 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         constexpr std::integral_constant<int, 1> odd{};
 #pragma unroll
         for (int t = 0; t < RING - 1; ++t)
-            if (t < stages) issue(t, t);
+            if (t < stages)
+#pragma unroll
+                for (int d = 0; d < kPerWave; ++d) issue(t, t, d);
         meet(RING - 1 <= stages);
-        if (RING - 1 < stages) issue(RING - 1, RING - 1);
-        fragments(0, even);
+        if (RING - 1 < stages)
+#pragma unroll
+            for (int d = 0; d < kPerWave; ++d) issue(RING - 1, RING - 1, d);
+        static_for<4 * TB>([&](auto r) { fragment(0, even, r); });
         int slot = 0;
         auto step = [&](int t, auto from, auto to) {             // multiplies stage t, reads stage t + 1
             const int next = slot + 1 == RING ? 0 : slot + 1;
             meet(t + RING <= stages);
-            if (t + RING < stages) issue(t + RING, slot);
-            fragments(next, to);
+            if (t + RING < stages)
+#pragma unroll
+                for (int i = 0; i < kPerWave; ++i) issue(t + RING, slot, i);
+            static_for<4 * TB>([&](auto r) { fragment(next, to, r); });
             multiply(from);
             slot = next;
         };
+        // pairs of stages, for the two sets of registers; an odd last one by itself
         int t = 0;
         for (; t + 2 < stages; t += 2) {
             step(t, even, odd);
             step(t + 1, odd, even);
         }
-        step(t, even, odd);
-        multiply(odd);
-        if (STAGE == STAGE_GRAM && a.splits > 1) {
-#pragma unroll
-            for (int i = 0; i < TB * TB; ++i) partials[part * partial_stride + i * 64] = acc[i / TB][i % TB];
-            return;
+        if (t + 1 < stages) {
+            step(t, even, odd);
+            multiply(odd);
+        } else {
+            multiply(even);
         }
     }
 
-    // A wave's results meet in its own part of LDS (free once all waves have read their last operands).
+    // The groups' sums meet in the first one's registers, its results in LDS, every wave's in its own part (free once all
+    // waves have read their last operands).
     __syncthreads();
-    float *mine = reinterpret_cast<float *>(lds) + wave * kSub * kStride;
+    float *mine = reinterpret_cast<float *>(lds) + in_group * kSub * kStride;
+    static_assert(S::KG <= 2, "");
+    if (S::KG == 2) {
+        f32x4 *sums = reinterpret_cast<f32x4 *>(lds) + in_group * TB * TB * 64 + lane;
+        if (kg == 1)
+#pragma unroll
+            for (int i = 0; i < TB * TB; ++i) sums[i * 64] = acc[i / TB][i % TB];
+        __syncthreads();
+        if (kg == 0)
+#pragma unroll
+            for (int i = 0; i < TB * TB; ++i) acc[i / TB][i % TB] += sums[i * 64];
+        __syncthreads();
+        if (kg == 1) return;
+    }
+    const int r0 = ti * S::kRows + wr * kSub, c0 = tj * S::kCols + wc * kSub;
+    // behind the padding, or below the diagonal, where the mirror image of another sub-tile goes
+    if (r0 >= a.mp || c0 >= (symmetric ? a.mp : a.np) || (symmetric && r0 > c0)) return;
+    if (STAGE == STAGE_GRAM && a.splits > 1) {
+        f32x4 *partials = reinterpret_cast<f32x4 *>(area + a.partial) + ((size_t)part * a.sub_tiles + sub_tile(r0 / kSub, c0 / kSub, a.mp / kSub)) * TB * TB * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < TB * TB; ++i) partials[i * 64] = acc[i / TB][i % TB];
+        return;
+    }
     const float out_scale = STAGE == STAGE_POLY ? s.c : s.out_scale[which];
 #pragma unroll
     for (int i = 0; i < TB; ++i)
@@ -361,8 +406,6 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 mine[(16 * i + 4 * (lane >> 4) + e) * kStride + 16 * j + (lane & 15)] = acc[i][j][e] * out_scale;
-    const int r0 = ti * kTile + wr, c0 = tj * kTile + wc;
-    if (r0 >= a.mp || c0 >= (symmetric ? a.mp : a.np)) return;   // behind the padding
     if constexpr (symmetric) {
         unsigned char *dst = area + a.sq(s.out[which]);
         if constexpr (STAGE == STAGE_POLY) {
@@ -373,10 +416,10 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
                 for (int e = 0; e < 8; ++e) v[e] += s.b * ((float)hi[e] + (float)lo[e]) + (r == c + e ? s.a : 0.f);
             };
             emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, add_lower);
-            if (ti != tj) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, add_lower);
+            if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, add_lower);
         } else {
             emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
-            if (ti != tj) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
+            if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
         }
     } else if constexpr (STAGE == STAGE_APPLY) {
         emit_units<kSub, false>(mine, kStride, area + a.x, r0, c0, a.np, Unchanged{});
@@ -413,13 +456,55 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     }
 }
 
-template <int STAGE, int TB, int RING>
-__global__ __launch_bounds__(256, 2) void ortho_product_kernel(OrthoShapes g, OrthoParams p, StageArgs s) {
-    product<float, STAGE, TB, RING>(g, p, s, nullptr);
+template <int STAGE, typename S>
+__global__ __launch_bounds__(S::kThreads, 2) void ortho_product_kernel(OrthoShapes g, OrthoParams p, StageArgs s) {
+    product<float, STAGE, S>(g, p, s, nullptr);
 }
-template <typename T, int TB, int RING>
-__global__ __launch_bounds__(256, 2) void ortho_finish_kernel(OrthoShapes g, OrthoParams p, StageArgs s, OrthoGroup items) {
-    product<T, STAGE_FINISH, TB, RING>(g, p, s, &items);
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads, 2) void ortho_finish_kernel(OrthoShapes g, OrthoParams p, StageArgs s, OrthoGroup items) {
+    product<T, STAGE_FINISH, S>(g, p, s, &items);
+}
+
+// Adds up the parts of X X^T, one block of four waves per sub-tile (16 TB squared), and lays it out both ways round.
+template <int TB>
+__global__ __launch_bounds__(256) void ortho_reduce_kernel(OrthoShapes g, StageArgs s) {
+    constexpr int kSub = 16 * TB, kStride = kSub + 4, kEach = TB * TB / 4;
+    __shared__ float tile[kSub * kStride];
+    int local;
+    const OrthoShape &it = g.item[find_item(g, blockIdx.x, local)];
+    const OrthoArea a = ortho_area(it.rows, it.cols);
+    const int batch = local / a.sub_tiles, index = local % a.sub_tiles, side = a.mp / kSub;
+    int ti = 0, tj = index;
+    while (tj >= side - ti) tj -= side - ti++;
+    tj += ti;
+    unsigned char *area = g.ws + it.ws + batch * it.ws_stride;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const f32x4 *partials = reinterpret_cast<const f32x4 *>(area + a.partial) + ((size_t)index * TB * TB + wave * kEach) * 64 + lane;
+    f32x4 sum[kEach] = {};
+#pragma unroll 4
+    for (int k = 0; k < a.splits; ++k)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sum[i] += partials[((size_t)k * a.sub_tiles * TB * TB + i) * 64];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int b = wave * kEach + i;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            tile[(16 * (b / TB) + 4 * (lane >> 4) + e) * kStride + 16 * (b % TB) + (lane & 15)] = sum[i][e] * s.out_scale[0];
+    }
+    __syncthreads();
+    // a wave takes a quarter of the units, each way round
+    unsigned char *dst = area + a.sq(s.out[0]);
+    constexpr int kQuarter = kSub / 2;
+    const int qr = wave / 2 * kQuarter, qc = wave % 2 * kQuarter;
+    if constexpr (kQuarter >= 32) {
+        const float *q = tile + qr * kStride + qc;
+        emit_units<kQuarter, false>(q, kStride, dst, ti * kSub + qr, tj * kSub + qc, a.mp, Unchanged{});
+        if (ti != tj) emit_units<kQuarter, true>(q, kStride, dst, ti * kSub + qr, tj * kSub + qc, a.mp, Unchanged{});
+    } else {
+        if (wave == 0) emit_units<kSub, false>(tile, kStride, dst, ti * kSub, tj * kSub, a.mp, Unchanged{});
+        if (wave == 1 && ti != tj) emit_units<kSub, true>(tile, kStride, dst, ti * kSub, tj * kSub, a.mp, Unchanged{});
+    }
 }
 
 // ------------------------------------------------------------------------------------- matrices in one block's LDS
@@ -710,6 +795,10 @@ bool ortho_coefficients_ok(const OrthoParams &p) {
 
 namespace {
 
+template <typename S> int all_tiles(const OrthoArea &a) {
+    return (a.mp + S::kRows - 1) / S::kRows * ((a.np + S::kCols - 1) / S::kCols);
+}
+
 void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     OrthoSmallSteps steps = {};
     double rho = 1.0;
@@ -760,62 +849,81 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     OrthoShapes shapes = {};
     shapes.count = g.count;
     shapes.ws = g.ws;
-    long long symmetric128 = 0, full128 = 0;
+    auto with_tile = [](int k, auto &&f) {
+        if (k == 0) f(LargeTile{});
+        else if (k == 1) f(SmallTile{});
+        else f(LoneTile{});
+    };
+    long long upper[2] = {}, full[2] = {};
     bool any64 = false, any128 = false, gram_of[2] = {}, reduce_of[2] = {};
     for (int i = 0; i < g.count; ++i) {
         const OrthoItem &it = g.item[i];
         const OrthoArea a = ortho_area(it.rows, it.cols);
         shapes.item[i] = {it.ws, it.ws_stride, it.rows, it.cols, it.batch};
-        const int mt = (a.mp + 127) / 128, nt = (a.np + 127) / 128;
-        symmetric128 += (long long)it.batch * ortho_triangle(mt);
-        full128 += (long long)it.batch * mt * nt;
+        for (int k = 0; k < 2; ++k)
+            with_tile(k, [&](auto shape) {
+                typedef decltype(shape) S;
+                upper[k] += (long long)it.batch * upper_tiles<S>(a.mp);
+                full[k] += (long long)it.batch * all_tiles<S>(a);
+            });
         any64 |= a.mp == 64;
         any128 |= a.mp == 128;
-        gram_of[a.tile == 128] = true;
-        reduce_of[a.tile == 128] |= a.splits > 1;
+        gram_of[a.sub == 64] = true;
+        reduce_of[a.sub == 64] |= a.splits > 1;
     }
-    // Tiles of 128 need half the LDS traffic, tiles of 64 give four times the blocks: 128 where they fill the chip.
-    const int symmetric_tile = symmetric128 >= 200 ? 128 : 64, full_tile = full128 >= 200 ? 128 : 64;
+    // Large tiles where they give most CUs at least one; where even small ones give no CU two, two groups share each
+    // (1024 x 1024 x 1024, 136 tiles: 11.5 us against 12.8; 273 tiles of 832 x 832 x 832: 17.9 against 13.9).
+    auto pick = [](const long long (&n)[2]) { return n[0] >= 200 ? 0 : n[1] > 256 ? 1 : 2; };
+    const int symmetric_tile = pick(upper), full_tile = pick(full);
     auto blocks = [&](auto &group, auto per_matrix) {
         int n = 0;
         for (int i = 0; i < g.count; ++i) {
             group.first[i] = n;
-            n += g.item[i].batch * per_matrix(ortho_area(g.item[i].rows, g.item[i].cols), g.item[i]);
+            n += g.item[i].batch * per_matrix(ortho_area(g.item[i].rows, g.item[i].cols));
         }
         group.first[g.count] = n;
         return n;
     };
     auto squares = [&] {
-        return blocks(shapes, [&](const OrthoArea &a, const OrthoItem &) { return ortho_triangle((a.mp + symmetric_tile - 1) / symmetric_tile); });
+        int n = 0;
+        with_tile(symmetric_tile, [&](auto tile) { n = blocks(shapes, [](const OrthoArea &a) { return upper_tiles<decltype(tile)>(a.mp); }); });
+        return n;
     };
     auto whole = [&] {
-        return blocks(shapes, [&](const OrthoArea &a, const OrthoItem &) { return (a.mp + full_tile - 1) / full_tile * ((a.np + full_tile - 1) / full_tile); });
+        int n = 0;
+        with_tile(full_tile, [&](auto tile) {
+            typedef decltype(tile) S;
+            n = blocks(shapes, [](const OrthoArea &a) { return all_tiles<S>(a); });
+        });
+        return n;
     };
-    auto launch = [&](auto stage, bool large, dim3 grid, const StageArgs &s) {
+    auto launch = [&](auto stage, int tile, dim3 grid, const StageArgs &s) {
         constexpr int STAGE = stage;
-        if (large) ortho_product_kernel<STAGE, 4, 2><<<grid, 256, 0, st>>>(shapes, p, s);
-        else ortho_product_kernel<STAGE, 2, 4><<<grid, 256, 0, st>>>(shapes, p, s);
+        with_tile(tile, [&](auto shape) {
+            typedef decltype(shape) S;
+            ortho_product_kernel<STAGE, S><<<grid, S::kThreads, 0, st>>>(shapes, p, s);
+        });
     };
     auto gram = [&](const StageArgs &s) {
         for (int large = 0; large < 2; ++large) {
             if (!gram_of[large]) continue;
-            auto mine = [&](const OrthoArea &a) { return (a.tile == 128) == (large == 1); };
-            int n = blocks(shapes, [&](const OrthoArea &a, const OrthoItem &) {
-                return mine(a) ? ortho_triangle((a.mp + a.tile - 1) / a.tile) * a.splits : 0; });
-            launch(std::integral_constant<int, STAGE_GRAM>{}, large, n, s);
+            auto mine = [&](const OrthoArea &a) { return (a.sub == 64) == (large == 1); };
+            int n = blocks(shapes, [&](const OrthoArea &a) {
+                return !mine(a) ? 0 : (large ? upper_tiles<LargeTile>(a.mp) : upper_tiles<SmallTile>(a.mp)) * a.splits; });
+            launch(std::integral_constant<int, STAGE_GRAM>{}, large ? 0 : 1, n, s);
             if (!reduce_of[large]) continue;
-            n = blocks(shapes, [&](const OrthoArea &a, const OrthoItem &) {
-                return mine(a) && a.splits > 1 ? ortho_triangle((a.mp + a.tile - 1) / a.tile) : 0; });
-            launch(std::integral_constant<int, STAGE_REDUCE>{}, large, n, s);
+            n = blocks(shapes, [&](const OrthoArea &a) { return mine(a) && a.splits > 1 ? a.sub_tiles : 0; });
+            if (large) ortho_reduce_kernel<4><<<n, 256, 0, st>>>(shapes, s);
+            else ortho_reduce_kernel<2><<<n, 256, 0, st>>>(shapes, s);
         }
     };
     with_dtype(p.type, [&](auto type) {
         typedef decltype(type) T;
-        int n = blocks(g, [](const OrthoArea &a, const OrthoItem &) { return a.parts_used; });
+        int n = blocks(g, [](const OrthoArea &a) { return a.parts_used; });
         ortho_norm_kernel<T><<<n, 256, 0, st>>>(g, p);
         double rho = 1.0;                       // bound of A's largest eigenvalue
         int kx = exponent_for(1.0), xt = 0;
-        n = blocks(g, [](const OrthoArea &a, const OrthoItem &) { return a.mp / 64 * (a.np / 64); });
+        n = blocks(g, [](const OrthoArea &a) { return a.mp / 64 * (a.np / 64); });
         ortho_split_kernel<T><<<n, 256, 0, st>>>(g, p, (float)std::ldexp(1.0, kx));
         for (int s0 = 0; s0 < p.steps; s0 += kOrthoSegment) {
             const int len = p.steps - s0 < kOrthoSegment ? p.steps - s0 : kOrthoSegment;
@@ -838,7 +946,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 s.f = cur; s.out[0] = pout;
                 s.a = (float)std::ldexp(c[0], kp); s.b = (float)std::ldexp(c[1], kp - ka); s.c = (float)std::ldexp(c[2], kp - 2 * ka);
                 all.step[i].a = s.a; all.step[i].b = s.b; all.step[i].c = s.c;
-                if (!segments) launch(std::integral_constant<int, STAGE_POLY>{}, symmetric_tile == 128, n, s);
+                if (!segments) launch(std::integral_constant<int, STAGE_POLY>{}, symmetric_tile, n, s);
                 q_max *= p_max;
                 // T = P A and Q <- P Q in one launch, then A <- T P
                 int pair = 0;
@@ -856,18 +964,19 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                     s.out_scale[pair++] = all.step[i].q_scale = (float)std::ldexp(1.0, kn - kp - kq);
                     q = next; kq = kn;
                 }
-                if (pair && !segments) launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 128, dim3(n, pair), s);
+                if (pair && !segments)
+                    launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 2 && n * pair > 256 ? 1 : symmetric_tile, dim3(n, pair), s);
                 if (i + 1 < len) {
                     const int kn = exponent_for(lpp_max), next = cur == SQ_A0 ? SQ_A1 : SQ_A0;
                     s.f = SQ_T; s.g[0] = pout; s.out[0] = next;
                     s.out_scale[0] = all.step[i].a_scale = (float)std::ldexp(1.0, kn - kt - kp);
-                    if (!segments) launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 128, dim3(n, 1), s);
+                    if (!segments) launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile, dim3(n, 1), s);
                     cur = next; ka = kn;
                 }
                 rho = std::fmax(lpp_max, 1e-6);
             }
             if (segments) {
-                n = blocks(shapes, [](const OrthoArea &, const OrthoItem &) { return 1; });
+                n = blocks(shapes, [](const OrthoArea &) { return 1; });
                 if (any64) ortho_segment_kernel<64><<<n, 512, 0, st>>>(shapes, all, a_from, q);
                 if (any128) ortho_segment_kernel<128><<<n, 512, 0, st>>>(shapes, all, a_from, q);
             }
@@ -876,13 +985,15 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
             if (s0 + len < p.steps) {
                 const int kn = exponent_for(std::sqrt(rho));
                 s.out_scale[0] = (float)std::ldexp(1.0, kn - kq - kx);
-                launch(std::integral_constant<int, STAGE_APPLY>{}, full_tile == 128, n, s);
+                launch(std::integral_constant<int, STAGE_APPLY>{}, full_tile, n, s);
                 kx = kn;
                 xt = 1 - xt;
             } else {
                 s.out_scale[0] = (float)std::ldexp(1.0, -kq - kx);
-                if (full_tile == 128) ortho_finish_kernel<T, 4, 2><<<n, 256, 0, st>>>(shapes, p, s, g);
-                else ortho_finish_kernel<T, 2, 4><<<n, 256, 0, st>>>(shapes, p, s, g);
+                with_tile(full_tile, [&](auto shape) {
+                    typedef decltype(shape) S;
+                    ortho_finish_kernel<T, S><<<n, S::kThreads, 0, st>>>(shapes, p, s, g);
+                });
             }
         }
     });

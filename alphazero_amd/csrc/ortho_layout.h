@@ -51,8 +51,9 @@ typedef OrthoGroupOf<OrthoShape> OrthoShapes;
 // them: lane l holds k 8 (l / 16) .. + 7 of row l % 16.
 struct OrthoArea {
     int m, n, mp, np;
-    int tile;                    // side of the Gram product's tiles
-    int splits;                  // parts that the long side is cut into for it
+    int sub;                     // side of the sub-tiles X X^T is made of: 64 (128 x 128 tiles) or 32 (64 x 64 tiles)
+    int sub_tiles;               // of those on and above the diagonal
+    int splits;                  // parts that the long side is cut into for X X^T
     int parts_used;              // partial sums of squares
     size_t parts, x, xt0, sq0, partial, bytes;
     size_t wide, square;         // bytes of an m x n and of an m x m matrix
@@ -69,9 +70,10 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     a.n = rows < cols ? cols : rows;
     a.mp = ortho_padded(a.m);
     a.np = ortho_padded(a.n);
-    a.tile = a.mp > 256 ? 128 : 64;
-    // enough blocks for two per CU, at least 256 of the long side each
-    const int tiles = ortho_triangle((a.mp + a.tile - 1) / a.tile);
+    a.sub = a.mp > 256 ? 64 : 32;
+    a.sub_tiles = ortho_triangle(a.mp / a.sub);
+    // parts that give every CU two blocks, at least 256 of the long side each
+    const int tiles = ortho_triangle(a.sub == 64 ? (a.mp + 127) / 128 : a.mp / 64);
     a.splits = ortho_max(1, ortho_min(512 / tiles, a.np / 256));
     const long long count = (long long)rows * cols;
     a.parts_used = (int)(count / 4096 < 1 ? 1 : count / 4096 < kOrthoNormParts ? count / 4096 : kOrthoNormParts);
@@ -83,7 +85,7 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     a.xt0 = o; o += 2 * a.wide;
     a.sq0 = o; o += 6 * a.square;
     a.partial = o;
-    if (a.splits > 1) o += (size_t)a.splits * tiles * a.tile * a.tile * sizeof(float);
+    if (a.splits > 1) o += (size_t)a.splits * a.sub_tiles * a.sub * a.sub * sizeof(float);
     a.bytes = o;
     return a;
 }
