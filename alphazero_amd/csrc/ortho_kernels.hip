@@ -127,6 +127,31 @@ __device__ __forceinline__ half8 pack_hi(const float (&v)[8], half8 &lo) {
     return hi;
 }
 
+// sum[j] += a 16 x 16 block of 32 products: hi + lo halves of F's rows times those of N blocks of G's rows.
+template <int N> __device__ __forceinline__ void add_to(half8 fh, half8 fl, const half8 (&gh)[N], const half8 (&gl)[N], f32x4 (&sum)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, gh[j], sum[j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, gl[j], sum[j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, gh[j], sum[j], 0, 0, 0);
+}
+// The same from zero.
+// The matrix unit aligns the products of an instruction, and the sum they are added to, to the largest of them and cuts
+// off what lies more than 3 bits below that one's last place.  In a running sum this takes away from every product once
+// the sum has grown (a diagonal entry of X X^T lost 2e-6 of itself over 2048 columns); from zero, with the small cross
+// products first, what is cut is small against the stage's own sum.  ALL: the product of the lo halves too, which
+// reaches 2^-22 of the whole and matters where one product makes up an entry, as on the diagonals of the squares.
+template <int N, bool ALL>
+__device__ __forceinline__ void add_products(half8 fh, half8 fl, const half8 (&gh)[N], const half8 (&gl)[N], f32x4 (&sum)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (ALL)
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, gl[j], sum[j], 0, 0, 0);
+    add_to<N>(fh, fl, gh, gl, sum);
+}
+
 // Where lane l of unit (row block rb, k block kb) of a matrix with K columns finds its hi halves; the lo ones lie 1 KB on.
 __device__ __forceinline__ size_t unit_offset(int rb, int kb, int k) { return ((size_t)rb * (k / 32) + kb) * 2048; }
 
@@ -151,6 +176,15 @@ __device__ __forceinline__ void emit_units(const float *tile, int stride, unsign
         *reinterpret_cast<half8 *>(at + 1024) = lo;
     }
 }
+// Keeps the diagonal in float32 on the way.
+struct KeepDiagonal {
+    float *diag;
+    __device__ __forceinline__ void operator()(float (&v)[8], int r, int c, unsigned char *) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (r == c + e) diag[r] = v[e];
+    }
+};
 struct Unchanged {
     __device__ __forceinline__ void operator()(float (&)[8], int, int, unsigned char *) const {}
 };
@@ -313,21 +347,26 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
             if constexpr (R % 4 == 2) fh[B][I] = *reinterpret_cast<const half8 *>(fu);
             if constexpr (R % 4 == 3) hl[B][I] = *reinterpret_cast<const half8 *>(hu + 1024);
         };
-        // The three products of an entry stand TB * TB instructions apart: none waits for the one before.
+        // A row of blocks at a time, every stage's sum from zero, smallest products first; the sums are added up by the
+        // vector pipe (see add_products).
+        constexpr bool kAll = STAGE == STAGE_POLY || STAGE == STAGE_MUL, kFromZero = kAll || STAGE == STAGE_GRAM;
         auto multiply = [&](auto from) {
             constexpr int B = from;
+            if constexpr (!kFromZero) {                          // a short sum without a large diagonal
+                static_for<TB>([&](auto row) { add_to<TB>(fh[B][row], fl[B][row], hh[B], hl[B], acc[row]); });
+                __builtin_amdgcn_sched_barrier(0);
+                return;
+            }
+            f32x4 sum[2][TB];
+            static_for<TB>([&](auto row) {
+                constexpr int I = row;
+                add_products<TB, kAll>(fh[B][I], fl[B][I], hh[B], hl[B], sum[I & 1]);
+                if constexpr (I > 0)
 #pragma unroll
-            for (int i = 0; i < TB; ++i)
+                    for (int j = 0; j < TB; ++j) acc[I - 1][j] += sum[(I - 1) & 1][j];
+            });
 #pragma unroll
-                for (int j = 0; j < TB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[B][i], hh[B][j], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < TB; ++i)
-#pragma unroll
-                for (int j = 0; j < TB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[B][i], hl[B][j], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < TB; ++i)
-#pragma unroll
-                for (int j = 0; j < TB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[B][i], hh[B][j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < TB; ++j) acc[TB - 1][j] += sum[(TB - 1) & 1][j];
             __builtin_amdgcn_sched_barrier(0);
         };
         constexpr int kInFlight = (RING - 2) * kPerWave;         // a wave's loads behind the stage it waits for
@@ -418,7 +457,10 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
             emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, add_lower);
             if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, add_lower);
         } else {
-            emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
+            if (STAGE == STAGE_GRAM && r0 == c0)
+                emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, KeepDiagonal{reinterpret_cast<float *>(area + a.diag)});
+            else
+                emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
             if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
         }
     } else if constexpr (STAGE == STAGE_APPLY) {
@@ -495,14 +537,15 @@ __global__ __launch_bounds__(256) void ortho_reduce_kernel(OrthoShapes g, StageA
     __syncthreads();
     // a wave takes a quarter of the units, each way round
     unsigned char *dst = area + a.sq(s.out[0]);
+    const KeepDiagonal keep{reinterpret_cast<float *>(area + a.diag)};       // (off the diagonal nothing is kept)
     constexpr int kQuarter = kSub / 2;
     const int qr = wave / 2 * kQuarter, qc = wave % 2 * kQuarter;
     if constexpr (kQuarter >= 32) {
         const float *q = tile + qr * kStride + qc;
-        emit_units<kQuarter, false>(q, kStride, dst, ti * kSub + qr, tj * kSub + qc, a.mp, Unchanged{});
+        emit_units<kQuarter, false>(q, kStride, dst, ti * kSub + qr, tj * kSub + qc, a.mp, keep);
         if (ti != tj) emit_units<kQuarter, true>(q, kStride, dst, ti * kSub + qr, tj * kSub + qc, a.mp, Unchanged{});
     } else {
-        if (wave == 0) emit_units<kSub, false>(tile, kStride, dst, ti * kSub, tj * kSub, a.mp, Unchanged{});
+        if (wave == 0) emit_units<kSub, false>(tile, kStride, dst, ti * kSub, tj * kSub, a.mp, keep);
         if (wave == 1 && ti != tj) emit_units<kSub, true>(tile, kStride, dst, ti * kSub, tj * kSub, a.mp, Unchanged{});
     }
 }
@@ -511,6 +554,12 @@ __global__ __launch_bounds__(256) void ortho_reduce_kernel(OrthoShapes g, StageA
 //
 // A square's results come four rows of one column to a lane: eight bytes of hi and of lo halves of the transposed
 // matrix's units, which for a symmetric matrix is the matrix.
+//
+// A square M is kept as D + O: its diagonal in float32, the units hold the rest with zeros there, and
+//     F G = D_F D_G + D_F O_G + O_F D_G + O_F O_G
+// of which only the last goes through the matrix unit.  The diagonal is what is large in these matrices: in the products
+// it costs halves their last bits and makes the matrix unit cut off the small ones (see add_products), errors that the
+// recursion on A then multiplies (100 x 130 of normal numbers: 2.4e-6 of the result's size with the diagonal in the units).
 
 // Address of lane (row r, k .. k + 3) in units of a matrix with K columns.
 __device__ __forceinline__ int unit_bytes(int r, int k, int kdim) {
@@ -534,6 +583,35 @@ __device__ __forceinline__ f32x4 get4(const unsigned char *unit) {
     for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
     return v;
 }
+// Four rows r .. r + 3 of column c of a square with K columns, as D + O in units and a float32 diagonal.
+__device__ __forceinline__ void put_square(unsigned char *units, float *diag, int r, int c, int kdim, f32x4 v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (r + e == c) {
+            diag[c] = v[e];
+            v[e] = 0.f;
+        }
+    put4(units + unit_bytes(c, r, kdim), v);
+}
+__device__ __forceinline__ f32x4 get_square(const unsigned char *units, const float *diag, int r, int c, int kdim) {
+    f32x4 v = get4(units + unit_bytes(c, r, kdim));
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (r + e == c) v[e] = diag[c];
+    return v;
+}
+// O_F O_G completed to F G at rows r .. r + 3, column c.
+__device__ __forceinline__ f32x4 add_diagonals(f32x4 product, const unsigned char *f, const float *diag_f, const unsigned char *g,
+                                               const float *diag_g, int r, int c, int kdim) {
+    const f32x4 of = get4(f + unit_bytes(c, r, kdim)), og = get4(g + unit_bytes(c, r, kdim));
+    const float dg = diag_g[c];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float df = diag_f[r + e];
+        product[e] += df * (r + e == c ? dg : og[e]) + of[e] * dg;       // (O is zero on the diagonal)
+    }
+    return product;
+}
 // acc += rows rb of F times rows cb .. cb + N - 1 (blocks of 16) of G, both units with K columns; G may lie in global memory.
 template <int N>
 __device__ __forceinline__ void multiply_units(const unsigned char *f, const unsigned char *g, int rb, int cb, int kdim, f32x4 (&acc)[N]) {
@@ -548,12 +626,7 @@ __device__ __forceinline__ void multiply_units(const unsigned char *f, const uns
             gh[j] = *reinterpret_cast<const half8 *>(gu);
             gl[j] = *reinterpret_cast<const half8 *>(gu + 1024);
         }
-#pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, gh[j], acc[j], 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, gl[j], acc[j], 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, gh[j], acc[j], 0, 0, 0);
+        add_to<N>(fh, fl, gh, gl, acc);
     }
 }
 
@@ -562,8 +635,9 @@ __device__ __forceinline__ void multiply_units(const unsigned char *f, const uns
 template <typename T, int NP>
 __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoParams p, OrthoSmallSteps steps) {
     constexpr int M = kOrthoSmallRows, kWide = M * NP * 4, kSquare = M * M * 4, TN = NP / 32;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kWide + 2 * kSquare];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kWide + 2 * kSquare + 2 * M * 4];
     unsigned char *x = lds, *xt = lds + kWide, *sq_a = lds + 2 * kWide, *sq_b = sq_a + kSquare;
+    float *diag_a = reinterpret_cast<float *>(sq_b + kSquare), *diag_b = diag_a + M;
     int batch;
     const OrthoItem &it = g.item[find_item(g, blockIdx.x, batch)];
     const bool tall = it.rows > it.cols;
@@ -630,20 +704,25 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoPar
         f32x4 a[2] = {};
         multiply_units<2>(x, x, rb, cb, NP, a);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) put4(sq_a + unit_bytes((cb + j) * 16 + col, row, M), a[j] * st.a_scale);
+        for (int j = 0; j < 2; ++j) put_square(sq_a, diag_a, row, (cb + j) * 16 + col, M, a[j] * st.a_scale);
         __syncthreads();
         f32x4 b[2] = {};
         multiply_units<2>(sq_a, sq_a, rb, cb, M, b);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int o = unit_bytes((cb + j) * 16 + col, row, M);
-            put4(sq_b + o, get4(sq_a + o) * st.b + b[j] * st.c);
+            const int c = (cb + j) * 16 + col;
+            const f32x4 low = get_square(sq_a, diag_a, row, c, M), square = add_diagonals(b[j], sq_a, diag_a, sq_a, diag_a, row, c, M);
+            put_square(sq_b, diag_b, row, c, M, low * st.b + square * st.c);
         }
         __syncthreads();
         f32x4 y[TN] = {};
         multiply_units<TN>(sq_b, xt, rb, nb, M, y);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) y[j] = get4(xt + unit_bytes((nb + j) * 16 + col, row, M)) * st.ax + y[j] * st.y_scale;
+        for (int j = 0; j < TN; ++j) {                                  // (a + D_B) X + O_B X
+            const f32x4 old = get4(xt + unit_bytes((nb + j) * 16 + col, row, M));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[j][e] = ((st.ax + diag_b[row + e]) * old[e] + y[j][e]) * st.y_scale;
+        }
         if (s + 1 < p.steps) {
             __syncthreads();                                            // everybody has read the old X
 #pragma unroll
@@ -677,69 +756,79 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoPar
     }
 }
 
-// All products of a segment for a matrix with m <= 128: A comes from memory, Q goes there, a block of eight waves each;
+// All products of a segment for a matrix with m <= 128: A comes from memory, Q goes there, a block each, a wave per 16 rows and half the
+// columns;
 // A (then T, then the next A) and P stay in LDS, Q is read back from memory where it is multiplied.
 template <int MP>
-__global__ __launch_bounds__(512) void ortho_segment_kernel(OrthoShapes g, OrthoSegmentSteps steps, int a_from, int q_to) {
-    constexpr int kSquare = MP * MP * 4, RB = MP / 64, CB = MP / 32;     // a wave's blocks of 16: RB rows x CB columns
+__global__ __launch_bounds__(MP * 8) void ortho_segment_kernel(OrthoShapes g, OrthoSegmentSteps steps, int a_from, int q_to) {
+    constexpr int kSquare = MP * MP * 4, CB = MP / 32;                   // a wave's blocks of 16 columns
     __shared__ __attribute__((aligned(16))) unsigned char sq_a[kSquare], sq_p[kSquare];
+    __shared__ float diag_a[MP], diag_t[MP], diag_p[MP], diag_q[2][MP];
     int batch;
     const OrthoShape &it = g.item[find_item(g, blockIdx.x, batch)];
     const OrthoArea area = ortho_area(it.rows, it.cols);
     if (area.mp != MP) return;                                           // the other size's launch takes it
     unsigned char *ws = g.ws + it.ws + batch * it.ws_stride;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rb = wave / 2 * RB, cb = wave % 2 * CB;
-    const int row = (lane >> 4) * 4, col = lane & 15;
-    for (int i = tid * 16; i < kSquare; i += 512 * 16)
-        *reinterpret_cast<u32x4 *>(sq_a + i) = *reinterpret_cast<const u32x4 *>(ws + area.sq(a_from) + i);
+    const int rb = wave / 2, cb = wave % 2 * CB, r = rb * 16 + (lane >> 4) * 4;
+    auto col_of = [&](int j) { return (cb + j) * 16 + (lane & 15); };
+    const float *diag = reinterpret_cast<const float *>(ws + area.diag);
+#pragma unroll
+    for (int j = 0; j < CB; ++j) {
+        const int c = col_of(j);
+        f32x4 v = get4(ws + area.sq(a_from) + unit_bytes(c, r, MP));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (r + e == c) v[e] = diag[c];
+        put_square(sq_a, diag_a, r, c, MP, v);
+    }
     __syncthreads();
-    // Q alternates between two places so that the last one is q_to
+    // Q alternates between two places so that the last one, whole, is q_to
     int q = (steps.count & 1) ? q_to : (q_to == SQ_Q0 ? SQ_Q1 : SQ_Q0);
-    f32x4 acc[RB][CB];
-    auto product = [&](const unsigned char *f, const unsigned char *h) {
+    f32x4 acc[CB];
+    auto product = [&](const unsigned char *f, const float *diag_f, const unsigned char *h, const float *diag_h, float scale) {
 #pragma unroll
-        for (int i = 0; i < RB; ++i) {
+        for (int j = 0; j < CB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        multiply_units<CB>(f, h, rb, cb, MP, acc);
 #pragma unroll
-            for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            multiply_units<CB>(f, h, rb + i, cb, MP, acc[i]);
+        for (int j = 0; j < CB; ++j) acc[j] = add_diagonals(acc[j], f, diag_f, h, diag_h, r, col_of(j), MP) * scale;
+    };
+    auto store = [&](unsigned char *to, float *diag_to, bool whole) {
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+            if (whole) put4(to + unit_bytes(col_of(j), r, MP), acc[j]);
+            else put_square(to, diag_to, r, col_of(j), MP, acc[j]);
         }
     };
-    auto store = [&](unsigned char *to, float scale) {
-#pragma unroll
-        for (int i = 0; i < RB; ++i)
-#pragma unroll
-            for (int j = 0; j < CB; ++j) put4(to + unit_bytes((cb + j) * 16 + col, (rb + i) * 16 + row, MP), acc[i][j] * scale);
-    };
+    const float *diag_s = diag_a;
     for (int s = 0; s < steps.count; ++s) {
         const OrthoSegmentStep &st = steps.step[s];
-        product(sq_a, sq_a);
+        const bool last = s + 1 == steps.count;
+        product(sq_a, diag_s, sq_a, diag_s, st.c);
 #pragma unroll
-        for (int i = 0; i < RB; ++i)
+        for (int j = 0; j < CB; ++j) {
+            const int c = col_of(j);
+            acc[j] += get_square(sq_a, diag_s, r, c, MP) * st.b;
 #pragma unroll
-            for (int j = 0; j < CB; ++j) {
-                const int r = (rb + i) * 16 + row, c = (cb + j) * 16 + col, o = unit_bytes(c, r, MP);
-                f32x4 v = get4(sq_a + o) * st.b + acc[i][j] * st.c;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += r + e == c ? st.a : 0.f;
-                put4(sq_p + o, v);
-                if (s == 0) put4(ws + area.sq(q) + o, v);                // the first step's P is Q
-            }
+            for (int e = 0; e < 4; ++e) acc[j][e] += r + e == c ? st.a : 0.f;
+        }
+        store(sq_p, diag_p, false);
+        if (s == 0) store(ws + area.sq(q), diag_q[q == SQ_Q1], last);     // the first step's P is Q
         __syncthreads();
         if (s > 0) {
             const int next = q == SQ_Q0 ? SQ_Q1 : SQ_Q0;
-            product(sq_p, ws + area.sq(q));
-            store(ws + area.sq(next), st.q_scale);
+            product(sq_p, diag_p, ws + area.sq(q), diag_q[q == SQ_Q1], st.q_scale);
+            store(ws + area.sq(next), diag_q[next == SQ_Q1], last);
             q = next;
         }
-        if (s + 1 < steps.count) {
-            product(sq_p, sq_a);
+        if (!last) {
+            product(sq_p, diag_p, sq_a, diag_s, st.t_scale);
             __syncthreads();                                             // everybody has read A
-            store(sq_a, st.t_scale);
+            store(sq_a, diag_t, false);
             __syncthreads();
-            product(sq_a, sq_p);
+            product(sq_a, diag_t, sq_p, diag_p, st.a_scale);
             __syncthreads();                                             // everybody has read T
-            store(sq_a, st.a_scale);
+            store(sq_a, diag_a, false);
         }
         __syncthreads();
     }
@@ -815,7 +904,7 @@ void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         s.a_scale = (float)std::ldexp(1.0, ka - 2 * kx);
         s.b = (float)std::ldexp(c[1], kb - ka);
         s.c = (float)std::ldexp(c[2], kb - 2 * ka);
-        s.ax = (float)std::ldexp(c[0], kn - kx);
+        s.ax = (float)std::ldexp(c[0], kb);
         s.y_scale = (float)std::ldexp(1.0, kn - kb - kx);
         kx = kn;
         rho = std::fmax(lpp_max, 1e-6);
@@ -830,7 +919,7 @@ void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         typedef decltype(type) T;
         if (widest <= 64) ortho_small_kernel<T, 64><<<blocks, 512, 0, st>>>(g, p, steps);
         else if (widest <= 128) ortho_small_kernel<T, 128><<<blocks, 512, 0, st>>>(g, p, steps);
-        else ortho_small_kernel<T, 256><<<blocks, 512, 0, st>>>(g, p, steps);
+        else ortho_small_kernel<T, kOrthoSmallCols><<<blocks, 512, 0, st>>>(g, p, steps);
     });
 }
 
@@ -977,8 +1066,8 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
             }
             if (segments) {
                 n = blocks(shapes, [](const OrthoArea &) { return 1; });
-                if (any64) ortho_segment_kernel<64><<<n, 512, 0, st>>>(shapes, all, a_from, q);
-                if (any128) ortho_segment_kernel<128><<<n, 512, 0, st>>>(shapes, all, a_from, q);
+                if (any64) ortho_segment_kernel<64><<<n, 64 * 8, 0, st>>>(shapes, all, a_from, q);
+                if (any128) ortho_segment_kernel<128><<<n, 128 * 8, 0, st>>>(shapes, all, a_from, q);
             }
             s.f = q; s.xt = xt;
             n = whole();

@@ -55,7 +55,7 @@ struct OrthoArea {
     int sub_tiles;               // of those on and above the diagonal
     int splits;                  // parts that the long side is cut into for X X^T
     int parts_used;              // partial sums of squares
-    size_t parts, x, xt0, sq0, partial, bytes;
+    size_t parts, x, xt0, sq0, diag, partial, bytes;     // diag: float32 diagonal of X X^T
     size_t wide, square;         // bytes of an m x n and of an m x m matrix
     __host__ __device__ size_t xt(int i) const { return xt0 + i * wide; }
     __host__ __device__ size_t sq(int i) const { return sq0 + i * square; }
@@ -84,6 +84,7 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     a.x = o; o += a.wide;
     a.xt0 = o; o += 2 * a.wide;
     a.sq0 = o; o += 6 * a.square;
+    a.diag = o; o += (size_t)a.mp * sizeof(float);
     a.partial = o;
     if (a.splits > 1) o += (size_t)a.splits * a.sub_tiles * a.sub * a.sub * sizeof(float);
     a.bytes = o;
@@ -91,11 +92,11 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
 }
 
 // A small matrix stays in one block's LDS from its first to its last step: X <- a X + (b A + c A^2) X as it is written.
-constexpr int kOrthoSmallRows = 64, kOrthoSmallCols = 256;
+constexpr int kOrthoSmallRows = 64, kOrthoSmallCols = 192;
 struct OrthoSmallStep {
     float a_scale;               // 2^(k_A - 2 k_X)
     float b, c;                  // b 2^(k_B - k_A), c 2^(k_B - 2 k_A)
-    float ax, y_scale;           // a 2^(k_X' - k_X), 2^(k_X' - k_B - k_X); the last step's k_X' is 0
+    float ax, y_scale;           // a 2^(k_B), 2^(k_X' - k_B - k_X); the last step's k_X' is 0
 };
 struct OrthoSmallSteps {
     float pow_kx;                // 2^(k_X) at the start
