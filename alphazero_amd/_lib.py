@@ -17,8 +17,8 @@ EVAL_NET, EVAL_CONST, EVAL_HASH_Q8, EVAL_HASH_F32, EVAL_ROLLOUT = 0, 1, 2, 3, 4
 EVALUATORS = {"net": EVAL_NET, "const": EVAL_CONST, "hash_q8": EVAL_HASH_Q8,
               "hash_f32": EVAL_HASH_F32, "rollout": EVAL_ROLLOUT}
 FLAG_LOCKSTEP = 1
-NET_F16, NET_F32, NET_F32S = 0, 1, 2
-PRECISIONS = {"f16": NET_F16, "f32": NET_F32, "f32s": NET_F32S}
+NET_F16, NET_F32, NET_F32S, NET_MX4 = 0, 1, 2, 3
+PRECISIONS = {"f16": NET_F16, "f32": NET_F32, "f32s": NET_F32S, "mx4": NET_MX4}
 MODES = {"compat": MODE_COMPAT, "az": MODE_AZ}
 
 

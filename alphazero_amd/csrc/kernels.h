@@ -77,6 +77,8 @@ struct NetWeights {            // one resident weight set, kernel layouts
     void *conv0_wh, *conv0_wl; // half [128][32]
     SplitScales *sp_scales;
     void *sp_maxbits;          // 4 x uint32 scratch of the weight preparation
+    // 4-bit linear layer (NNB_NET_MX4): units of [1024][11520], elements in the order of the activations
+    uint8_t *fc_codes, *fc_scales;
 };
 struct NetBuffers {            // activations, channels-last float32
     float *act1;               // [G][7][8][128]
@@ -100,6 +102,10 @@ struct NetBuffers {            // activations, channels-last float32
     // and meet through float32 activations [boards][(72 + 90) * 128] and two maximum words per board (zero between passes)
     float *spread_f32, *spread_f32_b1;
     uint32_t *spread_max, *spread_max_b1;
+    // 4-bit linear layer: the batch's rows quantised (units of [G][11520]), and float32 weights on their way to codes
+    uint8_t *row_codes, *row_codes_b1;
+    uint8_t *row_scales, *row_scales_b1;
+    float *fc_order;           // [1024][11520]
     int fc_pairs;              // ticket words per batch (the flag words follow them)
     int heads_all;             // 1: the linear layer's last step produces all 8 heads, 0: the value head only
     int write_hidden;          // 1: it also writes the hidden activations to `fc`
@@ -132,6 +138,8 @@ void launch_repack(hipStream_t st, const NetWeights &dst, const float *conv0_w, 
                    const float *fc_w, const float *fc_b, const float *policy_w, const float *policy_b,
                    const float *value_w, const float *value_b);
 void launch_planes_to_bits(hipStream_t st, int n, const float *planes, u64 *side);
+// Linear weight [1024][c * 90 + hw] -> [1024][hw * 128 + c], the order of a board's activations.
+void launch_order_fc(hipStream_t st, const float *fc_w, float *out);
 // One stage of the forward pass over `n_max` rows at most; the live row count is read
 // from *count_ptr on the device when count_ptr != nullptr, else it is n_max.
 void launch_net_stage(hipStream_t st, int stage, const NetWeights &w, const NetBuffers &b, const u64 *side,
@@ -141,7 +149,7 @@ void launch_net_stage(hipStream_t st, int stage, const NetWeights &w, const NetB
 // net_kernels_f16.hip: same stages with half activations / weights on v_mfma_f32_32x32x16_f16
 hipError_t prepare_net_kernels_f16();
 void launch_repack_f16(hipStream_t st, const NetWeights &dst, const float *conv2_w, const float *conv4_w,
-                       const float *fc_w);
+                       const float *fc_w);       // fc_w null: the convolutions alone
 void launch_net_stage_f16(hipStream_t st, int stage, const NetWeights &w, const NetBuffers &b, const u64 *side,
                           const uint8_t *legal, float *logp_out, float *value_out, float *prior_out,
                           const int32_t *count_ptr, int n_max);
@@ -170,6 +178,7 @@ struct Mx4Linear {                      // y [rows][n] = x * w^T (+ bias, ReLU)
     const int32_t *row_count;           // live rows, read on the device, or null
     long long rows, y_stride;
     int kp, n, bias_type, y_type, relu, wide;
+    long long order_rows;               // > 0: the sums are ordered as in a product of this many rows
 };
 struct Mx4Rows {                        // rows that are still numbers
     const void *x;
@@ -181,7 +190,7 @@ void launch_mx4_quantize(hipStream_t st, int type, long long rows, int cols, con
 void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, const uint8_t *codes, const uint8_t *scales,
                            void *out);
 // Few rows are quantised inside the product's own launch: then launch_mx4_linear takes them as `x`, not as codes.
-bool mx4_linear_fuses(long long rows, int cols);
+bool mx4_linear_fuses(long long rows, int cols, int n = 0, long long order_rows = 0);
 void launch_mx4_linear(hipStream_t st, Mx4Linear a, const Mx4Rows *x);
 
 // ortho_kernels.hip: Newton-Schulz orthogonalisation and the optimiser step on it.  The group's workspace holds an area

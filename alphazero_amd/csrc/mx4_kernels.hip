@@ -518,8 +518,6 @@ void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, c
     });
 }
 
-bool mx4_linear_fuses(long long rows, int cols) { return rows <= 16 && rows * mx4_padded(cols) <= kMx4FusedElements; }
-
 namespace {
 
 // Which kernel multiplies: the cheapest by these costs in microseconds (256 CUs; measured at rows 1 .. 2048 of 1024 x 11520,
@@ -528,17 +526,33 @@ namespace {
 //   128 x 128, one block of eight waves per CU (a ring of four stages)   3.5 + 0.6 per stage of 256 elements and 256 tiles
 //   128 x 128, two blocks of four waves per CU (two stages each)         3.5 + 0.9 per stage and 512 tiles
 //   256 x 256       8 + 1.65 per stage and 256 tiles
+// The rows kernel and the tiles add a row's products in different orders, but all forms of each in one: with `order_rows`
+// the choice between the two goes by that count, so that a row's results do not depend on how many come with it.
 // For example 1024 rows of 11520 -> 1024: 26 / 31 / 35 / 86 us in this order, 2048 rows of 1024 -> 8192: 95 / 30 / 23 / 25.
+struct ProductCosts {
+    double rows, one, two, large;
+    bool rows_form;
+};
+
+ProductCosts product_costs(long long rows, int n, int kp) {
+    auto rounds = [&](int r, int f, int at_once) {
+        const long long blocks = (rows + r - 1) / r * ((n + f - 1) / f);
+        return (double)((blocks + at_once - 1) / at_once);
+    };
+    const double stages = kp / 256;
+    ProductCosts c;
+    c.rows = 3.0 + rounds(64, 16, 256) * (1.2 + kp / 2300.0);
+    c.one = 3.5 + rounds(128, 128, 256) * stages * 0.6;
+    c.two = 3.5 + rounds(128, 128, 512) * stages * 0.9;
+    c.large = 8.0 + rounds(256, 256, 256) * stages * 1.65;
+    c.rows_form = rows <= 16 || (c.rows <= c.one && c.rows <= c.two && c.rows <= c.large);
+    return c;
+}
+
 template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
     auto tiles = [&](int r, int f) { return (a.rows + r - 1) / r * ((a.n + f - 1) / f); };
-    auto rounds = [](long long blocks, int at_once) { return (double)((blocks + at_once - 1) / at_once); };
-    const double stages = a.kp / 256;
-    const double rows_cost = 3.0 + rounds(tiles(64, 16), 256) * (1.2 + a.kp / 2300.0);
-    const double one_cost = 3.5 + rounds(tiles(128, 128), 256) * stages * 0.6;
-    const double two_cost = 3.5 + rounds(tiles(128, 128), 512) * stages * 0.9;
-    const double large_cost = 8.0 + rounds(tiles(256, 256), 256) * stages * 1.65;
-    const double tile_cost = one_cost < two_cost ? one_cost : two_cost;
-    if (a.rows <= 16 || rows_cost <= (tile_cost < large_cost ? tile_cost : large_cost)) {
+    const ProductCosts cost = product_costs(a.rows, a.n, a.kp);
+    if (a.order_rows > 0 ? product_costs(a.order_rows, a.n, a.kp).rows_form : cost.rows_form) {
         auto rows_form = [&](auto rt) {
             constexpr int RT = rt;
             mx4_rows_kernel<T, RT, float, false><<<(unsigned)tiles(RT * 16, 16), kRowsWaves * 64, 0, st>>>(a, nullptr, 0, 0, 0);
@@ -548,9 +562,9 @@ template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
         if (a.rows <= 16 || tiles(16, 16) <= 256) rows_form(std::integral_constant<int, 1>{});
         else if (a.rows <= 32 || tiles(32, 16) <= 256) rows_form(std::integral_constant<int, 2>{});
         else rows_form(std::integral_constant<int, 4>{});
-    } else if (large_cost <= tile_cost) {
+    } else if (cost.large <= cost.one && cost.large <= cost.two) {
         mx4_tile_kernel<T, 2, 2, 4, 4, 2, 1><<<(unsigned)tiles(256, 256), 256, 0, st>>>(a);
-    } else if (two_cost < one_cost) {
+    } else if (cost.two < cost.one) {
         mx4_tile_kernel<T, 2, 2, 2, 2, 2, 2><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
     } else {
         mx4_tile_kernel<T, 4, 2, 1, 2, 4, 3><<<(unsigned)tiles(128, 128), 512, 0, st>>>(a);
@@ -558,6 +572,11 @@ template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
 }
 
 }  // namespace
+
+bool mx4_linear_fuses(long long rows, int cols, int n, long long order_rows) {
+    return rows <= 16 && rows * mx4_padded(cols) <= kMx4FusedElements &&
+           (order_rows <= 0 || product_costs(order_rows, n, mx4_padded(cols)).rows_form);
+}
 
 void launch_mx4_linear(hipStream_t st, Mx4Linear a, const Mx4Rows *x) {
     with_dtype(a.y_type, [&](auto t) {

@@ -49,6 +49,14 @@ __global__ void repack_fc_kernel(const float *__restrict__ w, float *__restrict_
     wp[i] = w[(size_t)n * 11520 + c * 90 + hw];
 }
 
+// Linear weight [n=1024][c*90 + hw] -> [n][kk], kk = hw*128 + c
+__global__ void order_fc_kernel(const float *__restrict__ w, float *__restrict__ out) {
+    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (size_t)1024 * 11520) return;
+    const int n = (int)(i / 11520), kk = (int)(i % 11520), hw = kk >> 7, c = kk & 127;
+    out[i] = w[(size_t)n * 11520 + c * 90 + hw];
+}
+
 // policy_head [7][1024] + value_head [1][1024] -> [8][1024]; biases -> [8].
 __global__ void repack_heads_kernel(const float *__restrict__ pw, const float *__restrict__ pb,
                                     const float *__restrict__ vw, const float *__restrict__ vb,
@@ -387,6 +395,10 @@ void launch_repack(hipStream_t st, const NetWeights &dst, const float *conv0_w, 
     if (dst.fc_w) repack_fc_kernel<<<(1024 * 11520) / 256, 256, 0, st>>>(fc_w, dst.fc_w);
     copy_kernel<<<4, 256, 0, st>>>(fc_b, dst.fc_b, 1024);
     repack_heads_kernel<<<32, 256, 0, st>>>(policy_w, policy_b, value_w, value_b, dst.heads_w, dst.heads_b);
+}
+
+void launch_order_fc(hipStream_t st, const float *fc_w, float *out) {
+    order_fc_kernel<<<(1024 * 11520) / 256, 256, 0, st>>>(fc_w, out);
 }
 
 void launch_planes_to_bits(hipStream_t st, int n, const float *planes, u64 *side) {

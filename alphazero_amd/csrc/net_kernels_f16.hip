@@ -793,7 +793,7 @@ void launch_repack_f16(hipStream_t st, const NetWeights &dst, const float *conv2
                        const float *fc_w) {
     repack_conv_f16_kernel<<<cdiv16(128 * 128 * 16, 256), 256, 0, st>>>(conv2_w, (_Float16 *)dst.conv2_wh);
     repack_conv_f16_kernel<<<cdiv16(128 * 128 * 16, 256), 256, 0, st>>>(conv4_w, (_Float16 *)dst.conv4_wh);
-    repack_fc_f16_kernel<<<(1024 * 11520) / 256, 256, 0, st>>>(fc_w, (_Float16 *)dst.fc_wh);
+    if (fc_w) repack_fc_f16_kernel<<<(1024 * 11520) / 256, 256, 0, st>>>(fc_w, (_Float16 *)dst.fc_wh);
 }
 
 void launch_net_stage_f16(hipStream_t st, int stage, const NetWeights &w, const NetBuffers &b, const u64 *side,

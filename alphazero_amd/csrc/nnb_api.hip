@@ -192,6 +192,8 @@ size_t carve(const nnb_config &cfg, Carver &c, EngineDev &d, NetBuffers &b, std:
     b.sync_err = d.counters ? d.counters + kSyncErr : nullptr;
     b.clk = c.take<unsigned long long>(8);              // profiling stamps; kernels get the pointer only while profiling is on
     b.fcq = b.fcq_b1 = b.fchand = b.fchand_b1 = nullptr;
+    b.row_codes = b.row_codes_b1 = b.row_scales = b.row_scales_b1 = nullptr;
+    b.fc_order = nullptr;
     b.heads_all = 1; b.write_hidden = 0;
     c.take<unsigned char>(kAlign);
     const size_t state_bytes = c.off;
@@ -231,9 +233,21 @@ size_t carve(const nnb_config &cfg, Carver &c, EngineDev &d, NetBuffers &b, std:
         b.act1 = nullptr;
         b.act2 = reinterpret_cast<float *>(c.take<uint16_t>(G * 72 * 128));
         b.act3 = reinterpret_cast<float *>(c.take<uint16_t>(G * 90 * 128));
-        b.fc = b.fc_b1 = nullptr;
-        b.fcpart = c.take<float>(2 * G * 1024);
-        b.fcpart_b1 = c.take<float>(2 * G * 1024);
+        if (cfg.net_precision == NNB_NET_MX4) {
+            const size_t units = mx4_units((long long)G, 11520);
+            b.fc = c.take<float>(G * 1024);
+            b.fc_b1 = c.take<float>(G * 1024);
+            b.fcpart = b.fcpart_b1 = nullptr;
+            b.row_codes = c.take<uint8_t>(units * 4096);
+            b.row_codes_b1 = c.take<uint8_t>(units * 4096);
+            b.row_scales = c.take<uint8_t>(units * 256);
+            b.row_scales_b1 = c.take<uint8_t>(units * 256);
+            b.fc_order = c.take<float>((size_t)1024 * 11520);
+        } else {
+            b.fc = b.fc_b1 = nullptr;
+            b.fcpart = c.take<float>(2 * G * 1024);
+            b.fcpart_b1 = c.take<float>(2 * G * 1024);
+        }
         const bool two = true;
         b.act1_b1 = nullptr;
         b.act2_b1 = two ? reinterpret_cast<float *>(c.take<uint16_t>(G * 72 * 128)) : nullptr;
@@ -245,13 +259,14 @@ size_t carve(const nnb_config &cfg, Carver &c, EngineDev &d, NetBuffers &b, std:
         s.conv0_w = c.take<float>(128 * 32);  s.conv0_b = c.take<float>(128);
         const bool f32 = cfg.net_precision == NNB_NET_F32;
         const bool split = cfg.net_precision == NNB_NET_F32S;
+        const bool mx4 = cfg.net_precision == NNB_NET_MX4;
         s.conv2_b = c.take<float>(128); s.conv4_b = c.take<float>(128); s.fc_b = c.take<float>(1024);
         s.conv2_w = f32 ? c.take<float>(128 * 128 * 16) : nullptr;
         s.conv4_w = f32 ? c.take<float>(128 * 128 * 16) : nullptr;
         s.fc_w = f32 ? c.take<float>((size_t)1024 * 11520) : nullptr;
         s.conv2_wh = f32 ? nullptr : (void *)c.take<uint16_t>(128 * 128 * 16);
         s.conv4_wh = f32 ? nullptr : (void *)c.take<uint16_t>(128 * 128 * 16);
-        s.fc_wh = f32 ? nullptr : (void *)c.take<uint16_t>((size_t)1024 * 11520);
+        s.fc_wh = f32 || mx4 ? nullptr : (void *)c.take<uint16_t>((size_t)1024 * 11520);
         s.conv2_wl = split ? (void *)c.take<uint16_t>(128 * 128 * 16) : nullptr;
         s.conv4_wl = split ? (void *)c.take<uint16_t>(128 * 128 * 16) : nullptr;
         s.fc_wl = split ? (void *)c.take<uint16_t>((size_t)1024 * 11520) : nullptr;
@@ -259,6 +274,8 @@ size_t carve(const nnb_config &cfg, Carver &c, EngineDev &d, NetBuffers &b, std:
         s.conv0_wl = split ? (void *)c.take<uint16_t>(128 * 32) : nullptr;
         s.sp_scales = split ? c.take<SplitScales>(1) : nullptr;
         s.sp_maxbits = split ? (void *)c.take<uint32_t>(4) : nullptr;
+        s.fc_codes = mx4 ? c.take<uint8_t>(mx4_units(1024, 11520) * 4096) : nullptr;
+        s.fc_scales = mx4 ? c.take<uint8_t>(mx4_units(1024, 11520) * 256) : nullptr;
         s.heads_w = c.take<float>(8 * 1024);  s.heads_b = c.take<float>(8);
     }
     c.take<unsigned char>(kAlign);          // tail pad
@@ -273,7 +290,8 @@ int check_cfg(const nnb_config *cfg) {
         return fail(NNB_ERR_ARG, "max_sims %d out of range [1, %d]", cfg->max_sims, kMaxSims);
     if (cfg->n_weight_sets < 1 || cfg->n_weight_sets > 8)
         return fail(NNB_ERR_ARG, "n_weight_sets %d out of range [1, 8]", cfg->n_weight_sets);
-    if (cfg->net_precision != NNB_NET_F16 && cfg->net_precision != NNB_NET_F32 && cfg->net_precision != NNB_NET_F32S)
+    if (cfg->net_precision != NNB_NET_F16 && cfg->net_precision != NNB_NET_F32 && cfg->net_precision != NNB_NET_F32S &&
+        cfg->net_precision != NNB_NET_MX4)
         return fail(NNB_ERR_ARG, "net_precision %d out of range", cfg->net_precision);
     const int cs = cfg->eval_cache_slots;
     if (cs != 0 && (cs < 0 || cs > 65536 || (cs & (cs - 1)) != 0))
@@ -362,12 +380,33 @@ int check_params(nnb_engine *e, const nnb_search_params *p, int n) {
     return NNB_OK;
 }
 
+// The linear layer on 4-bit floats: the activations' rows quantised, then multiplied.  The sums are ordered by the
+// engine's capacity, so that a position's outputs do not depend on its batch.
+void mx4_fc(hipStream_t st, const NetWeights &w, const NetBuffers &b, const int32_t *count_ptr, int n_max) {
+    if (n_max <= 0) return;
+    Mx4Linear a = {};
+    a.x_codes = b.row_codes; a.x_scales = b.row_scales; a.w_codes = w.fc_codes; a.w_scales = w.fc_scales;
+    a.bias = w.fc_b; a.bias_type = NNB_F32; a.y = b.fc; a.y_type = NNB_F32; a.y_stride = 1024;
+    a.row_count = count_ptr; a.rows = n_max; a.kp = mx4_padded(11520); a.n = 1024; a.relu = 1; a.order_rows = b.max_rows;
+    if (mx4_linear_fuses(n_max, 11520, 1024, b.max_rows)) {
+        const Mx4Rows x = {b.act3, 11520, 1, NNB_F16, 11520};
+        launch_mx4_linear(st, a, &x);
+        return;
+    }
+    launch_mx4_quantize(st, NNB_F16, n_max, 11520, b.act3, 11520, 1, count_ptr, b.row_codes, b.row_scales);
+    launch_mx4_linear(st, a, nullptr);
+}
+
 void net_stage(nnb_engine *e, hipStream_t st, int stage, const NetWeights &w, const NetBuffers &b, const u64 *side,
                const uint8_t *legal, float *logp, float *value, float *prior, const int32_t *count_ptr, int n_max) {
     if (e->cfg.net_precision == NNB_NET_F32)
         launch_net_stage(st, stage, w, b, side, legal, logp, value, prior, count_ptr, n_max);
     else if (e->cfg.net_precision == NNB_NET_F32S)
         launch_net_stage_split(st, stage, w, b, side, legal, logp, value, prior, count_ptr, n_max);
+    else if (e->cfg.net_precision == NNB_NET_MX4 && stage == NET_FC)
+        mx4_fc(st, w, b, count_ptr, n_max);
+    else if (e->cfg.net_precision == NNB_NET_MX4 && stage == NET_HEADS)       // they read float32 rows, as there
+        launch_net_stage(st, stage, w, b, side, legal, logp, value, prior, count_ptr, n_max);
     else
         launch_net_stage_f16(st, stage, w, b, side, legal, logp, value, prior, count_ptr, n_max);
 }
@@ -384,6 +423,7 @@ NetBuffers batch_buffers(const nnb_engine *e, int batch) {
         b.act1 = b.act1_b1; b.act2 = b.act2_b1; b.act3 = b.act3_b1;
         b.act2_inv = b.act2_inv_b1; b.act3_inv = b.act3_inv_b1;
         b.spread_f32 = b.spread_f32_b1; b.spread_max = b.spread_max_b1;
+        b.row_codes = b.row_codes_b1; b.row_scales = b.row_scales_b1;
     }
     return b;
 }
@@ -391,8 +431,8 @@ NetBuffers batch_buffers(const nnb_engine *e, int batch) {
 HeadsDev heads_input(const nnb_engine *e, int weight_set, int batch) {
     const NetBuffers b = batch_buffers(e, batch);
     if (e->cfg.net_precision == NNB_NET_F32S) return heads_input_split(e->weights[weight_set], b);
-    return e->cfg.net_precision == NNB_NET_F32 ? heads_input_f32(e->weights[weight_set], b)
-                                               : heads_input_f16(e->weights[weight_set], b);
+    return e->cfg.net_precision == NNB_NET_F16 ? heads_input_f16(e->weights[weight_set], b)
+                                               : heads_input_f32(e->weights[weight_set], b);
 }
 
 // Forward pass over one of the engine's compacted leaf batches (count on the device).  With
@@ -728,7 +768,8 @@ int run_free_rounds(nnb_engine *e, hipStream_t st, const nnb_search_params &para
     // pass, and the CUs that the last blocks of one kernel leave idle take blocks of the other half's kernels.
     // Games do not interact, so the records are the same byte for byte.
     // Measured on 4096 slots x 200 simulations: +5 % games/s with the float32-faithful kernels (one block per CU,
-    // long tails), -3 % with the half-input kernels (two blocks per CU already overlap), so those keep one chain.
+    // long tails), -3 % with the half-input kernels (two blocks per CU already overlap), so those keep one chain;
+    // with the 4-bit linear layer 448 ms against 465 (100 simulations).
     const bool wanted = (p->flags & NNB_FLAG_TWO_STREAMS) ||
                         (slots >= kHalvesMinSlots && e->cfg.net_precision != NNB_NET_F16);
     const bool halves = plan.nbatch == 1 && slots >= 2 * kStepGamesHost && wanted && !(p->flags & NNB_FLAG_ONE_STREAM);
@@ -963,6 +1004,12 @@ int nnb_load_weights(nnb_engine *e, int weight_set, void *stream, const float *c
     launch_repack(st, e->weights[weight_set], conv0_w, conv0_b, conv2_w, conv2_b, conv4_w, conv4_b, fc_w, fc_b,
                   policy_w, policy_b, value_w, value_b);
     if (e->cfg.net_precision == NNB_NET_F16) launch_repack_f16(st, e->weights[weight_set], conv2_w, conv4_w, fc_w);
+    if (e->cfg.net_precision == NNB_NET_MX4) {
+        launch_repack_f16(st, e->weights[weight_set], conv2_w, conv4_w, nullptr);
+        launch_order_fc(st, fc_w, e->buf.fc_order);
+        launch_mx4_quantize(st, NNB_F32, 1024, 11520, e->buf.fc_order, 11520, 1, nullptr, e->weights[weight_set].fc_codes,
+                            e->weights[weight_set].fc_scales);
+    }
     if (e->cfg.net_precision == NNB_NET_F32S)
         launch_repack_split(st, e->weights[weight_set], conv0_w, conv0_b, conv2_w, conv4_w, fc_w);
     HIP_TRY(hipGetLastError());
@@ -1070,7 +1117,7 @@ int nnb_debug_activations(nnb_engine *e, int weight_set, void *stream, int layer
     if (layer == 4) {
         const size_t total = (size_t)n * 1024;
         const unsigned blocks = (unsigned)((total + 255) / 256);
-        if (prec == NNB_NET_F32 || prec == NNB_NET_F32S) debug_act_kernel<<<blocks, 256, 0, st>>>(0, b.fc, nullptr, nullptr, total, out);
+        if (prec != NNB_NET_F16) debug_act_kernel<<<blocks, 256, 0, st>>>(0, b.fc, nullptr, nullptr, total, out);
         else debug_act_kernel<<<blocks, 256, 0, st>>>(2, b.fcpart, b.fcpart + (size_t)b.max_rows * 1024,
                                                       e->weights[weight_set].fc_b, total, out);
     } else {

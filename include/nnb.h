@@ -91,8 +91,8 @@ enum nnb_flags {
     /* nnb_selfplay_round on the lock-step path with one network.  The slots can be split in two halves
      * that run their tree step -> forward pass chains on two streams, unsynchronised, so that one half's
      * tree step and the idle tail of its kernels hide under the other half's forward pass.  Same games
-     * either way.  Default: two streams from 1024 slots on with NNB_NET_F32S / NNB_NET_F32, one stream with
-     * NNB_NET_F16 (where it measured slower).  ONE_STREAM / TWO_STREAMS force the choice. */
+     * either way.  Default: two streams from 1024 slots on with NNB_NET_F32S, NNB_NET_F32 and NNB_NET_MX4, one
+     * stream with NNB_NET_F16 (where it measured slower).  ONE_STREAM / TWO_STREAMS force the choice. */
     NNB_FLAG_ONE_STREAM = 16,
     NNB_FLAG_TWO_STREAMS = 32,
     /* Accepted and ignored (it once selected a two-launch form of the NNB_NET_F32S convolutions; one kernel now
@@ -107,8 +107,11 @@ enum nnb_flags {
  *   NNB_NET_F32 : float32 inputs, v_mfma_f32_32x32x2_f32 (exact f32 FMA chains, 1/16 the rate);
  *   NNB_NET_F32S: float32-faithful on the half-input matrix cores: every float32 operand is carried as
  *                 a scaled hi + lo pair of halves (2^-22 relative), three MFMAs per product, a third of
- *                 the NNB_NET_F16 rate; as close to the float32 forward as NNB_NET_F32 is. */
-enum nnb_precision { NNB_NET_F16 = 0, NNB_NET_F32 = 1, NNB_NET_F32S = 2 };
+ *                 the NNB_NET_F16 rate; as close to the float32 forward as NNB_NET_F32 is;
+ *   NNB_NET_MX4 : convolutions as NNB_NET_F16; the linear layer's weights and activations as 4-bit floats with a
+ *                 power-of-two scale per 32 elements (see nnb_mx4_linear; blocks of 32 channels of one cell), so
+ *                 its outputs are those of the rounded weights and activations, some percent off. */
+enum nnb_precision { NNB_NET_F16 = 0, NNB_NET_F32 = 1, NNB_NET_F32S = 2, NNB_NET_MX4 = 3 };
 
 typedef struct nnb_config {
     int32_t max_games;   /* concurrent games / root positions per call (>= 1)      */
