@@ -39,3 +39,27 @@ def ptr(t: torch.Tensor) -> C.c_void_p:
 def no_grad(what: str, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NnbError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def _span(t: torch.Tensor) -> tuple:
+    """First and last address + 1 of the elements (torch's strides are never negative)."""
+    reach = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (reach + 1) * t.element_size()
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors may have elements in common.  Column ranges of one buffer that lie apart are recognised; of
+    other interleaved views it is assumed."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    strides = [s * t.element_size() for t in (a, b) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1]
+    if strides and a.stride(-1) == 1 and b.stride(-1) == 1:
+        row = min(strides)
+        if row > 0 and all(s % row == 0 for s in strides):
+            gap = (b0 - a0) % row                        # from a's columns to b's, around the row
+            if gap >= a.shape[-1] * a.element_size() and gap + b.shape[-1] * b.element_size() <= row:
+                return False
+    return True

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import Mx4LinearArgs, check
-from ._tensors import dtype_code, no_grad, on_device, ptr, stream_of
+from ._tensors import dtype_code, no_grad, on_device, ptr, share_memory, stream_of
 
 BLOCK = 32                              # elements that share a scale
 UNIT_ROWS, UNIT_COLS = 32, 256          # rows and columns are padded with zeros to whole units
@@ -108,8 +108,8 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
     """x [..., K] times weight [N, K] transposed, plus bias [N], then ReLU if asked: [..., N].
 
     x may be numbers (quantised inside the call) or an MX4Tensor.  Products are exact, sums, bias and ReLU in float32,
-    one rounding to `out_dtype` (default: x's type, float32 for an MX4Tensor).  `out` ([..., N], rows contiguous) is
-    written instead of a new tensor when given."""
+    one rounding to `out_dtype` (default: x's type, float32 for an MX4Tensor).  `out` ([..., N], rows contiguous, no
+    element in common with the inputs) is written instead of a new tensor when given."""
     if not isinstance(weight, MX4Tensor) or len(weight.shape) != 2:
         raise ValueError("weight must be a two-dimensional MX4Tensor (mx4.quantize)")
     quantized = isinstance(x, MX4Tensor)
@@ -135,6 +135,11 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
             out = torch.empty(y_shape, dtype=out_dtype, device=device)
         elif tuple(out.shape) != y_shape or out.dtype != out_dtype:
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, expected {out_dtype} {y_shape}")
+        else:
+            if any(t is not None and share_memory(out, t) for t in ((x.codes, x.scales) if quantized else (x,))
+                   + (weight.codes, weight.scales, bias)):
+                raise ValueError("out shares memory with an input")
+            torch.autograd.graph.increment_version(out)              # the kernels write behind torch's back
         no_grad("mx4.linear", out)
         y_stride = n if out.is_contiguous() else _row_stride(out, n)
         args = Mx4LinearArgs()

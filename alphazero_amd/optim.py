@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._lib import NS_MAX_STEPS, MuonMatrix, MuonParams, NewtonSchulz, check
-from ._tensors import dtype_code, no_grad, on_device, ptr, stream_of
+from ._tensors import dtype_code, no_grad, on_device, ptr, share_memory, stream_of
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
@@ -50,7 +50,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=QUINTIC, eps: fl
     times X <- a X + b (X X^T) X + c (X X^T)^2 X: the singular values go towards 1, the singular vectors stay.
 
     float32-faithful inside whatever the type, one rounding at the end.  A matrix with a NaN or an infinity gives NaN.
-    `out` (same shape and type, may be x itself) is written instead of a new tensor when given.  No backward pass."""
+    `out` (same shape and type; x itself, or no element in common with it) is written instead of a new tensor when given.  No backward pass."""
     code = dtype_code(x, "x")
     no_grad("optim.orthogonalize", x, out)
     if x.dim() < 2:
@@ -58,6 +58,9 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=QUINTIC, eps: fl
     ns = _newton_schulz(steps, coefficients, eps)
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device):
         raise ValueError(f"out is {out.dtype} {tuple(out.shape)} on {out.device}, expected {x.dtype} {tuple(x.shape)} on {x.device}")
+    given = out
+    if out is not None and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) and share_memory(out, x):
+        raise ValueError("out shares memory with x but is not x")
     with on_device(x):
         x = x.detach()
         if out is None:
@@ -77,6 +80,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=QUINTIC, eps: fl
         strides = C.c_int64 * 3
         check(lib.nnb_orthogonalize(stream_of(x), code, xb.shape[0], rows, cols, ptr(xb), strides(*xb.stride()), ptr(ob),
                                     strides(*ob.stride()), C.byref(ns), ptr(workspace), nbytes.value), "nnb_orthogonalize")
+    if given is not None:
+        torch.autograd.graph.increment_version(given)             # the kernels write behind torch's back
     return out
 
 
@@ -97,7 +102,8 @@ def muon_update(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
         m' = momentum m + g;   u = g + momentum m' (nesterov) or m'
         w' = w (1 - lr weight_decay) - lr max(1, rows / cols)^(1/2) orthogonalize(u)
 
-    weights and grads of one type (float32, float16, bfloat16), momenta float32, all contiguous on one device.  Returns
+    weights and grads of one type (float32, float16, bfloat16), momenta float32, all contiguous on one device, without
+    elements in common.  Returns
     (weights, momenta): the given tensors, updated, or new ones with inplace=False."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
@@ -116,9 +122,11 @@ def muon_update(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
         if any(t.device != first.device for t in (w, g, m)):
             raise ValueError(f"matrix {i}: all tensors must be on {first.device}")
     if inplace:
-        written = [t.data_ptr() for t in weights + momenta if t.numel()]
-        if len(set(written)) != len(written):
-            raise ValueError("a tensor appears twice among the weights and momenta")
+        used = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written)
+                      for ts, written in ((weights, True), (momenta, True), (grads, False)) for t in ts if t.numel())
+        for (_, end, a), (start, _, b) in zip(used, used[1:]):
+            if end > start and (a or b):
+                raise ValueError("a weight or momentum shares memory with another tensor of the call")
     with on_device(first):
         wv = [_as_matrix(t, f"weights[{i}]") for i, t in enumerate(weights)]
         gv = [_as_matrix(t, f"grads[{i}]") for i, t in enumerate(grads)]

@@ -11,7 +11,9 @@ trajectories are all-gathered once per round (`gather_trajectories`).
 from __future__ import annotations
 
 import logging
-from typing import List, Tuple
+import os
+import time
+from typing import List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -169,12 +171,62 @@ def self_play_sample_tensors(agent, num_games, first_game_id: int = 0):
     return eng.trajectory_samples(traj)
 
 
+def train_network(agent, planes: torch.Tensor, probs: torch.Tensor, z: torch.Tensor, epochs: int = 1, batch_size: int = 32,
+                  lr: float = 1e-3, muon_lr: float = 0.02, weight_decay: float = 0.0,
+                  time_limit: Optional[float] = None, seed: int = 0) -> List[float]:
+    """Fits agent.model to samples as self_play_sample_tensors returns them, with the reference's loss
+    (lightning_module.py:20-27): KL divergence of the policy from the visit distribution plus mean squared error of
+    the value.  The hidden weights are stepped by optim.Muon, heads and biases by Adam.  Samples are drawn in a new
+    order each epoch (from `seed`).  Ends after `epochs`, or with the batch that `time_limit` seconds run out in.
+    Returns each epoch's mean loss.  The network has to be on the GPU (use_gpu=True): Muon has no CPU path."""
+    from . import optim
+    n = int(planes.shape[0])
+    if probs.shape[0] != n or z.shape[0] != n:
+        raise ValueError(f"{n} positions, {probs.shape[0]} distributions and {z.shape[0]} results")
+    if epochs < 1 or batch_size < 1:
+        raise ValueError(f"epochs {epochs} and batch_size {batch_size} must be at least 1")
+    if n == 0:
+        return []
+    device = next(agent.model.parameters()).device
+    planes, probs, z = planes.to(device), probs.to(device), z.to(device=device, dtype=torch.float32)
+    matrices, rest = optim.split_parameters(agent.model)
+    optimizers = [optim.Muon(matrices, lr=muon_lr, weight_decay=weight_decay),
+                  torch.optim.Adam(rest, lr=lr, weight_decay=weight_decay)]
+    generator = torch.Generator().manual_seed(int(seed))
+    start, losses = time.monotonic(), []
+    for _ in range(epochs):
+        order = torch.randperm(n, generator=generator).to(device)
+        total, seen, in_time = torch.zeros((), device=device), 0, True
+        for first in range(0, n, batch_size):
+            rows = order[first:first + batch_size]
+            log_policy, value = agent.model(planes[rows])
+            loss = (torch.nn.functional.kl_div(log_policy, probs[rows], reduction="batchmean")
+                    + torch.nn.functional.mse_loss(value[:, 0], z[rows]))
+            for optimizer in optimizers:
+                optimizer.zero_grad()
+            loss.backward()
+            for optimizer in optimizers:
+                optimizer.step()
+            total += loss.detach() * len(rows)
+            seen += len(rows)
+            in_time = time_limit is None or time.monotonic() - start < time_limit
+            if not in_time:
+                break
+        losses.append(total.item() / seen)
+        logger.info("epoch %d: loss %.4f over %d samples", len(losses), losses[-1], seen)
+        if not in_time:
+            break
+    return losses
+
+
 def train_alphazero(time_limit, num_self_play_games=100, use_gpu=True, load_model=True):
-    """Entry point kept for import compatibility (train_alpha_zero.py:57-119).  The self-play half
-    runs on the engine; the Lightning training half is not part of this package."""
-    from .agent import initialize_agent
+    """train_alpha_zero.py:57-119: self-play, then training on its per-ply samples for `time_limit` seconds, ten
+    epochs at most, then the network is saved to agent.MODEL_PATH.  Returns the agent."""
+    from .agent import MODEL_PATH, initialize_agent
     agent = initialize_agent(action_dim=7, state_dim=2, use_gpu=use_gpu, num_simulations=800, c_puct=1.4,
                              load_model=load_model)
-    self_play(agent, num_self_play_games)
-    raise NotImplementedError("self-play finished and agent.memory is filled; the pytorch_lightning trainer of "
-                              "the reference (train_alpha_zero.py:79-115) is outside this package")
+    planes, probs, z = self_play_sample_tensors(agent, num_self_play_games)
+    train_network(agent, planes, probs, z, epochs=10, time_limit=time_limit)
+    os.makedirs(os.path.dirname(MODEL_PATH), exist_ok=True)
+    agent.save_model(MODEL_PATH)
+    return agent

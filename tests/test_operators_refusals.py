@@ -195,3 +195,17 @@ def test_optimiser_python_refusals():
         optim.Muon([torch.nn.Parameter(x[0])])
     with pytest.raises(ValueError):
         optim.Muon([torch.nn.Parameter(x.t())])
+
+
+def test_which_tensors_share_memory():
+    import torch
+    from alphazero_amd._tensors import share_memory
+    buf = torch.zeros(8, 100)
+    assert share_memory(buf, buf) and share_memory(buf[2:5], buf[4:]) and share_memory(buf[0], buf[:, 0])
+    assert not share_memory(buf[:4], buf[4:]) and not share_memory(buf, torch.zeros(8, 100)) and not share_memory(buf[:0], buf)
+    assert not share_memory(buf[:, :40], buf[:, 40:]) and not share_memory(buf[:, 40:], buf[:, :40])
+    assert share_memory(buf[:, :41], buf[:, 40:]) and share_memory(buf[:, 40:], buf[:, :41])
+    assert share_memory(buf[:, 60:], buf.view(-1)[90:].unfold(0, 20, 100))          # the second wraps around the row's end
+    assert not share_memory(buf[:, 20:40], buf[1:, :20]) and not share_memory(buf[1:, :20], buf[:, 20:40])
+    half = torch.zeros(8, 100, dtype=torch.float16)
+    assert not share_memory(half[:, :50], half[:, 50:]) and share_memory(half[::2, :60], half[1:, 50:])
