@@ -756,80 +756,139 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoPar
     }
 }
 
-// All products of a segment for a matrix with m <= 128: A comes from memory, Q goes there, a block each, a wave per 16 rows and half the
-// columns;
-// A (then T, then the next A) and P stay in LDS, Q is read back from memory where it is multiplied.
-template <int MP>
-__global__ __launch_bounds__(MP * 8) void ortho_segment_kernel(OrthoShapes g, OrthoSegmentSteps steps, int a_from, int q_to) {
-    constexpr int kSquare = MP * MP * 4, CB = MP / 32;                   // a wave's blocks of 16 columns
+// All products of a segment for a matrix with m <= 128 in one block, a wave per B x B blocks of 16: A comes from memory, Q
+// goes there.  The units of A (then T, then the next A) and of P stay in LDS, Q's are read back from memory; every wave
+// keeps its own part of A, P and Q in float32 registers, so that the products with the diagonals cost two operations per
+// element: read back from the units, they and the conversions took most of the time (128 x 128, three steps: 43.5 us, now
+// 29.4; their matrix instructions alone 12).
+template <int MP, int B>
+__global__ __launch_bounds__(MP / 16 / B * (MP / 16 / B) * 64) void ortho_segment_kernel(OrthoShapes g, OrthoSegmentSteps steps, int a_from,
+                                                                                      int q_to) {
+    constexpr int kSquare = MP * MP * 4, kSide = MP / 16 / B;
     __shared__ __attribute__((aligned(16))) unsigned char sq_a[kSquare], sq_p[kSquare];
-    __shared__ float diag_a[MP], diag_t[MP], diag_p[MP], diag_q[2][MP];
+    __shared__ __attribute__((aligned(16))) float diag_a[MP], diag_t[MP], diag_p[MP], diag_q[2][MP];
     int batch;
     const OrthoShape &it = g.item[find_item(g, blockIdx.x, batch)];
     const OrthoArea area = ortho_area(it.rows, it.cols);
     if (area.mp != MP) return;                                           // the other size's launch takes it
     unsigned char *ws = g.ws + it.ws + batch * it.ws_stride;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rb = wave / 2, cb = wave % 2 * CB, r = rb * 16 + (lane >> 4) * 4;
-    auto col_of = [&](int j) { return (cb + j) * 16 + (lane & 15); };
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rb = wave / kSide * B, cb = wave % kSide * B;              // this wave's first blocks
+    const bool diagonal = rb == cb;                                      // its blocks i, i hold the diagonal
+    auto row = [&](int i) { return (rb + i) * 16 + (lane >> 4) * 4; };
+    auto col = [&](int j) { return (cb + j) * 16 + (lane & 15); };
+    auto at = [&](int i, int j) { return unit_bytes(col(j), row(i), MP); };
+    typedef f32x4 Part[B][B];
+    Part own_a, own_p, own_q, acc;
+    auto store = [&](unsigned char *to, float *diag, const Part &v) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                if (diagonal && i == j) put_square(to, diag, row(i), col(j), MP, v[i][j]);
+                else put4(to + at(i, j), v[i][j]);
+            }
+    };
+    // acc = scale F G
+    auto product = [&](const unsigned char *f, const float *diag_f, const Part &own_f, const unsigned char *h, const float *diag_h,
+                       const Part &own_h, float scale) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int j = 0; j < B; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int k = 0; k < MP / 32; ++k) {
+            half8 fh[B], fl[B], gh[B], gl[B];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const unsigned char *fu = f + ((rb + i) * (MP / 32) + k) * 2048 + lane * 16, *gu = h + ((cb + i) * (MP / 32) + k) * 2048 + lane * 16;
+                fh[i] = *reinterpret_cast<const half8 *>(fu), fl[i] = *reinterpret_cast<const half8 *>(fu + 1024);
+                gh[i] = *reinterpret_cast<const half8 *>(gu), gl[i] = *reinterpret_cast<const half8 *>(gu + 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i) add_to<B>(fh[i], fl[i], gh, gl, acc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const f32x4 df = *reinterpret_cast<const f32x4 *>(diag_f + row(i));
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                f32x4 of = own_f[i][j];
+                if (diagonal && i == j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (row(i) + e == col(j)) of[e] = 0.f;
+                acc[i][j] = (acc[i][j] + df * own_h[i][j] + of * diag_h[col(j)]) * scale;
+            }
+        }
+    };
     const float *diag = reinterpret_cast<const float *>(ws + area.diag);
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
-        const int c = col_of(j);
-        f32x4 v = get4(ws + area.sq(a_from) + unit_bytes(c, r, MP));
+    for (int i = 0; i < B; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (r + e == c) v[e] = diag[c];
-        put_square(sq_a, diag_a, r, c, MP, v);
-    }
+        for (int j = 0; j < B; ++j) {
+            own_a[i][j] = get4(ws + area.sq(a_from) + at(i, j));
+            if (diagonal && i == j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (row(i) + e == col(j)) own_a[i][j][e] = diag[col(j)];
+        }
+    store(sq_a, diag_a, own_a);
     __syncthreads();
     // Q alternates between two places so that the last one, whole, is q_to
     int q = (steps.count & 1) ? q_to : (q_to == SQ_Q0 ? SQ_Q1 : SQ_Q0);
-    f32x4 acc[CB];
-    auto product = [&](const unsigned char *f, const float *diag_f, const unsigned char *h, const float *diag_h, float scale) {
+    auto store_q = [&](bool last) {
 #pragma unroll
-        for (int j = 0; j < CB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        multiply_units<CB>(f, h, rb, cb, MP, acc);
+        for (int i = 0; i < B; ++i)
 #pragma unroll
-        for (int j = 0; j < CB; ++j) acc[j] = add_diagonals(acc[j], f, diag_f, h, diag_h, r, col_of(j), MP) * scale;
-    };
-    auto store = [&](unsigned char *to, float *diag_to, bool whole) {
-#pragma unroll
-        for (int j = 0; j < CB; ++j) {
-            if (whole) put4(to + unit_bytes(col_of(j), r, MP), acc[j]);
-            else put_square(to, diag_to, r, col_of(j), MP, acc[j]);
+            for (int j = 0; j < B; ++j) own_q[i][j] = acc[i][j];
+        if (!last) {
+            store(ws + area.sq(q), diag_q[q == SQ_Q1], own_q);
+            return;
         }
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int j = 0; j < B; ++j) put4(ws + area.sq(q) + at(i, j), own_q[i][j]);
     };
-    const float *diag_s = diag_a;
     for (int s = 0; s < steps.count; ++s) {
         const OrthoSegmentStep &st = steps.step[s];
         const bool last = s + 1 == steps.count;
-        product(sq_a, diag_s, sq_a, diag_s, st.c);
+        product(sq_a, diag_a, own_a, sq_a, diag_a, own_a, st.c);
 #pragma unroll
-        for (int j = 0; j < CB; ++j) {
-            const int c = col_of(j);
-            acc[j] += get_square(sq_a, diag_s, r, c, MP) * st.b;
+        for (int i = 0; i < B; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] += r + e == c ? st.a : 0.f;
-        }
-        store(sq_p, diag_p, false);
-        if (s == 0) store(ws + area.sq(q), diag_q[q == SQ_Q1], last);     // the first step's P is Q
+            for (int j = 0; j < B; ++j) {
+                acc[i][j] += own_a[i][j] * st.b;
+                if (diagonal && i == j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] += row(i) + e == col(j) ? st.a : 0.f;
+                own_p[i][j] = acc[i][j];
+            }
+        store(sq_p, diag_p, own_p);
+        if (s == 0) store_q(last);                                       // the first step's P is Q
         __syncthreads();
         if (s > 0) {
-            const int next = q == SQ_Q0 ? SQ_Q1 : SQ_Q0;
-            product(sq_p, diag_p, ws + area.sq(q), diag_q[q == SQ_Q1], st.q_scale);
-            store(ws + area.sq(next), diag_q[next == SQ_Q1], last);
-            q = next;
+            product(sq_p, diag_p, own_p, ws + area.sq(q), diag_q[q == SQ_Q1], own_q, st.q_scale);
+            q = q == SQ_Q0 ? SQ_Q1 : SQ_Q0;
+            store_q(last);
         }
-        if (!last) {
-            product(sq_p, diag_p, sq_a, diag_s, st.t_scale);
-            __syncthreads();                                             // everybody has read A
-            store(sq_a, diag_t, false);
-            __syncthreads();
-            product(sq_a, diag_t, sq_p, diag_p, st.a_scale);
-            __syncthreads();                                             // everybody has read T
-            store(sq_a, diag_a, false);
-        }
+        if (last) break;
+        product(sq_p, diag_p, own_p, sq_a, diag_a, own_a, st.t_scale);
+        __syncthreads();                                                 // everybody has read A
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int j = 0; j < B; ++j) own_a[i][j] = acc[i][j];
+        store(sq_a, diag_t, own_a);                                      // T
+        __syncthreads();
+        product(sq_a, diag_t, own_a, sq_p, diag_p, own_p, st.a_scale);
+        __syncthreads();                                                 // everybody has read T
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int j = 0; j < B; ++j) own_a[i][j] = acc[i][j];
+        store(sq_a, diag_a, own_a);
         __syncthreads();
     }
 }
@@ -1066,8 +1125,8 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
             }
             if (segments) {
                 n = blocks(shapes, [](const OrthoArea &) { return 1; });
-                if (any64) ortho_segment_kernel<64><<<n, 64 * 8, 0, st>>>(shapes, all, a_from, q);
-                if (any128) ortho_segment_kernel<128><<<n, 128 * 8, 0, st>>>(shapes, all, a_from, q);
+                if (any64) ortho_segment_kernel<64, 1><<<n, 1024, 0, st>>>(shapes, all, a_from, q);
+                if (any128) ortho_segment_kernel<128, 2><<<n, 1024, 0, st>>>(shapes, all, a_from, q);
             }
             s.f = q; s.xt = xt;
             n = whole();
