@@ -29,16 +29,21 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // The item a block works on, and the block's index within it.
 template <typename Group> __device__ __forceinline__ int find_item(const Group &g, int block, int &local) {
-    int i = 0;
-    while (i + 1 < g.count && block >= g.first[i + 1]) ++i;
-    local = block - g.first[i];
-    return i;
+    int item = 0, start = 0;                             // without branches: one wait for all reads
+#pragma unroll
+    for (int i = 1; i < kOrthoItems; ++i) {
+        const bool behind = block >= g.first[i];
+        item += behind;
+        start = behind ? g.first[i] : start;
+    }
+    local = block - start;
+    return item;
 }
 
 // Consecutive logical blocks on one XCD (hardware deals blocks to the eight XCDs in turn), so that its L2 holds what
 // neighbours share.
-__device__ __forceinline__ int xcd_block() {
-    const int total = gridDim.x, each = total / 8, extra = total % 8, xcd = blockIdx.x % 8;
+template <typename Group> __device__ __forceinline__ int xcd_block(const Group &g) {
+    const unsigned total = g.blocks, each = total / 8, extra = total % 8, xcd = blockIdx.x % 8;
     return xcd * each + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
 }
 
@@ -72,8 +77,8 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroup g, OrthoPara
     constexpr int N = 16 / sizeof(T);
     int local;
     const OrthoItem &it = g.item[find_item(g, blockIdx.x, local)];
-    const OrthoArea a = ortho_area(it.rows, it.cols);
-    const int b = local / a.parts_used, part = local % a.parts_used;
+    const OrthoArea a = ortho_area(it.rows, it.cols, 1);
+    const int b = it.batch == 1 ? 0 : local / a.parts_used, part = local - b * a.parts_used;
     // a matrix without gaps is one long row
     const bool flat = it.x_cs == 1 && (it.x_rs == it.cols || it.rows == 1);
     const int rows = flat ? 1 : it.rows, cols = flat ? it.rows * it.cols : it.cols;
@@ -196,8 +201,8 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroup g, OrthoPar
     __shared__ float tile[64 * kStride];
     __shared__ double wave_sum[4];
     int local;
-    const OrthoItem &it = g.item[find_item(g, xcd_block(), local)];
-    const OrthoArea a = ortho_area(it.rows, it.cols);
+    const OrthoItem &it = g.item[find_item(g, xcd_block(g), local)];
+    const OrthoArea a = ortho_area(it.rows, it.cols, 1);
     const int rt = ortho_padded(it.rows) / 64, ct = ortho_padded(it.cols) / 64;
     const int b = local / (rt * ct), t = local % (rt * ct), r0 = t / ct * 64, c0 = t % ct * 64;
     unsigned char *area = g.ws + it.ws + b * it.ws_stride;
@@ -270,17 +275,14 @@ template <int TB_, int WR_, int WC_, int KG_, int RING_> struct Shape {
                          kWaves = WR * WC * KG, kThreads = 64 * kWaves, kUnits = (WR + WC) * TB;
 };
 typedef Shape<4, 2, 2, 1, 2> LargeTile;                          // 128 x 128
-typedef Shape<2, 2, 2, 1, 4> SmallTile;                          // 64 x 64, two blocks per CU
+typedef Shape<2, 2, 2, 1, 3> SmallTile;                          // 64 x 64, three blocks per CU
 typedef Shape<2, 2, 2, 2, 4> LoneTile;                           // 64 x 64, two groups of waves, one block per CU
 
 // Tiles of rows x cols that hold anything on or above the diagonal of an m x m matrix, and the tile of index `tile`.
-template <typename S> __host__ __device__ inline int upper_tiles_of_row(int ti, int mp) {
-    return (mp + S::kCols - 1) / S::kCols - ti * S::kRows / S::kCols;
-}
+template <typename S> __host__ __device__ inline int tiles_a_side(int mp) { return (mp + S::kRows - 1) / S::kRows; }
 template <typename S> __host__ __device__ inline int upper_tiles(int mp) {
-    int n = 0;
-    for (int ti = 0; ti * S::kRows < mp; ++ti) n += upper_tiles_of_row<S>(ti, mp);
-    return n;
+    static_assert(S::kRows == S::kCols, "");
+    return ortho_triangle(tiles_a_side<S>(mp));
 }
 
 template <typename T, int STAGE, typename S>
@@ -292,18 +294,18 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     static_assert(2 * kUnits % kGroup == 0, "whole loads");
     __shared__ __attribute__((aligned(16))) unsigned char lds[kRingBytes > kOutBytes ? kRingBytes : kOutBytes];
     int local;
-    const int index = find_item(g, xcd_block(), local);
+    const int index = find_item(g, xcd_block(g), local);
     const OrthoShape &it = g.item[index];
-    const OrthoArea a = ortho_area(it.rows, it.cols);
-    const int mt = (a.mp + S::kRows - 1) / S::kRows, nt = (a.np + S::kCols - 1) / S::kCols;
+    const OrthoArea a = ortho_area(it.rows, it.cols, it.splits);
+    const int mt = tiles_a_side<S>(a.mp), nt = (a.np + S::kCols - 1) / S::kCols;
     const int tiles = symmetric ? upper_tiles<S>(a.mp) : mt * nt;
     int part = 0;
-    if (STAGE == STAGE_GRAM) { part = local / tiles % a.splits; local = local / (tiles * a.splits) * tiles + local % tiles; }
-    const int batch = local / tiles;
-    int ti = 0, tj = local % tiles;
+    if (STAGE == STAGE_GRAM && a.splits > 1) { part = local / tiles % a.splits; local = local / (tiles * a.splits) * tiles + local % tiles; }
+    const int batch = it.batch == 1 ? 0 : local / tiles;
+    int ti = 0, tj = local - batch * tiles;
     if (symmetric) {
-        while (tj >= upper_tiles_of_row<S>(ti, a.mp)) tj -= upper_tiles_of_row<S>(ti++, a.mp);
-        tj += ti * S::kRows / S::kCols;
+        while (tj >= mt - ti) tj -= mt - ti++;
+        tj += ti;
     } else {
         ti = tj % mt;
         tj /= mt;
@@ -450,12 +452,13 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         if constexpr (STAGE == STAGE_POLY) {
             const unsigned char *from = area + a.sq(s.f);
             auto add_lower = [&](float (&v)[8], int r, int c, unsigned char *at) {
+                float *keep = mine + (r - r0) * kStride + c - c0;         // for the mirror image
                 const half8 hi = *reinterpret_cast<const half8 *>(from + (at - dst)), lo = *reinterpret_cast<const half8 *>(from + (at - dst) + 1024);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += s.b * ((float)hi[e] + (float)lo[e]) + (r == c + e ? s.a : 0.f);
+                for (int e = 0; e < 8; ++e) keep[e] = v[e] += s.b * ((float)hi[e] + (float)lo[e]) + (r == c + e ? s.a : 0.f);
             };
             emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, add_lower);
-            if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, add_lower);
+            if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
         } else {
             if (STAGE == STAGE_GRAM && r0 == c0)
                 emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, KeepDiagonal{reinterpret_cast<float *>(area + a.diag)});
@@ -514,8 +517,8 @@ __global__ __launch_bounds__(256) void ortho_reduce_kernel(OrthoShapes g, StageA
     __shared__ float tile[kSub * kStride];
     int local;
     const OrthoShape &it = g.item[find_item(g, blockIdx.x, local)];
-    const OrthoArea a = ortho_area(it.rows, it.cols);
-    const int batch = local / a.sub_tiles, index = local % a.sub_tiles, side = a.mp / kSub;
+    const OrthoArea a = ortho_area(it.rows, it.cols, it.splits);
+    const int batch = it.batch == 1 ? 0 : local / a.sub_tiles, index = local - batch * a.sub_tiles, side = a.mp / kSub;
     int ti = 0, tj = index;
     while (tj >= side - ti) tj -= side - ti++;
     tj += ti;
@@ -769,7 +772,7 @@ __global__ __launch_bounds__(MP / 16 / B * (MP / 16 / B) * 64) void ortho_segmen
     __shared__ __attribute__((aligned(16))) float diag_a[MP], diag_t[MP], diag_p[MP], diag_q[2][MP];
     int batch;
     const OrthoShape &it = g.item[find_item(g, blockIdx.x, batch)];
-    const OrthoArea area = ortho_area(it.rows, it.cols);
+    const OrthoArea area = ortho_area(it.rows, it.cols, it.splits);
     if (area.mp != MP) return;                                           // the other size's launch takes it
     unsigned char *ws = g.ws + it.ws + batch * it.ws_stride;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -973,7 +976,8 @@ void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         blocks += g.item[i].batch;
         widest = ortho_max(widest, ortho_max(g.item[i].rows, g.item[i].cols));
     }
-    g.first[g.count] = blocks;
+    for (int i = g.count; i < kOrthoItems; ++i) g.first[i] = INT32_MAX;
+    g.blocks = blocks;
     with_dtype(p.type, [&](auto type) {
         typedef decltype(type) T;
         if (widest <= 64) ortho_small_kernel<T, 64><<<blocks, 512, 0, st>>>(g, p, steps);
@@ -1007,7 +1011,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     for (int i = 0; i < g.count; ++i) {
         const OrthoItem &it = g.item[i];
         const OrthoArea a = ortho_area(it.rows, it.cols);
-        shapes.item[i] = {it.ws, it.ws_stride, it.rows, it.cols, it.batch};
+        shapes.item[i] = {it.ws, it.ws_stride, it.rows, it.cols, it.batch, a.splits};
         for (int k = 0; k < 2; ++k)
             with_tile(k, [&](auto shape) {
                 typedef decltype(shape) S;
@@ -1029,7 +1033,8 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
             group.first[i] = n;
             n += g.item[i].batch * per_matrix(ortho_area(g.item[i].rows, g.item[i].cols));
         }
-        group.first[g.count] = n;
+        for (int i = g.count; i < kOrthoItems; ++i) group.first[i] = INT32_MAX;
+        group.blocks = n;
         return n;
     };
     auto squares = [&] {

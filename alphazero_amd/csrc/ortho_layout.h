@@ -33,14 +33,16 @@ struct OrthoItem {
 // What the products need of an item.
 struct OrthoShape {
     size_t ws, ws_stride;
-    int rows, cols, batch;
+    int rows, cols, batch, splits;
 };
 
+// A block looks for its item in two rounds of reads: the head of the group, then the item.
 template <typename Item> struct OrthoGroupOf {
-    Item item[kOrthoItems];
-    int first[kOrthoItems + 1];  // first block of every item in the launch at hand
+    int blocks;                  // of the launch at hand (blockIdx.x)
+    int first[kOrthoItems];      // first block of every item; behind the last one INT32_MAX
     int count;
     unsigned char *ws;
+    Item item[kOrthoItems];
 };
 typedef OrthoGroupOf<OrthoItem> OrthoGroup;
 typedef OrthoGroupOf<OrthoShape> OrthoShapes;
@@ -64,7 +66,15 @@ enum OrthoSquare { SQ_A0 = 0, SQ_A1 = 1, SQ_T = 2, SQ_P = 3, SQ_Q0 = 4, SQ_Q1 = 
 
 __host__ __device__ constexpr int ortho_triangle(int t) { return t * (t + 1) / 2; }
 
-__host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
+// Parts that the long side is cut into for X X^T: enough to give every CU two blocks, at least 256 each (a tile takes 1024
+// whole in 12.8 us; in four parts 7.4, and adding those up 4.1).
+inline int ortho_splits(int rows, int cols) {
+    const int mp = ortho_padded(ortho_min(rows, cols)), np = ortho_padded(ortho_max(rows, cols));
+    const int tiles = ortho_triangle(mp > 256 ? (mp + 127) / 128 : mp / 64);
+    return ortho_max(1, ortho_min(512 / tiles, np / 256));
+}
+
+__host__ __device__ inline OrthoArea ortho_area(int rows, int cols, int splits) {
     OrthoArea a;
     a.m = rows < cols ? rows : cols;
     a.n = rows < cols ? cols : rows;
@@ -72,9 +82,7 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     a.np = ortho_padded(a.n);
     a.sub = a.mp > 256 ? 64 : 32;
     a.sub_tiles = ortho_triangle(a.mp / a.sub);
-    // parts that give every CU two blocks, at least 256 of the long side each
-    const int tiles = ortho_triangle(a.sub == 64 ? (a.mp + 127) / 128 : a.mp / 64);
-    a.splits = ortho_max(1, ortho_min(512 / tiles, a.np / 256));
+    a.splits = splits;
     const long long count = (long long)rows * cols;
     a.parts_used = (int)(count / 4096 < 1 ? 1 : count / 4096 < kOrthoNormParts ? count / 4096 : kOrthoNormParts);
     a.wide = (size_t)a.mp * a.np * 4;
@@ -90,6 +98,7 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols) {
     a.bytes = o;
     return a;
 }
+inline OrthoArea ortho_area(int rows, int cols) { return ortho_area(rows, cols, ortho_splits(rows, cols)); }
 
 // A small matrix stays in one block's LDS from its first to its last step: X <- a X + (b A + c A^2) X as it is written.
 constexpr int kOrthoSmallRows = 64, kOrthoSmallCols = 192;
