@@ -349,27 +349,54 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
             if constexpr (R % 4 == 2) fh[B][I] = *reinterpret_cast<const half8 *>(fu);
             if constexpr (R % 4 == 3) hl[B][I] = *reinterpret_cast<const half8 *>(hu + 1024);
         };
-        // A row of blocks at a time, every stage's sum from zero, smallest products first; the sums are added up by the
-        // vector pipe (see add_products).
+        // Every stage's sum from zero, smallest products first, added up by the vector pipe (see add_products).  On large
+        // tiles a row of blocks at a time; the four blocks of small ones together, since a block's products wait for each
+        // other, and added while the next stage multiplies (three 832 x 832 x 832: 17.0 us by rows, 16.1 so).
         constexpr bool kAll = STAGE == STAGE_POLY || STAGE == STAGE_MUL, kFromZero = kAll || STAGE == STAGE_GRAM;
+        f32x4 sum[2][TB][TB] = {};
         auto multiply = [&](auto from) {
             constexpr int B = from;
-            if constexpr (!kFromZero) {                          // a short sum without a large diagonal
+            if constexpr (TB == 2) {
+                auto products = [&](const half8 (&f)[TB], const half8 (&h)[TB], bool first) {
+#pragma unroll
+                    for (int i = 0; i < TB; ++i)
+#pragma unroll
+                        for (int j = 0; j < TB; ++j) {
+                            f32x4 &to = kFromZero ? sum[B][i][j] : acc[i][j];
+                            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[i], h[j], kFromZero && first ? f32x4{0.f, 0.f, 0.f, 0.f} : to, 0, 0, 0);
+                        }
+                };
+                if (kAll) products(fl[B], hl[B], true);
+                products(fl[B], hh[B], !kAll);
+                products(fh[B], hl[B], false);
+                products(fh[B], hh[B], false);
+                if (kFromZero)
+#pragma unroll
+                    for (int i = 0; i < TB; ++i)
+#pragma unroll
+                        for (int j = 0; j < TB; ++j) acc[i][j] += sum[1 - B][i][j];
+            } else if constexpr (!kFromZero) {                   // a short sum without a large diagonal
                 static_for<TB>([&](auto row) { add_to<TB>(fh[B][row], fl[B][row], hh[B], hl[B], acc[row]); });
-                __builtin_amdgcn_sched_barrier(0);
-                return;
+            } else {
+                static_for<TB>([&](auto row) {
+                    constexpr int I = row;
+                    add_products<TB, kAll>(fh[B][I], fl[B][I], hh[B], hl[B], sum[0][I & 1]);
+                    if constexpr (I > 0)
+#pragma unroll
+                        for (int j = 0; j < TB; ++j) acc[I - 1][j] += sum[0][(I - 1) & 1][j];
+                });
+#pragma unroll
+                for (int j = 0; j < TB; ++j) acc[TB - 1][j] += sum[0][(TB - 1) & 1][j];
             }
-            f32x4 sum[2][TB];
-            static_for<TB>([&](auto row) {
-                constexpr int I = row;
-                add_products<TB, kAll>(fh[B][I], fl[B][I], hh[B], hl[B], sum[I & 1]);
-                if constexpr (I > 0)
-#pragma unroll
-                    for (int j = 0; j < TB; ++j) acc[I - 1][j] += sum[(I - 1) & 1][j];
-            });
-#pragma unroll
-            for (int j = 0; j < TB; ++j) acc[TB - 1][j] += sum[(TB - 1) & 1][j];
             __builtin_amdgcn_sched_barrier(0);
+        };
+        auto add_last = [&](auto from) {
+            constexpr int B = from;
+            if constexpr (TB == 2 && kFromZero)
+#pragma unroll
+                for (int i = 0; i < TB; ++i)
+#pragma unroll
+                    for (int j = 0; j < TB; ++j) acc[i][j] += sum[B][i][j];
         };
         constexpr int kInFlight = (RING - 2) * kPerWave;         // a wave's loads behind the stage it waits for
         auto meet = [&](bool all_issued) {
@@ -408,8 +435,10 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         if (t + 1 < stages) {
             step(t, even, odd);
             multiply(odd);
+            add_last(odd);
         } else {
             multiply(even);
+            add_last(even);
         }
     }
 
@@ -596,30 +625,12 @@ __device__ __forceinline__ void put_square(unsigned char *units, float *diag, in
         }
     put4(units + unit_bytes(c, r, kdim), v);
 }
-__device__ __forceinline__ f32x4 get_square(const unsigned char *units, const float *diag, int r, int c, int kdim) {
-    f32x4 v = get4(units + unit_bytes(c, r, kdim));
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (r + e == c) v[e] = diag[c];
-    return v;
-}
-// O_F O_G completed to F G at rows r .. r + 3, column c.
-__device__ __forceinline__ f32x4 add_diagonals(f32x4 product, const unsigned char *f, const float *diag_f, const unsigned char *g,
-                                               const float *diag_g, int r, int c, int kdim) {
-    const f32x4 of = get4(f + unit_bytes(c, r, kdim)), og = get4(g + unit_bytes(c, r, kdim));
-    const float dg = diag_g[c];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float df = diag_f[r + e];
-        product[e] += df * (r + e == c ? dg : og[e]) + of[e] * dg;       // (O is zero on the diagonal)
-    }
-    return product;
-}
-// acc += rows rb of F times rows cb .. cb + N - 1 (blocks of 16) of G, both units with K columns; G may lie in global memory.
+// acc += rows rb of F times rows cb .. cb + N - 1 (blocks of 16) of G, both units with K columns, k_units of 32 of them.
 template <int N>
-__device__ __forceinline__ void multiply_units(const unsigned char *f, const unsigned char *g, int rb, int cb, int kdim, f32x4 (&acc)[N]) {
+__device__ __forceinline__ void multiply_units(const unsigned char *f, const unsigned char *g, int rb, int cb, int kdim, int k_units,
+                                               f32x4 (&acc)[N]) {
     const int lane = threadIdx.x & 63, ku = kdim / 32;
-    for (int k = 0; k < ku; ++k) {
+    for (int k = 0; k < k_units; ++k) {
         const unsigned char *fu = f + (rb * ku + k) * 2048 + lane * 16;
         const half8 fh = *reinterpret_cast<const half8 *>(fu), fl = *reinterpret_cast<const half8 *>(fu + 1024);
         half8 gh[N], gl[N];
@@ -633,11 +644,14 @@ __device__ __forceinline__ void multiply_units(const unsigned char *f, const uns
     }
 }
 
-// A whole matrix (m <= 64, n <= NP) in one block of eight waves: the twenty launches of the long way would cost a small
-// matrix several times what it computes.
+// A whole matrix (m <= 64, n <= NP) in one block of sixteen waves: the twenty launches of the long way would cost a small
+// matrix several times what it computes.  What bounds it is the chain of a step: three products, each behind a barrier.
+// So a wave has one block of 16 of a square, its parts of A and X stay in float32 registers, blocks of padding are left
+// out, and X Y's tiles come out of the matrix unit both ways round, for the two orders of units they are stored in
+// (128 x 32, five steps: 28.0 us with two blocks to a wave, values read back from LDS and halves scattered, now 21.5).
 template <typename T, int NP>
-__global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoParams p, OrthoSmallSteps steps) {
-    constexpr int M = kOrthoSmallRows, kWide = M * NP * 4, kSquare = M * M * 4, TN = NP / 32;
+__global__ __launch_bounds__(1024) void ortho_small_kernel(OrthoGroup g, OrthoParams p, OrthoSmallSteps steps) {
+    constexpr int M = kOrthoSmallRows, kWide = M * NP * 4, kSquare = M * M * 4, TN = NP / 64;
     __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kWide + 2 * kSquare + 2 * M * 4];
     unsigned char *x = lds, *xt = lds + kWide, *sq_a = lds + 2 * kWide, *sq_b = sq_a + kSquare;
     float *diag_a = reinterpret_cast<float *>(sq_b + kSquare), *diag_b = diag_a + M;
@@ -649,16 +663,16 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoPar
     const T *src = static_cast<const T *>(it.x) + batch * it.x_bs;
     const long long rs = tall ? it.x_cs : it.x_rs, cs = tall ? it.x_rs : it.x_cs;
     // X is u or its transpose; a thread takes eight columns of a row
-    constexpr int kPer = M * NP / 8 / 512;
+    constexpr int kPer = (M * NP / 8 + 1023) / 1024;
     float u[kPer][8];
     double sum = 0.0;
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        const int at = q * 512 + tid, i = at / (NP / 8), j = at % (NP / 8) * 8;
+        const int at = q * 1024 + tid, i = at / (NP / 8), j = at % (NP / 8) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float v = 0.f;
-            if (i < m && j + e < n) {
+            if (i < m && j + e < n) {                            // (i >= 64 behind the last part)
                 v = to_f32(src[i * rs + (j + e) * cs]);
                 if (p.muon) {
                     const size_t o = tall ? (size_t)(j + e) * it.cols + i : (size_t)i * it.cols + j + e;
@@ -678,12 +692,13 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoPar
     __syncthreads();
     double norm = 0.0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) norm += wave_sum[w];
+    for (int w = 0; w < 16; ++w) norm += wave_sum[w];
     const double scale = (double)steps.pow_kx / (sqrt(norm) + p.eps);
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        const int at = q * 512 + tid, i = at / (NP / 8), j = at % (NP / 8) * 8;
+        const int at = q * 1024 + tid, i = at / (NP / 8), j = at % (NP / 8) * 8;
+        if (i >= M) break;
         float v[8];
         half8 lo;
 #pragma unroll
@@ -700,47 +715,79 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoPar
         }
     }
     __syncthreads();
-    const int rb = wave / 2, cb = wave % 2 * 2, nb = wave % 2 * TN;     // 16-row block; first 16-column block of a square, of X
-    const int row = rb * 16 + (lane >> 4) * 4, col = lane & 15;         // a lane's four rows and its column in a block
+    // This wave's block (rb, cb) of a square and its TN blocks of X: (rb, nb + j).  A lane holds four rows of a column, of
+    // X's blocks turned round four columns of a row too.  What lies behind m, n rounded up to 32 is zero and left out.
+    const int rb = wave / 4, cb = wave % 4, nb = wave % 4 * TN, mk = (m + 31) / 32, nk = (n + 31) / 32;
+    const int row = rb * 16 + (lane >> 4) * 4, col = cb * 16 + (lane & 15), turned_row = rb * 16 + (lane & 15);
+    const bool in_square = rb < 2 * mk && cb < 2 * mk, diagonal = rb == cb;
+    auto x_col = [&](int j) { return (nb + j) * 16 + (lane & 15); };
+    auto x_turned_col = [&](int j) { return (nb + j) * 16 + (lane >> 4) * 4; };
+    f32x4 own_x[TN], own_turned[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        own_x[j] = get4(xt + unit_bytes(x_col(j), row, M));
+        own_turned[j] = get4(x + unit_bytes(turned_row, x_turned_col(j), NP));
+    }
     for (int s = 0; s < p.steps; ++s) {
-        const OrthoSmallStep st = steps.step[s];
-        f32x4 a[2] = {};
-        multiply_units<2>(x, x, rb, cb, NP, a);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) put_square(sq_a, diag_a, row, (cb + j) * 16 + col, M, a[j] * st.a_scale);
-        __syncthreads();
-        f32x4 b[2] = {};
-        multiply_units<2>(sq_a, sq_a, rb, cb, M, b);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int c = (cb + j) * 16 + col;
-            const f32x4 low = get_square(sq_a, diag_a, row, c, M), square = add_diagonals(b[j], sq_a, diag_a, sq_a, diag_a, row, c, M);
-            put_square(sq_b, diag_b, row, c, M, low * st.b + square * st.c);
+        const OrthoSmallStep &st = steps.step[s];
+        f32x4 own_a[1] = {};
+        if (in_square) {
+            multiply_units<1>(x, x, rb, cb, NP, nk, own_a);
+            own_a[0] *= st.a_scale;
+            if (diagonal) put_square(sq_a, diag_a, row, col, M, own_a[0]);
+            else put4(sq_a + unit_bytes(col, row, M), own_a[0]);
         }
         __syncthreads();
-        f32x4 y[TN] = {};
-        multiply_units<TN>(sq_b, xt, rb, nb, M, y);
+        if (in_square) {
+            f32x4 b[1] = {};
+            multiply_units<1>(sq_a, sq_a, rb, cb, M, mk, b);
+            f32x4 off = own_a[0];
+            if (diagonal)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {                                  // (a + D_B) X + O_B X
-            const f32x4 old = get4(xt + unit_bytes((nb + j) * 16 + col, row, M));
+                for (int e = 0; e < 4; ++e)
+                    if (row + e == col) off[e] = 0.f;
+            const f32x4 df = *reinterpret_cast<const f32x4 *>(diag_a + row);
+            b[0] = own_a[0] * st.b + (b[0] + df * own_a[0] + off * diag_a[col]) * st.c;
+            if (diagonal) put_square(sq_b, diag_b, row, col, M, b[0]);
+            else put4(sq_b + unit_bytes(col, row, M), b[0]);
+        }
+        __syncthreads();
+        f32x4 y[TN] = {}, turned[TN] = {};
+        if (rb < 2 * mk) {
+#pragma unroll 1
+            for (int k = 0; k < mk; ++k) {
+                const unsigned char *fu = sq_b + (rb * (M / 32) + k) * 2048 + lane * 16;
+                const half8 fh = *reinterpret_cast<const half8 *>(fu), fl = *reinterpret_cast<const half8 *>(fu + 1024);
+                half8 gh[TN], gl[TN];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[j][e] = ((st.ax + diag_b[row + e]) * old[e] + y[j][e]) * st.y_scale;
+                for (int j = 0; j < TN; ++j) {
+                    const unsigned char *gu = xt + ((nb + j) * (M / 32) + k) * 2048 + lane * 16;
+                    gh[j] = *reinterpret_cast<const half8 *>(gu), gl[j] = *reinterpret_cast<const half8 *>(gu + 1024);
+                }
+                add_to<TN>(fh, fl, gh, gl, y);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    turned[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(gh[j], fl, turned[j], 0, 0, 0);
+                    turned[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(gl[j], fh, turned[j], 0, 0, 0);
+                    turned[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(gh[j], fh, turned[j], 0, 0, 0);
+                }
+            }
+            const f32x4 db = *reinterpret_cast<const f32x4 *>(diag_b + row);
+            const float db_turned = diag_b[turned_row];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {                              // (a + D_B) X + O_B X
+                own_x[j] = y[j] = ((db + st.ax) * own_x[j] + y[j]) * st.y_scale;
+                own_turned[j] = ((db_turned + st.ax) * own_turned[j] + turned[j]) * st.y_scale;
+            }
         }
         if (s + 1 < p.steps) {
             __syncthreads();                                            // everybody has read the old X
+            if (rb < 2 * mk)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const int c = (nb + j) * 16 + col;
-                unsigned char *turned = xt + unit_bytes(c, row, M);
-                put4(turned, y[j]);
-                const half4 hi = *reinterpret_cast<half4 *>(turned), lo = *reinterpret_cast<half4 *>(turned + 1024);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    unsigned char *straight = x + unit_bytes(row + e, c, NP);
-                    *reinterpret_cast<f16_t *>(straight) = hi[e];
-                    *reinterpret_cast<f16_t *>(straight + 1024) = lo[e];
+                for (int j = 0; j < TN; ++j) {
+                    put4(xt + unit_bytes(x_col(j), row, M), own_x[j]);
+                    put4(x + unit_bytes(turned_row, x_turned_col(j), NP), own_turned[j]);
                 }
-            }
             __syncthreads();
             continue;
         }
@@ -749,7 +796,7 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoGroup g, OrthoPar
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = row + e, c = (nb + j) * 16 + col;
+                const int i = row + e, c = x_col(j);
                 if (i >= m || c >= n) continue;
                 const int ur = tall ? c : i, uc = tall ? i : c;
                 float v = y[j][e];
@@ -980,9 +1027,9 @@ void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     g.blocks = blocks;
     with_dtype(p.type, [&](auto type) {
         typedef decltype(type) T;
-        if (widest <= 64) ortho_small_kernel<T, 64><<<blocks, 512, 0, st>>>(g, p, steps);
-        else if (widest <= 128) ortho_small_kernel<T, 128><<<blocks, 512, 0, st>>>(g, p, steps);
-        else ortho_small_kernel<T, kOrthoSmallCols><<<blocks, 512, 0, st>>>(g, p, steps);
+        if (widest <= 64) ortho_small_kernel<T, 64><<<blocks, 1024, 0, st>>>(g, p, steps);
+        else if (widest <= 128) ortho_small_kernel<T, 128><<<blocks, 1024, 0, st>>>(g, p, steps);
+        else ortho_small_kernel<T, kOrthoSmallCols><<<blocks, 1024, 0, st>>>(g, p, steps);
     });
 }
 
