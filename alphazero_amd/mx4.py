@@ -15,6 +15,7 @@ network's linear layer with the same kernels.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Union
 
 import torch
@@ -43,13 +44,18 @@ class MX4Tensor:
         shape = torch.Size(shape)
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError(f"shape {tuple(shape)} has no last dimension to cut into blocks")
-        units = _units(shape[:-1].numel(), shape[-1])
+        rows, cols = shape[:-1].numel(), shape[-1]
+        units = _units(rows, cols)
         for name, t, want in (("codes", codes, units + (4096,)), ("scales", scales, units + (256,))):
             if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous uint8 of shape {want}, got {t.dtype} {tuple(t.shape)}")
         if codes.device != scales.device:
             raise ValueError("codes and scales are on different devices")
-        self.codes, self.scales, self.shape = codes, scales, shape
+        self._take(codes, scales, shape, rows, cols)
+
+    def _take(self, codes, scales, shape, rows, cols):
+        self.codes, self.scales, self.shape, self._rows, self._cols = codes, scales, shape, rows, cols
+        return self
 
     @property
     def device(self):
@@ -58,10 +64,10 @@ class MX4Tensor:
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the codes stand for, rounded once to `dtype`."""
         with on_device(self.codes):
-            out = torch.empty(self.shape, dtype=dtype, device=self.device)
+            out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
             code = dtype_code(out, "dtype")
-            check(_lib.load().nnb_mx4_dequantize(stream_of(self.codes), code, self.shape[:-1].numel(), self.shape[-1],
-                                                 ptr(self.codes), ptr(self.scales), ptr(out)), "nnb_mx4_dequantize")
+            check(_lib.load().nnb_mx4_dequantize(stream_of(out), code, self._rows, self._cols, ptr(self.codes),
+                                                 ptr(self.scales), ptr(out)), "nnb_mx4_dequantize")
         return out
 
     def __repr__(self):
@@ -95,12 +101,20 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
     with on_device(x):
         v = _rows_view(x)
         rows, cols = v.shape
-        units = _units(rows, cols)
-        codes = torch.empty(units + (4096,), dtype=torch.uint8, device=x.device)
-        scales = torch.empty(units + (256,), dtype=torch.uint8, device=x.device)
-        check(_lib.load().nnb_mx4_quantize(stream_of(x), code, rows, cols, ptr(v), v.stride(0), v.stride(1), ptr(codes),
+        units, device, (row_stride, col_stride) = _units(rows, cols), x.device, v.stride()
+        codes = torch.empty(units + (4096,), dtype=torch.uint8, device=device)
+        scales = torch.empty(units + (256,), dtype=torch.uint8, device=device)
+        check(_lib.load().nnb_mx4_quantize(stream_of(x), code, rows, cols, ptr(v), row_stride, col_stride, ptr(codes),
                                            ptr(scales)), "nnb_mx4_quantize")
-    return MX4Tensor(codes, scales, x.shape)
+    return MX4Tensor.__new__(MX4Tensor)._take(codes, scales, x.shape, rows, cols)       # right by construction
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows: int, cols: int, n: int, quantized: bool) -> int:
+    nbytes = C.c_size_t()
+    check(_lib.load().nnb_mx4_linear_workspace_bytes(rows, cols, n, int(quantized), C.byref(nbytes)),
+          "nnb_mx4_linear_workspace_bytes")
+    return nbytes.value
 
 
 def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[torch.Tensor] = None, relu: bool = False,
@@ -143,23 +157,23 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
         no_grad("mx4.linear", out)
         y_stride = n if out.is_contiguous() else _row_stride(out, n)
         args = Mx4LinearArgs()
-        args.rows, args.cols, args.out_features = torch.Size(y_shape[:-1]).numel(), cols, n
         if quantized:
+            rows = x._rows
             args.x_codes, args.x_scales = ptr(x.codes), ptr(x.scales)
         else:
             v = _rows_view(x)
-            args.x, args.x_row_stride, args.x_col_stride = ptr(v), v.stride(0), v.stride(1)
+            rows = v.shape[0]
+            args.x = ptr(v)
+            args.x_row_stride, args.x_col_stride = v.stride()
+        args.rows, args.cols, args.out_features = rows, cols, n
         args.w_codes, args.w_scales = ptr(weight.codes), ptr(weight.scales)
         b = bias.contiguous() if bias is not None else None
         args.bias = ptr(b) if b is not None else None
         args.y, args.y_row_stride = ptr(out), y_stride
         args.x_type, args.y_type, args.relu = x_type, dtype_code(out, "out"), int(bool(relu))
         args.bias_type = dtype_code(bias, "bias") if bias is not None else 0
-        lib = _lib.load()
-        nbytes = C.c_size_t()
-        check(lib.nnb_mx4_linear_workspace_bytes(args.rows, cols, n, int(quantized), C.byref(nbytes)),
-              "nnb_mx4_linear_workspace_bytes")
-        workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=device) if nbytes.value else None
-        check(lib.nnb_mx4_linear(stream_of(out), C.byref(args), ptr(workspace) if workspace is not None else None, nbytes.value),
+        nbytes = _workspace_bytes(rows, cols, n, quantized)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        check(_lib.load().nnb_mx4_linear(stream_of(out), C.byref(args), ptr(workspace) if nbytes else None, nbytes),
               "nnb_mx4_linear")
     return out
