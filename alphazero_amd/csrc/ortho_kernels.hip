@@ -4,8 +4,9 @@
 // p(A) = a I + b A + c A^2.  p(A) commutes with A, so the steps can run on the m x m matrices alone: A <- p(A) A p(A),
 // Q <- p(A) Q, and X is touched only to form A (X X^T) and to apply the product of the polynomials (Q X).  Rounding
 // errors in A grow by up to a^2 a step in the directions of small singular values, so A is formed afresh from X after
-// every kOrthoSegment = 3 steps: five steps (3 + 2) are as accurate as five plain ones (float32, 256 x 1024 of
-// normal numbers: 3e-6 of the result's size against 2e-6; one segment of five on a square matrix: 1.6e-5 against 1.8e-6).
+// every kOrthoSegment = 3 steps: five steps (3 + 2) are as accurate as five plain ones (normal numbers, error over the
+// result's size against the plain float32 form's: 200 x 3000 2.0e-6 / 1.8e-6, 1024 x 11520 1.5e-6 / 5.1e-6, 128 x 2048
+// 5e-7 / 1.6e-6; one segment of five on a square matrix 1.6e-5 / 1.8e-6).
 // All m x m matrices are symmetric: half of their tiles are computed, the other half mirrored.
 //
 // Arithmetic: every operand is value * 2^k = hi + lo, two halves (22 bits), and a product is three matrix
@@ -71,7 +72,8 @@ __device__ __forceinline__ void load_row(const T *row, long long cs, int c, int 
 }
 
 // Sum of squares of u, in double (a gradient's squares leave float32's range long before the gradient does), as partial
-// sums that the next kernel adds in a fixed order; the optimiser step's new momentum is written on the way.
+// sums that the next kernel adds in a fixed order; the optimiser step's new momentum is written on the way.  Bound by
+// memory: 1024 x 11520 in float32 12.5 us (3.8 TB/s), 27.5 with the momentum (5.2 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroup g, OrthoParams p) {
     constexpr int N = 16 / sizeof(T);
@@ -194,7 +196,8 @@ struct Unchanged {
     __device__ __forceinline__ void operator()(float (&)[8], int, int, unsigned char *) const {}
 };
 
-// u / (|u| + eps) * 2^kx as units, X and its transpose, zero-padded.  One block per 64 x 64 tile.
+// u / (|u| + eps) * 2^kx as units, X and its transpose, zero-padded.  One block per 64 x 64 tile.  Bound by memory:
+// 1024 x 11520 in float32 26 us (5.5 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroup g, OrthoParams p, float pow_kx) {
     constexpr int N = 16 / sizeof(T), kStride = 68;
@@ -540,6 +543,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void ortho_finish_kernel(OrthoShape
 }
 
 // Adds up the parts of X X^T, one block of four waves per sub-tile (16 TB squared), and lays it out both ways round.
+// Bound by latency: 1024 x 1024 in 14 parts 8.5 us, 128 x 128 in 8 parts 4.1.
 template <int TB>
 __global__ __launch_bounds__(256) void ortho_reduce_kernel(OrthoShapes g, StageArgs s) {
     constexpr int kSub = 16 * TB, kStride = kSub + 4, kEach = TB * TB / 4;
@@ -1071,7 +1075,8 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         reduce_of[a.sub == 64] |= a.splits > 1;
     }
     // Large tiles where they give most CUs at least one; where even small ones give no CU two, two groups share each
-    // (1024 x 1024 x 1024, 136 tiles: 11.5 us against 12.8; 273 tiles of 832 x 832 x 832: 17.9 against 13.9).
+    // (one product of squares: 1024, 136 small tiles, 13.9 us with two groups, 17.1 without; 832 three times, 273 tiles,
+    // 22.4 and 16.4.  Q X of 832 x 1536 three times, 252 large tiles: 27.7, 31.8 on small ones).
     auto pick = [](const long long (&n)[2]) { return n[0] >= 200 ? 0 : n[1] > 256 ? 1 : 2; };
     const int symmetric_tile = pick(upper), full_tile = pick(full);
     auto blocks = [&](auto &group, auto per_matrix) {
