@@ -69,7 +69,8 @@ class AlphaZeroAgent(Agent):
         self.eval_cache = False         # True: a game does not send one position to the network twice (same moves)
         # arithmetic of the network's conv / linear layers on the device (engine.PRECISIONS): "f32s" is
         # float32-faithful (the reference computes in float32, network.py:43-50), "f16" rounds the
-        # operands to half and runs three times as fast, "f32" is the exact-FMA matrix path
+        # operands to half and runs three times as fast, "f32" is the exact-FMA matrix path, "mx4" is "f16" with the
+        # linear layer on 4-bit floats
         self.precision = DEFAULT_PRECISION
         self._engine = None
         self._engine_key = None

@@ -855,8 +855,9 @@ void carve_mx4_rows(Carver &c, int64_t rows, int cols, bool x_quantized, uint8_t
 int check_matrix(int64_t rows, int64_t cols) {
     if (rows < 0 || cols < 0) return fail(NNB_ERR_ARG, "matrix of %lld x %lld", (long long)rows, (long long)cols);
     const int64_t shorter = rows < cols ? rows : cols, longer = rows < cols ? cols : rows;
-    if (longer > 0x7fffffffLL || rows * cols > 0x7fffffffLL || shorter > 16384)
-        return fail(NNB_ERR_ARG, "matrix of %lld x %lld: more than 2^31 - 1 elements or a shorter side over 16384",
+    constexpr int64_t kMost = 0x7fffffffLL - 63;         // rounded up to whole tiles still an int
+    if (longer > kMost || rows * cols > kMost || shorter > 16384)
+        return fail(NNB_ERR_ARG, "matrix of %lld x %lld: more than 2^31 - 64 elements or a shorter side over 16384",
                     (long long)rows, (long long)cols);
     return NNB_OK;
 }

@@ -443,7 +443,7 @@ typedef struct nnb_newton_schulz {
 } nnb_newton_schulz;
 /* x and out: `batch` matrices [rows][cols] of type `type`, element (b, r, c) at b*strides[0] + r*strides[1] +
  * c*strides[2] (elements).  out's elements must not overlap each other or x, except out = x with equal strides.
- * Limits: rows*cols < 2^31, the shorter side at most 16384.  batch, rows or cols = 0 is a no-op. */
+ * Limits: rows*cols at most 2^31 - 64, the shorter side at most 16384.  batch, rows or cols = 0 is a no-op. */
 int nnb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, size_t *bytes_out);
 int nnb_orthogonalize(void *stream, int type, int64_t batch, int64_t rows, int64_t cols, const void *x,
                       const int64_t x_strides[3], void *out, const int64_t out_strides[3], const nnb_newton_schulz *ns,

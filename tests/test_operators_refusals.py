@@ -209,3 +209,12 @@ def test_which_tensors_share_memory():
     assert not share_memory(buf[:, 20:40], buf[1:, :20]) and not share_memory(buf[1:, :20], buf[:, 20:40])
     half = torch.zeros(8, 100, dtype=torch.float16)
     assert not share_memory(half[:, :50], half[:, 50:]) and share_memory(half[::2, :60], half[1:, 50:])
+
+
+def test_matrices_near_the_limit_of_indices(lib):
+    n = C.c_size_t()
+    most = 2 ** 31 - 64
+    for rows, cols in ((1, most + 1), (most + 63, 1), (7, 306783378), (16385, 16385)):
+        assert lib.nnb_orthogonalize_workspace_bytes(1, rows, cols, C.byref(n)) == -1 and "2^31" in _message(lib), (rows, cols)
+    for rows, cols in ((1, most), (most, 1), (16384, 131071)):
+        assert lib.nnb_orthogonalize_workspace_bytes(1, rows, cols, C.byref(n)) == 0 and n.value > 12 * rows * cols, (rows, cols)
