@@ -20,12 +20,13 @@ def dtype_code(t: torch.Tensor, name: str) -> int:
 _STAY = contextlib.nullcontext()
 
 
-def on_device(t: torch.Tensor):
+def on_device(t):
     """Makes the tensor's GPU current, which the library launches on."""
-    if not t.is_cuda:
-        raise NnbError(f"a tensor on {t.device}: the kernels run on an MI355X only (there is no CPU path)")
+    device = t.device
+    if device.type != "cuda":
+        raise NnbError(f"a tensor on {device}: the kernels run on an MI355X only (there is no CPU path)")
     # switching devices costs more than a small launch: only where it changes something
-    return _STAY if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _STAY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def stream_of(t: torch.Tensor) -> C.c_void_p:

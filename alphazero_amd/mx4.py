@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._lib import Mx4LinearArgs, check
-from ._tensors import dtype_code, no_grad, on_device, ptr, share_memory, stream_of
+from ._tensors import DTYPES, dtype_code, no_grad, on_device, share_memory, stream_of
 
 BLOCK = 32                              # elements that share a scale
 UNIT_ROWS, UNIT_COLS = 32, 256          # rows and columns are padded with zeros to whole units
@@ -51,23 +51,47 @@ class MX4Tensor:
                 raise ValueError(f"{name} must be contiguous uint8 of shape {want}, got {t.dtype} {tuple(t.shape)}")
         if codes.device != scales.device:
             raise ValueError("codes and scales are on different devices")
-        self._take(codes, scales, shape, rows, cols)
+        self.shape, self.device, self._rows, self._cols, self._units = shape, codes.device, rows, cols, units
+        self._codes, self._scales = codes, scales
 
-    def _take(self, codes, scales, shape, rows, cols):
-        self.codes, self.scales, self.shape, self._rows, self._cols = codes, scales, shape, rows, cols
+    @classmethod
+    def _of_buffer(cls, buffer, shape, rows, cols, units):
+        """All codes, then all scales in one allocation; the two tensors are made when somebody asks for them."""
+        self = cls.__new__(cls)
+        self.shape, self.device, self._rows, self._cols, self._units = shape, buffer.device, rows, cols, units
+        self._codes, self._scales, self._buffer = None, None, buffer
         return self
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._buffer[:self._units[0] * self._units[1] * 4096].view(self._units + (4096,))
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._buffer[self._units[0] * self._units[1] * 4096:].view(self._units + (256,))
+        return self._scales
+
+    def _pointers(self) -> tuple:
+        if self._codes is None or self._scales is None:
+            base = self._buffer.data_ptr()
+            return base, base + self._units[0] * self._units[1] * 4096
+        return self._codes.data_ptr(), self._scales.data_ptr()
+
+    def _tensors(self) -> tuple:
+        return (self._buffer,) if self._codes is None else (self.codes, self.scales)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the codes stand for, rounded once to `dtype`."""
-        with on_device(self.codes):
-            out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
-            code = dtype_code(out, "dtype")
-            check(_lib.load().nnb_mx4_dequantize(stream_of(out), code, self._rows, self._cols, ptr(self.codes),
-                                                 ptr(self.scales), ptr(out)), "nnb_mx4_dequantize")
+        if dtype not in DTYPES:
+            raise ValueError(f"dtype is {dtype}: expected float32, float16 or bfloat16")
+        with on_device(self):
+            out = torch.empty(self.shape, dtype=dtype, device=self.device)
+            codes, scales = self._pointers()
+            check(_lib.load().nnb_mx4_dequantize(stream_of(out), DTYPES[dtype], self._rows, self._cols, codes, scales,
+                                                 out.data_ptr()), "nnb_mx4_dequantize")
         return out
 
     def __repr__(self):
@@ -101,12 +125,13 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
     with on_device(x):
         v = _rows_view(x)
         rows, cols = v.shape
-        units, device, (row_stride, col_stride) = _units(rows, cols), x.device, v.stride()
-        codes = torch.empty(units + (4096,), dtype=torch.uint8, device=device)
-        scales = torch.empty(units + (256,), dtype=torch.uint8, device=device)
-        check(_lib.load().nnb_mx4_quantize(stream_of(x), code, rows, cols, ptr(v), row_stride, col_stride, ptr(codes),
-                                           ptr(scales)), "nnb_mx4_quantize")
-    return MX4Tensor.__new__(MX4Tensor)._take(codes, scales, x.shape, rows, cols)       # right by construction
+        units, (row_stride, col_stride) = _units(rows, cols), v.stride()
+        count = units[0] * units[1]
+        buffer = torch.empty(count * (4096 + 256), dtype=torch.uint8, device=x.device)
+        codes = buffer.data_ptr()
+        check(_lib.load().nnb_mx4_quantize(stream_of(x), code, rows, cols, v.data_ptr(), row_stride, col_stride, codes,
+                                           codes + count * 4096), "nnb_mx4_quantize")
+    return MX4Tensor._of_buffer(buffer, x.shape, rows, cols, units)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -144,36 +169,34 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else torch.float32 if quantized else x.dtype
     y_shape = tuple(x.shape[:-1]) + (n,)
-    with on_device(weight.codes):
+    with on_device(weight):
         if out is None:
             out = torch.empty(y_shape, dtype=out_dtype, device=device)
-        elif tuple(out.shape) != y_shape or out.dtype != out_dtype:
-            raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, expected {out_dtype} {y_shape}")
+            y_stride = n
         else:
-            if any(t is not None and share_memory(out, t) for t in ((x.codes, x.scales) if quantized else (x,))
-                   + (weight.codes, weight.scales, bias)):
-                raise ValueError("out shares memory with an input")
+            if tuple(out.shape) != y_shape or out.dtype != out_dtype:
+                raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, expected {out_dtype} {y_shape}")
+            no_grad("mx4.linear", out)
+            y_stride = n if out.is_contiguous() else _row_stride(out, n)
+            for t in (x._tensors() if quantized else (x,)) + weight._tensors() + (() if bias is None else (bias,)):
+                if share_memory(out, t):
+                    raise ValueError("out shares memory with an input")
             torch.autograd.graph.increment_version(out)              # the kernels write behind torch's back
-        no_grad("mx4.linear", out)
-        y_stride = n if out.is_contiguous() else _row_stride(out, n)
-        args = Mx4LinearArgs()
         if quantized:
-            rows = x._rows
-            args.x_codes, args.x_scales = ptr(x.codes), ptr(x.scales)
+            rows, x_ptr, row_stride, col_stride = x._rows, None, 0, 0
+            x_codes, x_scales = x._pointers()
         else:
             v = _rows_view(x)
-            rows = v.shape[0]
-            args.x = ptr(v)
-            args.x_row_stride, args.x_col_stride = v.stride()
-        args.rows, args.cols, args.out_features = rows, cols, n
-        args.w_codes, args.w_scales = ptr(weight.codes), ptr(weight.scales)
+            rows, x_ptr, x_codes, x_scales = v.shape[0], v.data_ptr(), None, None
+            row_stride, col_stride = v.stride()
+        w_codes, w_scales = weight._pointers()
         b = bias.contiguous() if bias is not None else None
-        args.bias = ptr(b) if b is not None else None
-        args.y, args.y_row_stride = ptr(out), y_stride
-        args.x_type, args.y_type, args.relu = x_type, dtype_code(out, "out"), int(bool(relu))
-        args.bias_type = dtype_code(bias, "bias") if bias is not None else 0
+        y_type = dtype_code(out, "out")
+        bias_type, b_ptr = (0, None) if b is None else (dtype_code(b, "bias"), b.data_ptr())
+        args = Mx4LinearArgs(rows, cols, n, x_ptr, row_stride, col_stride, x_codes, x_scales, w_codes, w_scales, b_ptr,
+                             out.data_ptr(), y_stride, x_type, bias_type, y_type, int(bool(relu)))
         nbytes = _workspace_bytes(rows, cols, n, quantized)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        check(_lib.load().nnb_mx4_linear(stream_of(out), C.byref(args), ptr(workspace) if nbytes else None, nbytes),
+        check(_lib.load().nnb_mx4_linear(stream_of(out), C.byref(args), workspace.data_ptr() if nbytes else None, nbytes),
               "nnb_mx4_linear")
     return out
