@@ -288,7 +288,7 @@ template <typename S> __host__ __device__ inline int upper_tiles(int mp) {
     return ortho_triangle(tiles_a_side<S>(mp));
 }
 
-template <typename T, int STAGE, typename S>
+template <typename T, int STAGE, typename S, bool ALL>
 __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams &p, const StageArgs &s, const OrthoGroup *items) {
     constexpr int TB = S::TB, RING = S::RING, kSub = S::kSub, kStride = kSub + 4, kUnits = S::kUnits, kGroup = S::WR * S::WC;
     constexpr bool symmetric = STAGE == STAGE_GRAM || STAGE == STAGE_POLY || STAGE == STAGE_MUL;
@@ -355,7 +355,7 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         // Every stage's sum from zero, smallest products first, added up by the vector pipe (see add_products).  On large
         // tiles a row of blocks at a time; the four blocks of small ones together, since a block's products wait for each
         // other, and added while the next stage multiplies (three 832 x 832 x 832: 17.0 us by rows, 16.1 so).
-        constexpr bool kAll = STAGE == STAGE_POLY || STAGE == STAGE_MUL, kFromZero = kAll || STAGE == STAGE_GRAM;
+        constexpr bool kAll = ALL, kFromZero = STAGE == STAGE_POLY || STAGE == STAGE_MUL || STAGE == STAGE_GRAM;
         f32x4 sum[2][TB][TB] = {};
         auto multiply = [&](auto from) {
             constexpr int B = from;
@@ -533,13 +533,14 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     }
 }
 
-template <int STAGE, typename S>
+// ALL: products of lo halves too (see add_products).
+template <int STAGE, typename S, bool ALL = false>
 __global__ __launch_bounds__(S::kThreads, 2) void ortho_product_kernel(OrthoShapes g, OrthoParams p, StageArgs s) {
-    product<float, STAGE, S>(g, p, s, nullptr);
+    product<float, STAGE, S, ALL>(g, p, s, nullptr);
 }
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads, 2) void ortho_finish_kernel(OrthoShapes g, OrthoParams p, StageArgs s, OrthoGroup items) {
-    product<T, STAGE_FINISH, S>(g, p, s, &items);
+    product<T, STAGE_FINISH, S, false>(g, p, s, &items);
 }
 
 // Adds up the parts of X X^T, one block of four waves per sub-tile (16 TB squared), and lays it out both ways round.
@@ -1058,6 +1059,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         else f(LoneTile{});
     };
     long long upper[2] = {}, full[2] = {};
+    int largest = 0;
     bool any64 = false, any128 = false, gram_of[2] = {}, reduce_of[2] = {};
     for (int i = 0; i < g.count; ++i) {
         const OrthoItem &it = g.item[i];
@@ -1069,6 +1071,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 upper[k] += (long long)it.batch * upper_tiles<S>(a.mp);
                 full[k] += (long long)it.batch * all_tiles<S>(a);
             });
+        largest = ortho_max(largest, a.mp);
         any64 |= a.mp == 64;
         any128 |= a.mp == 128;
         gram_of[a.sub == 64] = true;
@@ -1079,6 +1082,10 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     // 22.4 and 16.4.  Q X of 832 x 1536 three times, 252 large tiles: 27.7, 31.8 on small ones).
     auto pick = [](const long long (&n)[2]) { return n[0] >= 200 ? 0 : n[1] > 256 ? 1 : 2; };
     const int symmetric_tile = pick(upper), full_tile = pick(full);
+    // Where no square has more than 512 rows the products of lo halves are taken along: they cost little there (launches),
+    // and the plain float32 form is the more accurate the smaller the matrix (200 x 3000: 2.2e-6 of the result without, 2.0e-6
+    // with, plain 1.8e-6; 777 x 1501: 1.6e-6, 1.5e-6, plain 3.0e-6; three of them 304 us without, 332 with).
+    const bool all_products = largest <= 512;
     auto blocks = [&](auto &group, auto per_matrix) {
         int n = 0;
         for (int i = 0; i < g.count; ++i) {
@@ -1106,6 +1113,12 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         constexpr int STAGE = stage;
         with_tile(tile, [&](auto shape) {
             typedef decltype(shape) S;
+            if constexpr (STAGE == STAGE_POLY || STAGE == STAGE_MUL) {
+                if (all_products) {
+                    ortho_product_kernel<STAGE, S, true><<<grid, S::kThreads, 0, st>>>(shapes, p, s);
+                    return;
+                }
+            }
             ortho_product_kernel<STAGE, S><<<grid, S::kThreads, 0, st>>>(shapes, p, s);
         });
     };
