@@ -289,7 +289,15 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
 #pragma unroll
             for (int j = 0; j < TW; ++j)
                 acc[i][j] = mfma_mx4_32<S>(wf[S % kBuffers][j], xf[S % kBuffers][i], acc[i][j], sw[0][j], sx[0][i]);
-        __builtin_amdgcn_sched_barrier(0);                           // the products stay between the reads they hide
+        // The products stay between the reads they hide: nothing orders a matrix instruction and a load by itself.
+#pragma unroll
+        for (int i = 0; i < TX; ++i)
+#pragma unroll
+            for (int j = 0; j < TW; ++j) {
+                if constexpr (TX * TW >= 4) asm volatile("" : "+a"(acc[i][j]));
+                else asm volatile("" : "+v"(acc[i][j]));
+            }
+        __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
     for (int t = 0; t < RING - 1; ++t)
