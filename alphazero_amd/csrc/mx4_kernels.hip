@@ -248,13 +248,16 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
     const int sload = loads_scales ? wave : 0;
     const uint8_t *scales = (sload * 4 < kXUnits ? a.x_scales : a.w_scales) + unit_at(sload * 4) * 256;
     const uint32_t soffset = (uint32_t)(unit_at(sload * 4 + (lane >> 4)) - unit_at(sload * 4)) * 256 + (lane & 15) * 16;
+    constexpr int kLoads = 4 * kPerWave + 1;                         // of a stage, the last one of scales
+    auto issue_one = [&](int t, int slot, int n) {
+        if (n < 4 * kPerWave)
+            load_to_lds(codes[n / 4] + (size_t)t * 4096 + n % 4 * 1024, lane * 16, &lds[slot][wave * kPerWave + n / 4][n % 4 * 64]);
+        else if (kScaleLoads == kWaves || loads_scales)
+            load_to_lds(scales + (size_t)t * 256, soffset, &lds_scales[slot][sload * 4][0]);
+    };
     auto issue = [&](int t, int slot) {
 #pragma unroll
-        for (int i = 0; i < kPerWave; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                load_to_lds(codes[i] + (size_t)t * 4096 + j * 1024, lane * 16, &lds[slot][wave * kPerWave + i][j * 64]);
-        if (loads_scales) load_to_lds(scales + (size_t)t * 256, soffset, &lds_scales[slot][sload * 4][0]);
+        for (int n = 0; n < kLoads; ++n) issue_one(t, slot, n);
     };
     const int ux = wave % WX * TX, uw = kXUnits + wave / WX * TW;    // this wave's first units in the tile
 
@@ -282,28 +285,36 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
         else if (loads_scales) wait_and_meet<kInFlight + RING - 2>();
         else wait_and_meet<kInFlight>();
     };
-    auto multiply = [&](auto s) {
+    // A k-step's products, with between(n) behind product n.  They stay where they are: nothing orders a matrix instruction
+    // and a load by itself.
+    auto multiply_with = [&](auto s, auto &&between) {
         constexpr int S = s;
 #pragma unroll
         for (int i = 0; i < TX; ++i)
 #pragma unroll
-            for (int j = 0; j < TW; ++j)
-                acc[i][j] = mfma_mx4_32<S>(wf[S % kBuffers][j], xf[S % kBuffers][i], acc[i][j], sw[0][j], sx[0][i]);
-        // The products stay between the reads they hide: nothing orders a matrix instruction and a load by itself.
-#pragma unroll
-        for (int i = 0; i < TX; ++i)
-#pragma unroll
             for (int j = 0; j < TW; ++j) {
+                acc[i][j] = mfma_mx4_32<S>(wf[S % kBuffers][j], xf[S % kBuffers][i], acc[i][j], sw[0][j], sx[0][i]);
                 if constexpr (TX * TW >= 4) asm volatile("" : "+a"(acc[i][j]));
                 else asm volatile("" : "+v"(acc[i][j]));
+                between(i * TW + j);
             }
         __builtin_amdgcn_sched_barrier(0);
     };
+    auto multiply = [&](auto s) { multiply_with(s, [](int) {}); };
+    // Where a wave has many products and many loads, the loads go out one behind every second product of the last k-step
+    // (the stage's place is free from there on) and of the next stage's first: in a row they stop the wave until the
+    // memory pipe has taken them all.
+    constexpr bool kSpread = TX * TW >= 16;
+    constexpr int kFirst = TX * TW / 2;                              // loads of the last k-step
+    static_assert(!kSpread || (RING == 2 && AHEAD == 1 && kLoads == TX * TW + 1), "one behind every second product, one more in front");
 #pragma unroll
     for (int t = 0; t < RING - 1; ++t)
         if (t < stages) issue(t, t);
     meet(RING - 1 <= stages);
-    if (RING - 1 < stages) issue(RING - 1, RING - 1);
+    if (RING - 1 < stages) {
+#pragma unroll
+        for (int n = 0; n < (kSpread ? kFirst : kLoads); ++n) issue_one(RING - 1, RING - 1, n);
+    }
     static_for<AHEAD>([&](auto s) { fragments(0, s); });
     fragment_scales(0, 0);
     int slot = 0;
@@ -312,14 +323,24 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
         static_for<4>([&](auto s) {
             constexpr int S = s;
             if constexpr (S == 4 - AHEAD) {
-                meet(t + RING <= stages);
+                meet(!kSpread && t + RING <= stages);
                 fragment_scales(next, 1);
             }
             if constexpr (S + AHEAD < 4) fragments(slot, std::integral_constant<int, S + AHEAD>{});
             else fragments(next, std::integral_constant<int, S + AHEAD - 4>{});
-            if constexpr (S == 4 - AHEAD)
-                if (t + RING < stages) issue(t + RING, slot);
-            multiply(s);
+            if constexpr (kSpread && S == 3) {                       // behind the last stage the last again, never read
+                const int ahead = t + 2 < stages ? t + 2 : stages - 1;
+                multiply_with(s, [&](int n) { if (n % 2) issue_one(ahead, slot, n / 2); });
+            } else if constexpr (kSpread && S == 0) {                // the rest of the stage begun one step ago
+                multiply_with(s, [&](int n) {
+                    if (n == 0) issue_one(t + 1, next, kFirst);
+                    else if (n % 2) issue_one(t + 1, next, kFirst + 1 + n / 2);
+                });
+            } else {
+                if constexpr (!kSpread && S == 4 - AHEAD)
+                    if (t + RING < stages) issue(t + RING, slot);
+                multiply(s);
+            }
         });
 #pragma unroll
         for (int i = 0; i < TX; ++i) sx[0][i] = sx[1][i];
@@ -339,7 +360,7 @@ __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
     // Loops stay rolled where they can: this code runs once per tile, and what it costs is fetching its instructions.
     constexpr int kWidth = TW * 32, kStride = kWidth + 4, kPack = 16 / sizeof(T), kRowLanes = kWidth / kPack;
     static_assert((kWaves * 32 * kStride + kFeatures) * 4 <= (int)sizeof(lds), "the waves' parts and the bias fit");
-    __syncthreads();
+    wait_and_meet<0>();
     float *mine = reinterpret_cast<float *>(lds) + wave * 32 * kStride;
     float *bias = reinterpret_cast<float *>(lds) + kWaves * 32 * kStride;
     if ((int)threadIdx.x < kFeatures) {
