@@ -197,9 +197,12 @@ __device__ __forceinline__ void store_features(const Mx4Linear &a, long long r, 
 // rows, brought to LDS by the loads themselves into a ring of RING stages.  Operands are read from LDS AHEAD k-steps
 // before they multiply; all waves meet once per stage, when its last operands are in registers: from then on its place in
 // the ring is free for the stage RING further on, and the next one's operands are read while the last AHEAD k-steps
-// multiply.  Measured: 4096 rows of 11520 -> 1024 33.7 us (2.9 PFLOP/s), 8192 x 8192 x 8192 317 us (3.5 PFLOP/s; its
-// matrix instructions alone 170, eight waves instead of four 410).  What it waits for is the way into LDS: 68 KB a stage
-// at 54 bytes a clock, and the operands' way out of it.
+// multiply.
+// What bounds it: 8192 x 8192 x 8192 takes 278 us after a quantisation (4.0 PFLOP/s), 329 in a row of its own and 212 there
+// with codes of zero: the power cap (without the loads, 68 KB a stage for 2048 clocks of products, 291; touching lines
+// ahead of them saved nothing).  4096 rows of
+// 11520 -> 1024 take 33.2 us (2.9 PFLOP/s) on 128 x 128 tiles: 4 of it to store, the rest the operands' way out of LDS, 96 KB a
+// stage for 512 clocks of products (29 without the loads; four waves with half the reads 38).
 
 template <typename T, int WX, int WW, int TX, int TW, int RING, int AHEAD>
 __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {
@@ -557,7 +560,7 @@ namespace {
 //   rows kernel     3 + (1.2 + K / 2300) per 256 blocks of (64 rows x 16 features)
 //   128 x 128, one block of eight waves per CU (a ring of four stages)   3.5 + 0.6 per stage of 256 elements and 256 tiles
 //   128 x 128, two blocks of four waves per CU (two stages each)         3.5 + 0.9 per stage and 512 tiles
-//   256 x 256       8 + 1.65 per stage and 256 tiles
+//   256 x 256       8 + 1.65 per stage and 256 tiles (8192^3; less since its loads are spread)
 // For example 1024 rows of 11520 -> 1024: 26 / 31 / 35 / 86 us in this order, 2048 rows of 1024 -> 8192: 95 / 30 / 23 / 25.
 // The rows kernel and the tiles add a row's products in different orders, but all forms of each in one: with `order_rows`
 // the choice between the two goes by that count, so that a row's results do not depend on how many come with it.
