@@ -357,7 +357,8 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         // other, and added while the next stage multiplies (three 832 x 832 x 832: 17.0 us by rows, 16.1 so).
         constexpr bool kAll = ALL, kFromZero = STAGE == STAGE_POLY || STAGE == STAGE_MUL || STAGE == STAGE_GRAM;
         f32x4 sum[2][TB][TB] = {};
-        auto multiply = [&](auto from) {
+        auto nothing = [](auto) {};
+        auto multiply_with = [&](auto from, auto &&between) {    // between(n) behind every second of 48 products
             constexpr int B = from;
             if constexpr (TB == 2) {
                 auto products = [&](const half8 (&f)[TB], const half8 (&h)[TB], bool first) {
@@ -378,21 +379,34 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
                     for (int i = 0; i < TB; ++i)
 #pragma unroll
                         for (int j = 0; j < TB; ++j) acc[i][j] += sum[1 - B][i][j];
-            } else if constexpr (!kFromZero) {                   // a short sum without a large diagonal
-                static_for<TB>([&](auto row) { add_to<TB>(fh[B][row], fl[B][row], hh[B], hl[B], acc[row]); });
             } else {
                 static_for<TB>([&](auto row) {
                     constexpr int I = row;
-                    add_products<TB, kAll>(fh[B][I], fl[B][I], hh[B], hl[B], sum[0][I & 1]);
-                    if constexpr (I > 0)
+                    f32x4 (&to)[TB] = kFromZero ? sum[0][I & 1] : acc[I];
+                    if constexpr (kFromZero) {
+#pragma unroll
+                        for (int j = 0; j < TB; ++j) to[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        if constexpr (kAll)
+#pragma unroll
+                            for (int j = 0; j < TB; ++j) to[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[B][I], hl[B][j], to[j], 0, 0, 0);
+                    }
+                    static_for<3 * TB>([&](auto index) {
+                        constexpr int P = index / TB, J = index % TB, N = (I * 3 + P) * TB + J;
+                        to[J] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P == 0 ? fl[B][I] : fh[B][I], P == 1 ? hl[B][J] : hh[B][J], to[J], 0, 0, 0);
+                        asm volatile("" : "+v"(to[J]));          // holds it between the reads and loads around it
+                        if constexpr (N % 2 == 1) between(std::integral_constant<int, N / 2>{});
+                    });
+                    if constexpr (kFromZero && I > 0)
 #pragma unroll
                         for (int j = 0; j < TB; ++j) acc[I - 1][j] += sum[0][(I - 1) & 1][j];
                 });
+                if constexpr (kFromZero)
 #pragma unroll
-                for (int j = 0; j < TB; ++j) acc[TB - 1][j] += sum[0][(TB - 1) & 1][j];
+                    for (int j = 0; j < TB; ++j) acc[TB - 1][j] += sum[0][(TB - 1) & 1][j];
             }
             __builtin_amdgcn_sched_barrier(0);
         };
+        auto multiply = [&](auto from) { multiply_with(from, nothing); };
         auto add_last = [&](auto from) {
             constexpr int B = from;
             if constexpr (TB == 2 && kFromZero)
@@ -421,6 +435,18 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         int slot = 0;
         auto step = [&](int t, auto from, auto to) {             // multiplies stage t, reads stage t + 1
             const int next = slot + 1 == RING ? 0 : slot + 1;
+            if constexpr (TB == 4) {                             // behind the last stage the last again, never read
+                static_assert(TB != 4 || (kPerWave == 8 && RING == 2), "24 reads and loads");
+                meet(false);
+                const int ahead = t + RING < stages ? t + RING : stages - 1;
+                multiply_with(from, [&](auto n) {
+                    constexpr int N = n;
+                    if constexpr (N % 3 == 2) issue(ahead, slot, N / 3);
+                    else fragment(next, to, std::integral_constant<int, N - N / 3>{});
+                });
+                slot = next;
+                return;
+            }
             meet(t + RING <= stages);
             if (t + RING < stages)
 #pragma unroll
@@ -446,8 +472,8 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     }
 
     // The groups' sums meet in the first one's registers, its results in LDS, every wave's in its own part (free once all
-    // waves have read their last operands).
-    __syncthreads();
+    // waves have read their last operands and their last loads have landed).
+    wait_and_meet<0>();
     float *mine = reinterpret_cast<float *>(lds) + in_group * kSub * kStride;
     static_assert(S::KG <= 2, "");
     if (S::KG == 2) {
