@@ -265,14 +265,15 @@ struct StageArgs {
 
 // C = F G^T over K, both factors in units.  A block computes a tile of WR x WC sub-tiles (16 TB squared, one wave each)
 // with KG groups of such waves that share K; a stage is 32 of K per group, brought to LDS by the loads themselves into a
-// ring of RING stages; a wave reads a stage's operands into registers while it multiplies the one before, and all waves
-// meet once per stage.
+// ring of RING stages; a wave reads a stage's operands into registers while it multiplies the one before, a read or a load
+// behind every second product (of small tiles every product), and all waves meet once per stage.
 //
 // What bounds it: a CU takes in at most 64 bytes a clock (54 measured from L2, 18 to 24 from behind it), a 128 x 128
 // tile loads 32 KB a stage for 768 clocks of products, and the two overlap only where several blocks share a CU: of 1024 x
 // 1024 x 11520, loads alone take 50 us, products alone 46, both 73 with two blocks of four waves per CU.  One block per
 // CU is slower whatever it gains in reuse or depth (97 us with a ring of five stages, 85 with 128 x 256 tiles on eight
-// waves), and so is one load or read behind every few products (78).
+// waves).  Reads and loads between the products, not in front of them, take X X^T of that size from 45 to 40 us and a
+// product of squares (1024) from 12.2 to 11.4, and change nothing here.
 template <int TB_, int WR_, int WC_, int KG_, int RING_> struct Shape {
     static constexpr int TB = TB_, WR = WR_, WC = WC_, KG = KG_, RING = RING_, kSub = 16 * TB, kRows = WR * kSub, kCols = WC * kSub,
                          kWaves = WR * WC * KG, kThreads = 64 * kWaves, kUnits = (WR + WC) * TB;
@@ -358,27 +359,28 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         constexpr bool kAll = ALL, kFromZero = STAGE == STAGE_POLY || STAGE == STAGE_MUL || STAGE == STAGE_GRAM;
         f32x4 sum[2][TB][TB] = {};
         auto nothing = [](auto) {};
-        auto multiply_with = [&](auto from, auto &&between) {    // between(n) behind every second of 48 products
+        constexpr int kMemory = 4 * TB + kPerWave, kEvery = 3 * TB * TB / kMemory;      // reads and loads of a step
+        static_assert(kMemory * kEvery == 3 * TB * TB && (4 * TB) == 2 * kPerWave, "between the products, two reads and a load in turn");
+        auto multiply_with = [&](auto from, auto &&between) {    // between(n), n < kMemory, behind every kEvery products
             constexpr int B = from;
             if constexpr (TB == 2) {
-                auto products = [&](const half8 (&f)[TB], const half8 (&h)[TB], bool first) {
+                f32x4 (&to)[TB][TB] = kFromZero ? sum[B] : acc;
+                if constexpr (kFromZero)
 #pragma unroll
-                    for (int i = 0; i < TB; ++i)
+                    for (int i = 0; i < TB * TB; ++i) to[i / TB][i % TB] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (kAll)
 #pragma unroll
-                        for (int j = 0; j < TB; ++j) {
-                            f32x4 &to = kFromZero ? sum[B][i][j] : acc[i][j];
-                            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[i], h[j], kFromZero && first ? f32x4{0.f, 0.f, 0.f, 0.f} : to, 0, 0, 0);
-                        }
-                };
-                if (kAll) products(fl[B], hl[B], true);
-                products(fl[B], hh[B], !kAll);
-                products(fh[B], hl[B], false);
-                products(fh[B], hh[B], false);
-                if (kFromZero)
+                    for (int i = 0; i < TB * TB; ++i)
+                        to[i / TB][i % TB] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[B][i / TB], hl[B][i % TB], to[i / TB][i % TB], 0, 0, 0);
+                static_for<3 * TB * TB>([&](auto index) {
+                    constexpr int N = index, P = N / (TB * TB), I = N / TB % TB, J = N % TB;
+                    to[I][J] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P == 0 ? fl[B][I] : fh[B][I], P == 1 ? hl[B][J] : hh[B][J], to[I][J], 0, 0, 0);
+                    asm volatile("" : "+v"(to[I][J]));           // holds it between the reads and loads around it
+                    if constexpr (N % kEvery == kEvery - 1) between(std::integral_constant<int, N / kEvery>{});
+                });
+                if constexpr (kFromZero)
 #pragma unroll
-                    for (int i = 0; i < TB; ++i)
-#pragma unroll
-                        for (int j = 0; j < TB; ++j) acc[i][j] += sum[1 - B][i][j];
+                    for (int i = 0; i < TB * TB; ++i) acc[i / TB][i % TB] += sum[1 - B][i / TB][i % TB];
             } else {
                 static_for<TB>([&](auto row) {
                     constexpr int I = row;
@@ -393,8 +395,8 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
                     static_for<3 * TB>([&](auto index) {
                         constexpr int P = index / TB, J = index % TB, N = (I * 3 + P) * TB + J;
                         to[J] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P == 0 ? fl[B][I] : fh[B][I], P == 1 ? hl[B][J] : hh[B][J], to[J], 0, 0, 0);
-                        asm volatile("" : "+v"(to[J]));          // holds it between the reads and loads around it
-                        if constexpr (N % 2 == 1) between(std::integral_constant<int, N / 2>{});
+                        asm volatile("" : "+v"(to[J]));
+                        if constexpr (N % kEvery == kEvery - 1) between(std::integral_constant<int, N / kEvery>{});
                     });
                     if constexpr (kFromZero && I > 0)
 #pragma unroll
@@ -416,43 +418,28 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
                     for (int j = 0; j < TB; ++j) acc[i][j] += sum[B][i][j];
         };
         constexpr int kInFlight = (RING - 2) * kPerWave;         // a wave's loads behind the stage it waits for
-        auto meet = [&](bool all_issued) {
-            if (all_issued) wait_and_meet<kInFlight>();
-            else wait_and_meet<0>();
-        };
+        // behind the last stage the last again, never read: so many loads are in flight behind a stage throughout
+        auto at_most = [&](int t) { return t < stages ? t : stages - 1; };
         constexpr std::integral_constant<int, 0> even{};
         constexpr std::integral_constant<int, 1> odd{};
 #pragma unroll
         for (int t = 0; t < RING - 1; ++t)
-            if (t < stages)
 #pragma unroll
-                for (int d = 0; d < kPerWave; ++d) issue(t, t, d);
-        meet(RING - 1 <= stages);
-        if (RING - 1 < stages)
+            for (int d = 0; d < kPerWave; ++d) issue(at_most(t), t, d);
+        wait_and_meet<kInFlight>();
 #pragma unroll
-            for (int d = 0; d < kPerWave; ++d) issue(RING - 1, RING - 1, d);
+        for (int d = 0; d < kPerWave; ++d) issue(at_most(RING - 1), RING - 1, d);
         static_for<4 * TB>([&](auto r) { fragment(0, even, r); });
         int slot = 0;
         auto step = [&](int t, auto from, auto to) {             // multiplies stage t, reads stage t + 1
             const int next = slot + 1 == RING ? 0 : slot + 1;
-            if constexpr (TB == 4) {                             // behind the last stage the last again, never read
-                static_assert(TB != 4 || (kPerWave == 8 && RING == 2), "24 reads and loads");
-                meet(false);
-                const int ahead = t + RING < stages ? t + RING : stages - 1;
-                multiply_with(from, [&](auto n) {
-                    constexpr int N = n;
-                    if constexpr (N % 3 == 2) issue(ahead, slot, N / 3);
-                    else fragment(next, to, std::integral_constant<int, N - N / 3>{});
-                });
-                slot = next;
-                return;
-            }
-            meet(t + RING <= stages);
-            if (t + RING < stages)
-#pragma unroll
-                for (int i = 0; i < kPerWave; ++i) issue(t + RING, slot, i);
-            static_for<4 * TB>([&](auto r) { fragment(next, to, r); });
-            multiply(from);
+            wait_and_meet<kInFlight>();
+            const int ahead = at_most(t + RING);
+            multiply_with(from, [&](auto n) {
+                constexpr int N = n;
+                if constexpr (N % 3 == 2) issue(ahead, slot, N / 3);
+                else fragment(next, to, std::integral_constant<int, N - N / 3>{});
+            });
             slot = next;
         };
         // pairs of stages, for the two sets of registers; an odd last one by itself
