@@ -284,3 +284,21 @@ def test_large_offsets():
     got = mx4.linear(x, mx4.quantize(w.cuda()), out_dtype=torch.float32)
     assert not got[:-4].any()
     _check_linear(got[-4:], tail, w, None, False)
+
+
+@pytest.mark.parametrize("rows,cols,out", [(32768, 200, 32800), (20000, 500, 30000), (5000, 4096, 5001), (6000, 11000, 6100)])
+def test_linear_largest_tiles(rows, cols, out):
+    """Sizes at which 256 x 256 tiles multiply, with one stage of K, two, many and an odd number.  Rows from the start, the
+    middle and the end against float64 sums of the rounded operands, with the bounds of the smaller cases."""
+    torch = _torch()
+    from alphazero_amd import mx4
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, w = torch.randn(rows, cols, generator=g, device="cuda"), torch.randn(out, cols, generator=g, device="cuda")
+    rounded, weight = mx4.quantize(x), mx4.quantize(w)
+    y = mx4.linear(x, weight, out_dtype=torch.bfloat16)
+    xq, wq = rounded.dequantize(), weight.dequantize().double().t().contiguous()
+    steps = -(-cols // 128) + 32 + 16 + 1
+    for first in (0, rows // 2 - 40, rows - 130):
+        part = xq[first:first + 130].double()
+        want, size = part @ wq, part.abs() @ wq.abs()
+        assert ((y[first:first + 130].double() - want).abs() <= steps * 2.0 ** -23 * size + 2.0 ** -8 * want.abs()).all()
