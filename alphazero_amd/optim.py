@@ -124,9 +124,13 @@ def muon_update(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     if inplace:
         used = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written)
                       for ts, written in ((weights, True), (momenta, True), (grads, False)) for t in ts if t.numel())
-        for (_, end, a), (start, _, b) in zip(used, used[1:]):
-            if end > start and (a or b):
+        any_end = written_end = 0                     # how far the ranges so far reach, and the written ones among them
+        for start, end, written in used:
+            if start < written_end or (written and start < any_end):
                 raise ValueError("a weight or momentum shares memory with another tensor of the call")
+            any_end = max(any_end, end)
+            if written:
+                written_end = max(written_end, end)
     with on_device(first):
         wv = [_as_matrix(t, f"weights[{i}]") for i, t in enumerate(weights)]
         gv = [_as_matrix(t, f"grads[{i}]") for i, t in enumerate(grads)]
