@@ -42,6 +42,16 @@ def no_grad(what: str, *tensors):
         raise NnbError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
+def resolved(t: torch.Tensor) -> torch.Tensor:
+    """t as its memory holds it: the imaginary part of a conjugate is a view marked as negated, over numbers that are not."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
+def writable(t: torch.Tensor, name: str):
+    if t.is_neg():
+        raise ValueError(f"{name} is a negated view: the kernels would write the numbers without the sign")
+
+
 def _span(t: torch.Tensor) -> tuple:
     """First and last address + 1 of the elements (torch's strides are never negative)."""
     reach = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))

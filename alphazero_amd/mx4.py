@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._lib import Mx4LinearArgs, check
-from ._tensors import DTYPES, dtype_code, no_grad, on_device, share_memory, stream_of
+from ._tensors import DTYPES, dtype_code, no_grad, on_device, resolved, share_memory, stream_of, writable
 
 BLOCK = 32                              # elements that share a scale
 UNIT_ROWS, UNIT_COLS = 32, 256          # rows and columns are padded with zeros to whole units
@@ -100,6 +100,7 @@ class MX4Tensor:
 
 def _rows_view(x: torch.Tensor) -> torch.Tensor:
     """x as [rows, cols] without a copy where its strides allow one view."""
+    x = resolved(x)
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
 
 
@@ -168,6 +169,8 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
         raise ValueError(f"bias of shape {tuple(bias.shape)}, expected {(n,)}")
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else torch.float32 if quantized else x.dtype
+    if out is not None:
+        writable(out, "out")
     y_shape = tuple(x.shape[:-1]) + (n,)
     with on_device(weight):
         if out is None:
@@ -190,7 +193,7 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
             rows, x_ptr, x_codes, x_scales = v.shape[0], v.data_ptr(), None, None
             row_stride, col_stride = v.stride()
         w_codes, w_scales = weight._pointers()
-        b = bias.contiguous() if bias is not None else None
+        b = resolved(bias).contiguous() if bias is not None else None
         y_type = dtype_code(out, "out")
         bias_type, b_ptr = (0, None) if b is None else (dtype_code(b, "bias"), b.data_ptr())
         args = Mx4LinearArgs(rows, cols, n, x_ptr, row_stride, col_stride, x_codes, x_scales, w_codes, w_scales, b_ptr,

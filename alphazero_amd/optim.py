@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._lib import NS_MAX_STEPS, MuonMatrix, MuonParams, NewtonSchulz, check
-from ._tensors import dtype_code, no_grad, on_device, ptr, share_memory, stream_of
+from ._tensors import dtype_code, no_grad, on_device, ptr, resolved, share_memory, stream_of, writable
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
@@ -59,10 +59,12 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=QUINTIC, eps: fl
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device):
         raise ValueError(f"out is {out.dtype} {tuple(out.shape)} on {out.device}, expected {x.dtype} {tuple(x.shape)} on {x.device}")
     given = out
+    if out is not None:
+        writable(out, "out")
     if out is not None and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) and share_memory(out, x):
         raise ValueError("out shares memory with x but is not x")
     with on_device(x):
-        x = x.detach()
+        x = resolved(x.detach())
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         rows, cols = x.shape[-2:]
@@ -90,7 +92,7 @@ def _as_matrix(t: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name} of shape {tuple(t.shape)} is no matrix")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t.detach()
+    return resolved(t.detach())
 
 
 @torch.no_grad()
@@ -122,6 +124,9 @@ def muon_update(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
         if any(t.device != first.device for t in (w, g, m)):
             raise ValueError(f"matrix {i}: all tensors must be on {first.device}")
     if inplace:
+        for name, ts in (("weights", weights), ("momenta", momenta)):
+            for i, t in enumerate(ts):
+                writable(t, f"{name}[{i}]")
         used = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written)
                       for ts, written in ((weights, True), (momenta, True), (grads, False)) for t in ts if t.numel())
         any_end = written_end = 0                     # how far the ranges so far reach, and the written ones among them

@@ -20,3 +20,30 @@ def test_muon_update_sees_memory_shared_inside_a_longer_gradient():
     # gradients may share memory with each other, and neighbours may touch: only the device is wrong then
     with pytest.raises(NnbError):
         optim.muon_update([flat[900:904].view(2, 2), z(30, 30)], [inner, outer], [z(2, 2), z(30, 30)], lr=0.1)
+
+
+def _negated(t):
+    """-t as torch makes it for the imaginary part of a conjugate: t's own memory and a mark."""
+    import torch
+    view = torch.complex(torch.zeros_like(t), t).conj().imag
+    assert view.is_neg() and torch.equal(view, -t)
+    return view
+
+
+def test_negated_views_are_not_written_to():
+    import torch
+    from alphazero_amd import mx4, optim
+    weight = mx4.MX4Tensor(torch.zeros(1, 1, 4096, dtype=torch.uint8), torch.zeros(1, 1, 256, dtype=torch.uint8), (8, 64))
+    x = torch.ones(3, 64)
+    with pytest.raises(ValueError, match="negated"):
+        mx4.linear(x, weight, out=torch._neg_view(torch.zeros(3, 8)))
+    with pytest.raises(ValueError, match="negated"):
+        optim.orthogonalize(x, out=_negated(x))
+    with pytest.raises(ValueError, match="negated"):
+        optim.orthogonalize(_negated(x), out=_negated(x))
+    z = torch.zeros
+    for which in (0, 2):
+        args = [[z(4, 8)], [z(4, 8)], [z(4, 8)]]
+        args[which][0] = torch._neg_view(z(4, 8))
+        with pytest.raises(ValueError, match="negated"):
+            optim.muon_update(*args, lr=0.1)
