@@ -5,6 +5,7 @@ import contextlib
 import ctypes as C
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from ._lib import NnbError
 
@@ -40,6 +41,12 @@ def ptr(t: torch.Tensor) -> C.c_void_p:
 def no_grad(what: str, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NnbError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    no_tangent(what, *tensors)
+
+
+def no_tangent(what: str, *tensors):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NnbError(f"{what} has no forward-mode derivative: call it on tensors without a tangent")
 
 
 def resolved(t: torch.Tensor) -> torch.Tensor:

@@ -9,8 +9,8 @@ as halves, and a weight takes 4.25 bits.
     y = mx4.linear(x, weight, bias=layer.bias, relu=True)  # x is quantised on the way in, sums are float32
 
 The functions run on the tensors' device, on torch's current stream there; they wait for nothing and can be captured into
-a graph.  They have no backward pass and refuse tensors that ask for one.  Engine(precision="mx4") evaluates the
-network's linear layer with the same kernels.
+a graph.  They have no derivatives and refuse tensors that ask for a backward pass or carry a forward-mode tangent.
+Engine(precision="mx4") evaluates the network's linear layer with the same kernels.
 """
 from __future__ import annotations
 
@@ -171,6 +171,7 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
         out_dtype = out.dtype if out is not None else torch.float32 if quantized else x.dtype
     if out is not None:
         writable(out, "out")
+        no_grad("mx4.linear", out)
     y_shape = tuple(x.shape[:-1]) + (n,)
     with on_device(weight):
         if out is None:
@@ -179,7 +180,6 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
         else:
             if tuple(out.shape) != y_shape or out.dtype != out_dtype:
                 raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, expected {out_dtype} {y_shape}")
-            no_grad("mx4.linear", out)
             y_stride = n if out.is_contiguous() else _row_stride(out, n)
             for t in (x._tensors() if quantized else (x,)) + weight._tensors() + (() if bias is None else (bias,)):
                 if share_memory(out, t):

@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._lib import NS_MAX_STEPS, MuonMatrix, MuonParams, NewtonSchulz, check
-from ._tensors import dtype_code, no_grad, on_device, ptr, resolved, share_memory, stream_of, writable
+from ._tensors import dtype_code, no_grad, no_tangent, on_device, ptr, resolved, share_memory, stream_of, writable
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
@@ -50,7 +50,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=QUINTIC, eps: fl
     times X <- a X + b (X X^T) X + c (X X^T)^2 X: the singular values go towards 1, the singular vectors stay.
 
     float32-faithful inside whatever the type, one rounding at the end.  A matrix with a NaN or an infinity gives NaN.
-    `out` (same shape and type; x itself, or no element in common with it) is written instead of a new tensor when given.  No backward pass."""
+    `out` (same shape and type; x itself, or no element in common with it) is written instead of a new tensor when given.
+    No derivatives."""
     code = dtype_code(x, "x")
     no_grad("optim.orthogonalize", x, out)
     if x.dim() < 2:
@@ -115,6 +116,7 @@ def muon_update(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
         return weights, momenta
     first = weights[0]
     code = dtype_code(first, "weights[0]")
+    no_tangent("optim.muon_update", *weights, *grads, *momenta)
     for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
         if w.dtype != first.dtype or g.dtype != first.dtype or m.dtype != torch.float32:
             raise ValueError(f"matrix {i}: weight {w.dtype}, gradient {g.dtype}, momentum {m.dtype}; expected {first.dtype}, "

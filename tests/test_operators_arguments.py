@@ -47,3 +47,29 @@ def test_negated_views_are_not_written_to():
         args[which][0] = torch._neg_view(z(4, 8))
         with pytest.raises(ValueError, match="negated"):
             optim.muon_update(*args, lr=0.1)
+
+
+def test_forward_mode_tangents_are_refused():
+    """The kernels would return a result without a tangent, which reads as a derivative of zero."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+    from alphazero_amd import mx4, optim
+    from alphazero_amd._lib import NnbError
+    weight = mx4.MX4Tensor(torch.zeros(1, 1, 4096, dtype=torch.uint8), torch.zeros(1, 1, 256, dtype=torch.uint8), (8, 64))
+    x, z = torch.ones(8, 64), torch.zeros
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, x)
+        for guard in (torch.enable_grad, torch.no_grad):              # neither switches tangents on or off
+            with guard():
+                for call in (lambda: mx4.quantize(dual), lambda: mx4.linear(dual, weight),
+                             lambda: mx4.linear(x, weight, bias=fwd.make_dual(z(8), z(8))), lambda: optim.orthogonalize(dual),
+                             lambda: mx4.linear(x, weight, out=fwd.make_dual(z(8, 8), z(8, 8))),
+                             lambda: optim.orthogonalize(x, out=fwd.make_dual(z(8, 64), x)),
+                             lambda: optim.muon_update([x.clone()], [dual], [z(8, 64)], lr=0.1),
+                             lambda: optim.muon_update([fwd.make_dual(x.clone(), x)], [x], [z(8, 64)], lr=0.1, inplace=False),
+                             lambda: optim.muon_update([x.clone()], [x], [fwd.make_dual(z(8, 64), x)], lr=0.1)):
+                    with pytest.raises(NnbError, match="forward-mode"):
+                        call()
+        for call in (lambda: mx4.quantize(x), lambda: optim.muon_update([x.clone()], [x], [z(8, 64)], lr=0.1)):
+            with pytest.raises(NnbError, match="no CPU path"):        # a plain tensor under a dual level is as good as any
+                call()
