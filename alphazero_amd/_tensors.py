@@ -65,6 +65,19 @@ def _span(t: torch.Tensor) -> tuple:
     return t.data_ptr(), t.data_ptr() + (reach + 1) * t.element_size()
 
 
+def overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two of t's elements may share memory: from the smallest stride up, each has to step over all that the smaller
+    ones reach."""
+    if t.numel() == 0:
+        return False
+    reach = 0
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s <= reach:
+            return True
+        reach += (n - 1) * s
+    return False
+
+
 def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors may have elements in common.  Column ranges of one buffer that lie apart are recognised; of
     other interleaved views it is assumed."""

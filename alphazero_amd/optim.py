@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._lib import NS_MAX_STEPS, MuonMatrix, MuonParams, NewtonSchulz, check
-from ._tensors import dtype_code, no_grad, no_tangent, on_device, ptr, resolved, share_memory, stream_of, writable
+from ._tensors import dtype_code, no_grad, no_tangent, on_device, overlaps_itself, ptr, resolved, share_memory, stream_of, writable
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
@@ -62,6 +62,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=QUINTIC, eps: fl
     given = out
     if out is not None:
         writable(out, "out")
+        if overlaps_itself(out):
+            raise ValueError("out has elements that share memory")
     if out is not None and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) and share_memory(out, x):
         raise ValueError("out shares memory with x but is not x")
     with on_device(x):
@@ -74,8 +76,6 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=QUINTIC, eps: fl
             ob = out if out.dim() == 3 else out.view((-1, rows, cols) if x.numel() else (0, rows, cols))
         except RuntimeError:
             raise ValueError(f"out of shape {tuple(out.shape)}, strides {out.stride()} is no evenly spaced batch of matrices") from None
-        if out.numel() and any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
-            raise ValueError("out has elements that share memory")
         lib = _lib.load()
         nbytes = C.c_size_t()
         check(lib.nnb_orthogonalize_workspace_bytes(xb.shape[0], rows, cols, C.byref(nbytes)), "nnb_orthogonalize_workspace_bytes")

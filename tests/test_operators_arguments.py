@@ -73,3 +73,25 @@ def test_forward_mode_tangents_are_refused():
         for call in (lambda: mx4.quantize(x), lambda: optim.muon_update([x.clone()], [x], [z(8, 64)], lr=0.1)):
             with pytest.raises(NnbError, match="no CPU path"):        # a plain tensor under a dual level is as good as any
                 call()
+
+
+def test_orthogonalize_refuses_an_out_that_overlaps_itself():
+    import torch
+    from alphazero_amd import optim
+    from alphazero_amd._lib import NnbError
+    x, flat = torch.zeros(6, 20), torch.zeros(400)
+    for out in (flat[:25].unfold(0, 20, 1), flat.as_strided((6, 20), (19, 1)), flat.as_strided((6, 20), (3, 4)),
+                flat.as_strided((6, 20), (0, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            optim.orthogonalize(x, out=out)
+    windows = flat[:25].unfold(0, 20, 1)                              # reading overlapping rows is fine, writing over them is not
+    with pytest.raises(ValueError, match="share memory"):
+        optim.orthogonalize(windows, out=windows)
+    with pytest.raises(ValueError, match="share memory"):
+        optim.orthogonalize(x.expand(3, 6, 20), out=flat.as_strided((3, 6, 20), (119, 20, 1)))
+    for out in (flat.as_strided((6, 20), (20, 1)), flat.as_strided((6, 20), (1, 6)), flat.as_strided((6, 20), (41, 2)),
+                flat[1:].as_strided((6, 20), (1, 7))):
+        with pytest.raises(NnbError, match="no CPU path"):
+            optim.orthogonalize(x, out=out)
+    with pytest.raises(NnbError, match="no CPU path"):                # a stride of a dimension of one says nothing
+        optim.orthogonalize(x[:1], out=flat.as_strided((1, 20), (1, 1)))
