@@ -8,7 +8,8 @@ counts as output channels x everything else); biases, heads and embeddings belon
     muon, adam = optim.Muon(matrices, lr=0.02), torch.optim.Adam(rest)
 
 The kernels run on the tensors' device, on torch's current stream there, and wait for nothing.  They can be captured into
-a graph, which then keeps the learning rate and the other numbers of the call it recorded.
+a graph, which then keeps the learning rate and the other numbers of the call it recorded; `Muon` makes its momenta in its
+first step, which has to come before the capture.
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ from typing import List, Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import NS_MAX_STEPS, MuonMatrix, MuonParams, NewtonSchulz, check
+from ._lib import NS_MAX_STEPS, MuonMatrix, MuonParams, NewtonSchulz, NnbError, check
 from ._tensors import dtype_code, no_grad, no_tangent, on_device, overlaps_itself, ptr, resolved, share_memory, stream_of, writable
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
@@ -195,6 +196,8 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 if "momentum" not in self.state[p]:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise NnbError("a new momentum's zeros would be part of the graph: make one step before it is captured")
                     self.state[p]["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 batches.setdefault((p.device, p.dtype), []).append(p)
             for params in batches.values():

@@ -35,3 +35,30 @@ def test_negated_views_read_as_their_negative():
     want = optim.muon_update([-w], [x], [-m], lr=0.1, inplace=False)
     got = optim.muon_update([torch._neg_view(w)], [x], [torch._neg_view(m)], lr=0.1, inplace=False)
     assert all(torch.equal(a[0], c[0]) for a, c in zip(got, want))
+
+
+def test_muon_in_a_graph_behind_one_eager_step():
+    torch = _torch()
+    from alphazero_amd import optim
+    from alphazero_amd._lib import NnbError
+    g = torch.Generator().manual_seed(2)
+    start, grad = torch.randn(40, 90, generator=g).cuda(), torch.randn(40, 90, generator=g).cuda()
+    eager, p = (torch.nn.Parameter(start.clone()) for _ in range(2))
+    eager.grad, p.grad = grad.clone(), grad.clone()
+    a, b = optim.Muon([eager], lr=0.1), optim.Muon([p], lr=0.1)
+    with pytest.raises(NnbError, match="momentum"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            b.step()
+    assert torch.equal(p, start)
+    a.step()
+    b.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.step()
+    for k in range(4):
+        for t in (eager, p):
+            t.grad.copy_(grad * (k + 2))
+        a.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(p, eager) and torch.equal(a.state[eager]["momentum"], b.state[p]["momentum"]), k
