@@ -196,7 +196,7 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 if "momentum" not in self.state[p]:
-                    if torch.cuda.is_current_stream_capturing():
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
                         raise NnbError("a new momentum's zeros would be part of the graph: make one step before it is captured")
                     self.state[p]["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 batches.setdefault((p.device, p.dtype), []).append(p)

@@ -97,18 +97,11 @@ def test_orthogonalize_refuses_an_out_that_overlaps_itself():
         optim.orthogonalize(x[:1], out=flat.as_strided((1, 20), (1, 1)))
 
 
-def test_muon_refuses_to_create_its_momentum_inside_a_graph(monkeypatch):
-    """The zeros of a new momentum would be part of the graph: every replay would forget what the last one added."""
+def test_muon_on_the_cpu_says_that_it_has_no_path_there():
     import torch
     from alphazero_amd import optim
     from alphazero_amd._lib import NnbError
     p = torch.nn.Parameter(torch.randn(4, 8))
     p.grad = torch.ones(4, 8)
-    opt = optim.Muon([p], lr=0.1)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
-    with pytest.raises(NnbError, match="momentum"):
-        opt.step()
-    assert not opt.state[p]
-    opt.state[p]["momentum"] = torch.zeros(4, 8)                      # one that exists is updated by the graph as it should be
     with pytest.raises(NnbError, match="no CPU path"):
-        opt.step()
+        optim.Muon([p], lr=0.1).step()
