@@ -180,6 +180,8 @@ struct Mx4Linear {                      // y [rows][n] = x * w^T (+ bias, ReLU)
     int kp, n, bias_type, y_type, relu, wide;
     long long order_rows;               // > 0: the sums are ordered as in a product of this many rows
 };
+// A launch has less than 2^32 threads, and few rows take a block of 512 for every 16 features.
+constexpr long long kMx4MaxFeatures = (1LL << 27) - 16;
 struct Mx4Rows {                        // rows that are still numbers
     const void *x;
     long long row_stride, col_stride;

@@ -1416,6 +1416,8 @@ int nnb_mx4_linear_workspace_bytes(int64_t rows, int64_t cols, int64_t out_featu
     if (!bytes_out) return fail(NNB_ERR_ARG, "bytes_out is null");
     if (int rc = check_mx4_shape(rows, cols)) return rc;
     if (int rc = check_mx4_shape(out_features, cols)) return rc;
+    if (out_features > kMx4MaxFeatures)
+        return fail(NNB_ERR_ARG, "%lld output features, more than 2^27 - 16", (long long)out_features);
     Carver c(nullptr);
     uint8_t *codes, *scales;
     carve_mx4_rows(c, rows, (int)cols, x_quantized != 0, codes, scales);

@@ -412,7 +412,8 @@ int nnb_mx4_dequantize(void *stream, int out_type, int64_t rows, int64_t cols, c
 /* y = x w^T (+ bias) (then ReLU): a linear layer on 4-bit weights.  x is given either as numbers (x, x_type, strides: it
  * is quantised as nnb_mx4_quantize does, into the workspace) or already quantised (x = NULL, x_codes / x_scales);
  * products of codes and scales are exact, sums, bias and ReLU in float32, one rounding to y_type at the end.
- * y [rows][out_features], row r at y + r*y_row_stride, must not overlap the inputs. */
+ * y [rows][out_features], row r at y + r*y_row_stride, must not overlap the inputs.  rows and cols as above,
+ * out_features at most 2^27 - 16. */
 typedef struct nnb_mx4_linear_args {
     int64_t rows, cols, out_features;
     const void *x;

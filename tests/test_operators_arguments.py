@@ -105,3 +105,18 @@ def test_muon_on_the_cpu_says_that_it_has_no_path_there():
     p.grad = torch.ones(4, 8)
     with pytest.raises(NnbError, match="no CPU path"):
         optim.Muon([p], lr=0.1).step()
+
+
+def test_mx4_linear_refuses_more_features_than_a_grid_holds():
+    """A launch has less than 2^32 threads, 512 for every 16 features."""
+    import ctypes as C
+    from alphazero_amd import _lib
+    lib, n, most = _lib.load(), C.c_size_t(), 2 ** 27 - 16
+    for rows in (0, 1, 40):
+        assert lib.nnb_mx4_linear_workspace_bytes(rows, 32, most, 0, C.byref(n)) == 0
+        for features in (most + 1, 2 ** 27, 2 ** 31 - 1):
+            assert lib.nnb_mx4_linear_workspace_bytes(rows, 32, features, 0, C.byref(n)) == -1
+            assert "features" in lib.nnb_last_error().decode()
+            a = _lib.Mx4LinearArgs(rows=rows, cols=32, out_features=features, x=4096, x_row_stride=32, x_col_stride=1,
+                                   w_codes=4096, w_scales=4096, y=4096, y_row_stride=features)
+            assert lib.nnb_mx4_linear(None, C.byref(a), C.c_void_p(4096), 1 << 30) == -1
