@@ -171,6 +171,13 @@ def self_play_sample_tensors(agent, num_games, first_game_id: int = 0):
     return eng.trajectory_samples(traj)
 
 
+def _check_trainable(agent):
+    """Before any work: the hidden weights are stepped by kernels that have no CPU path."""
+    device = next(agent.model.parameters()).device
+    if device.type != "cuda":
+        raise RuntimeError(f"the network is on {device}: training needs it on the GPU (use_gpu=True)")
+
+
 def train_network(agent, planes: torch.Tensor, probs: torch.Tensor, z: torch.Tensor, epochs: int = 1, batch_size: int = 32,
                   lr: float = 1e-3, muon_lr: float = 0.02, weight_decay: float = 0.0,
                   time_limit: Optional[float] = None, seed: int = 0) -> List[float]:
@@ -180,6 +187,7 @@ def train_network(agent, planes: torch.Tensor, probs: torch.Tensor, z: torch.Ten
     order each epoch (from `seed`).  Ends after `epochs`, or with the batch that `time_limit` seconds run out in.
     Returns each epoch's mean loss.  The network has to be on the GPU (use_gpu=True): Muon has no CPU path."""
     from . import optim
+    _check_trainable(agent)
     n = int(planes.shape[0])
     if probs.shape[0] != n or z.shape[0] != n:
         raise ValueError(f"{n} positions, {probs.shape[0]} distributions and {z.shape[0]} results")
@@ -225,6 +233,7 @@ def train_alphazero(time_limit, num_self_play_games=100, use_gpu=True, load_mode
     from .agent import MODEL_PATH, initialize_agent
     agent = initialize_agent(action_dim=7, state_dim=2, use_gpu=use_gpu, num_simulations=800, c_puct=1.4,
                              load_model=load_model)
+    _check_trainable(agent)
     planes, probs, z = self_play_sample_tensors(agent, num_self_play_games)
     train_network(agent, planes, probs, z, epochs=10, time_limit=time_limit)
     os.makedirs(os.path.dirname(MODEL_PATH), exist_ok=True)
