@@ -227,15 +227,26 @@ def train_network(agent, planes: torch.Tensor, probs: torch.Tensor, z: torch.Ten
     return losses
 
 
-def train_alphazero(time_limit, num_self_play_games=100, use_gpu=True, load_model=True):
-    """train_alpha_zero.py:57-119: self-play, then training on its per-ply samples for `time_limit` seconds, ten
-    epochs at most, then the network is saved to agent.MODEL_PATH.  Returns the agent."""
-    from .agent import MODEL_PATH, initialize_agent
-    agent = initialize_agent(action_dim=7, state_dim=2, use_gpu=use_gpu, num_simulations=800, c_puct=1.4,
-                             load_model=load_model)
+def _play_for_training(agent, num_games):
+    """Self-play for one fit: the per-ply samples."""
+    return self_play_sample_tensors(agent, num_games)
+
+
+def train_agent(agent, time_limit, num_self_play_games):
+    """Self-play with `agent`, then training on its per-ply samples for `time_limit` seconds, ten epochs at most, then the
+    network is saved to agent.MODEL_PATH."""
+    from .agent import MODEL_PATH
     _check_trainable(agent)
-    planes, probs, z = self_play_sample_tensors(agent, num_self_play_games)
+    planes, probs, z = _play_for_training(agent, num_self_play_games)
     train_network(agent, planes, probs, z, epochs=10, time_limit=time_limit)
     os.makedirs(os.path.dirname(MODEL_PATH), exist_ok=True)
     agent.save_model(MODEL_PATH)
+
+
+def train_alphazero(time_limit, num_self_play_games=100, use_gpu=True, load_model=True):
+    """train_alpha_zero.py:57-119: train_agent with a new agent of 800 simulations a move.  Returns the agent."""
+    from .agent import initialize_agent
+    agent = initialize_agent(action_dim=7, state_dim=2, use_gpu=use_gpu, num_simulations=800, c_puct=1.4,
+                             load_model=load_model)
+    train_agent(agent, time_limit, num_self_play_games)
     return agent

@@ -28,3 +28,33 @@ def test_training_on_the_cpu_is_refused_before_a_game_is_played(played):
     with pytest.raises(RuntimeError, match="GPU"):
         train_network(agent, torch.zeros(4, 2, 6, 7), torch.zeros(4, 7), torch.zeros(4))
     assert not played
+
+
+@pytest.fixture
+def stand_ins(monkeypatch, tmp_path):
+    """Self-play and the fit replaced: notes who plays, who is fitted to what, and where the result is saved."""
+    from alphazero_amd import selfplay
+    notes = []
+    monkeypatch.chdir(tmp_path)
+    monkeypatch.setattr(selfplay, "_check_trainable", lambda agent: None)
+    monkeypatch.setattr(selfplay, "_play_for_training", lambda agent, n: notes.append(("play", agent, n)) or ("planes", "probs", "z"))
+    monkeypatch.setattr(selfplay, "train_network",
+                        lambda agent, *samples, **kw: notes.append(("fit", agent, samples, kw["time_limit"])) or [])
+    return notes
+
+
+def test_perform_training_trains_the_agent_itself(stand_ins):
+    from alphazero_amd.agent import MODEL_PATH, initialize_agent
+    agent = initialize_agent(load_model=False)
+    with torch.no_grad():
+        agent.model.value_head.bias.fill_(3.0)
+    agent.perform_training()
+    assert stand_ins == [("play", agent, 1000), ("fit", agent, ("planes", "probs", "z"), 3600)]
+    assert torch.load(MODEL_PATH, weights_only=True)["value_head.bias"].item() == 3.0
+
+
+def test_train_alphazero_trains_the_agent_it_returns(stand_ins):
+    from alphazero_amd.selfplay import train_alphazero
+    agent = train_alphazero(7.5, num_self_play_games=3, use_gpu=False, load_model=False)
+    assert stand_ins == [("play", agent, 3), ("fit", agent, ("planes", "probs", "z"), 7.5)]
+    assert (agent.num_simulations, agent.c_puct) == (800, 1.4)
