@@ -202,7 +202,7 @@ class AlphaZeroAgent(Agent):
             self.memory.append((s, p, 0 if winner_sign == 0 else (1 if winner_sign == who else -1)))
 
     def perform_training(self):
-        """An hour of training on 1000 games of this agent : it ends with the weights that it trained;
+        """An hour of training on 1000 games of this agent, which ends with the weights that it trained;
         they are saved to MODEL_PATH too."""
         from .selfplay import train_agent
         train_agent(self, time_limit=3600, num_self_play_games=1000)

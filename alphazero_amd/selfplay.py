@@ -125,6 +125,11 @@ def self_play(agent, num_games) -> List[tuple]:
     if agent.load_model_flag and not agent.model_loaded:
         agent.load_model()
     records, stats = play_games(agent, int(num_games))
+    return _remember(agent, records, stats)
+
+
+def _remember(agent, records, stats) -> List[tuple]:
+    """One sample per finished game, returned and appended to agent.memory (see self_play)."""
     memory = []
     for r in records:
         n = int(r["length"])
@@ -163,12 +168,18 @@ def self_play_sample_tensors(agent, num_games, first_game_id: int = 0):
     """self_play_samples without the host loop: the games are played and their per-ply samples built on the
     device (nnb_trajectory_samples); returns (planes [P,2,6,7], visit distributions [P,7], z [P]) as device
     tensors in the order self_play_samples lists them - what ConnectFourDataset (data_module.py:13-27) stacks."""
+    eng, traj, _ = _play_round(agent, num_games, first_game_id)
+    return eng.trajectory_samples(traj)
+
+
+def _play_round(agent, num_games, first_game_id: int = 0):
+    """(engine, trajectory bytes on the device, statistics) of one self-play round."""
     num_games = int(num_games)
     eng = agent.engine(min(max(num_games, 1), MAX_CONCURRENT_GAMES))
     params = eng.params(agent.num_simulations, agent.c_puct, evaluator=agent.evaluator, mode="compat",
                         eval_cache=getattr(agent, "eval_cache", False))
-    traj, _ = eng.selfplay_round(num_games, params, first_game_id=first_game_id)
-    return eng.trajectory_samples(traj)
+    traj, stats = eng.selfplay_round(num_games, params, first_game_id=first_game_id)
+    return eng, traj, stats
 
 
 def _check_trainable(agent):
@@ -228,8 +239,12 @@ def train_network(agent, planes: torch.Tensor, probs: torch.Tensor, z: torch.Ten
 
 
 def _play_for_training(agent, num_games):
-    """Self-play for one fit: the per-ply samples."""
-    return self_play_sample_tensors(agent, num_games)
+    """Self-play for one fit: returns the games' per-ply samples and appends one sample per game to agent.memory, as
+    self_play does (train_alpha_zero.py:33-55)."""
+    from .engine import trajectories_to_numpy
+    eng, traj, stats = _play_round(agent, num_games)
+    _remember(agent, trajectories_to_numpy(traj), dict(stats))
+    return eng.trajectory_samples(traj)
 
 
 def train_agent(agent, time_limit, num_self_play_games):

@@ -58,3 +58,39 @@ def test_train_alphazero_trains_the_agent_it_returns(stand_ins):
     agent = train_alphazero(7.5, num_self_play_games=3, use_gpu=False, load_model=False)
     assert stand_ins == [("play", agent, 3), ("fit", agent, ("planes", "probs", "z"), 7.5)]
     assert (agent.num_simulations, agent.c_puct) == (800, 1.4)
+
+
+class _Engine:
+    """Two finished games, as an engine returns them."""
+    def __init__(self):
+        import numpy as np
+        from alphazero_amd.engine import TRAJECTORY_DTYPE
+        self.records = np.zeros(2, dtype=TRAJECTORY_DTYPE)
+        for r, length, result in zip(self.records, (7, 8), (1, -1)):
+            r["length"], r["result"] = length, result
+            r["plies"]["player"][:length] = [1 + i % 2 for i in range(length)]
+        self.rounds = 0
+
+    def params(self, *args, **kwargs):
+        return None
+
+    def selfplay_round(self, n, params, **kwargs):
+        import numpy as np
+        self.rounds += 1
+        return torch.from_numpy(self.records.view(np.uint8).reshape(2, -1).copy()), {"games": 2, "plies": 15, "sims": 1}
+
+    def trajectory_samples(self, traj):
+        return traj, None, None
+
+
+def test_training_fills_the_agents_memory_as_self_play_does(monkeypatch):
+    from alphazero_amd import selfplay
+    from alphazero_amd.agent import AlphaZeroAgent, initialize_agent
+    engine, agent, other = _Engine(), initialize_agent(load_model=False), initialize_agent(load_model=False)
+    monkeypatch.setattr(AlphaZeroAgent, "engine", lambda self, *a, **k: engine)
+    traj, _, _ = selfplay._play_for_training(agent, 2)
+    assert engine.rounds == 1 and traj.shape[0] == 2                  # one set of games for both
+    selfplay.self_play(other, 2)
+    assert len(agent.memory) == 2 and [m[2] for m in agent.memory] == [m[2] for m in other.memory] == [1, -1]
+    for a, b in zip(agent.memory, other.memory):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
