@@ -249,8 +249,13 @@ def _play_for_training(agent, num_games):
 
 def train_agent(agent, time_limit, num_self_play_games):
     """Self-play with `agent`, then training on its per-ply samples for `time_limit` seconds, ten epochs at most, then the
-    network is saved to agent.MODEL_PATH."""
+    network is saved to agent.MODEL_PATH.  Of one process: where several share the work, distributed_play_games plays, and
+    train_network trains what is to be trained."""
+    import torch.distributed as dist
     from .agent import MODEL_PATH
+    if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+        raise RuntimeError(f"train_alphazero is the work of one process, here are {dist.get_world_size()}: each would play the "
+                           "same games, train alone and write the same file (see distributed_play_games, train_network)")
     _check_trainable(agent)
     planes, probs, z = _play_for_training(agent, num_self_play_games)
     train_network(agent, planes, probs, z, epochs=10, time_limit=time_limit)
