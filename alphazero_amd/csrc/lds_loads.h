@@ -18,7 +18,7 @@ template <typename T> __device__ __forceinline__ T *uniform(T *p) {
 __device__ __forceinline__ void load_to_lds(const void *base, uint32_t offset, void *to) {
     const uint32_t m0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)to;
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :: "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
+                 :: "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory", "m0");
 }
 
 // All but the wave's last IN_FLIGHT memory operations and all its LDS reads are done; after the barrier everybody's are.
