@@ -289,7 +289,7 @@ template <typename S> __host__ __device__ inline int upper_tiles(int mp) {
     return ortho_triangle(tiles_a_side<S>(mp));
 }
 
-template <typename T, int STAGE, typename S, bool ALL>
+template <typename T, int STAGE, typename S>
 __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams &p, const StageArgs &s, const OrthoGroup *items) {
     constexpr int TB = S::TB, RING = S::RING, kSub = S::kSub, kStride = kSub + 4, kUnits = S::kUnits, kGroup = S::WR * S::WC;
     constexpr bool symmetric = STAGE == STAGE_GRAM || STAGE == STAGE_POLY || STAGE == STAGE_MUL;
@@ -356,105 +356,115 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         // Every stage's sum from zero, smallest products first, added up by the vector pipe (see add_products).  On large
         // tiles a row of blocks at a time; the four blocks of small ones together, since a block's products wait for each
         // other, and added while the next stage multiplies (three 832 x 832 x 832: 17.0 us by rows, 16.1 so).
-        constexpr bool kAll = ALL, kFromZero = STAGE == STAGE_POLY || STAGE == STAGE_MUL || STAGE == STAGE_GRAM;
-        f32x4 sum[2][TB][TB] = {};
-        auto nothing = [](auto) {};
-        constexpr int kMemory = 4 * TB + kPerWave, kEvery = 3 * TB * TB / kMemory;      // reads and loads of a step
-        static_assert(kMemory * kEvery == 3 * TB * TB && (4 * TB) == 2 * kPerWave, "between the products, two reads and a load in turn");
-        auto multiply_with = [&](auto from, auto &&between) {    // between(n), n < kMemory, behind every kEvery products
-            constexpr int B = from;
-            if constexpr (TB == 2) {
-                f32x4 (&to)[TB][TB] = kFromZero ? sum[B] : acc;
-                if constexpr (kFromZero)
+        constexpr bool kFromZero = STAGE == STAGE_POLY || STAGE == STAGE_MUL || STAGE == STAGE_GRAM;
+        auto run = [&](auto with_lo) __attribute__((always_inline)) {
+            constexpr bool kAll = with_lo;                       // products of lo halves too (see add_products)
+            f32x4 sum[2][TB][TB] = {};
+            auto nothing = [](auto) {};
+            constexpr int kMemory = 4 * TB + kPerWave, kEvery = 3 * TB * TB / kMemory;      // reads and loads of a step
+            static_assert(kMemory * kEvery == 3 * TB * TB && (4 * TB) == 2 * kPerWave, "between the products, two reads and a load in turn");
+            auto multiply_with = [&](auto from, auto &&between) {    // between(n), n < kMemory, behind every kEvery products
+                constexpr int B = from;
+                if constexpr (TB == 2) {
+                    f32x4 (&to)[TB][TB] = kFromZero ? sum[B] : acc;
+                    if constexpr (kFromZero)
 #pragma unroll
-                    for (int i = 0; i < TB * TB; ++i) to[i / TB][i % TB] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if constexpr (kAll)
+                        for (int i = 0; i < TB * TB; ++i) to[i / TB][i % TB] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if constexpr (kAll)
 #pragma unroll
-                    for (int i = 0; i < TB * TB; ++i)
-                        to[i / TB][i % TB] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[B][i / TB], hl[B][i % TB], to[i / TB][i % TB], 0, 0, 0);
-                static_for<3 * TB * TB>([&](auto index) {
-                    constexpr int N = index, P = N / (TB * TB), I = N / TB % TB, J = N % TB;
-                    to[I][J] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P == 0 ? fl[B][I] : fh[B][I], P == 1 ? hl[B][J] : hh[B][J], to[I][J], 0, 0, 0);
-                    asm volatile("" : "+v"(to[I][J]));           // holds it between the reads and loads around it
-                    if constexpr (N % kEvery == kEvery - 1) between(std::integral_constant<int, N / kEvery>{});
-                });
-                if constexpr (kFromZero)
-#pragma unroll
-                    for (int i = 0; i < TB * TB; ++i) acc[i / TB][i % TB] += sum[1 - B][i / TB][i % TB];
-            } else {
-                static_for<TB>([&](auto row) {
-                    constexpr int I = row;
-                    f32x4 (&to)[TB] = kFromZero ? sum[0][I & 1] : acc[I];
-                    if constexpr (kFromZero) {
-#pragma unroll
-                        for (int j = 0; j < TB; ++j) to[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                        if constexpr (kAll)
-#pragma unroll
-                            for (int j = 0; j < TB; ++j) to[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[B][I], hl[B][j], to[j], 0, 0, 0);
-                    }
-                    static_for<3 * TB>([&](auto index) {
-                        constexpr int P = index / TB, J = index % TB, N = (I * 3 + P) * TB + J;
-                        to[J] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P == 0 ? fl[B][I] : fh[B][I], P == 1 ? hl[B][J] : hh[B][J], to[J], 0, 0, 0);
-                        asm volatile("" : "+v"(to[J]));
+                        for (int i = 0; i < TB * TB; ++i)
+                            to[i / TB][i % TB] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[B][i / TB], hl[B][i % TB], to[i / TB][i % TB], 0, 0, 0);
+                    static_for<3 * TB * TB>([&](auto index) {
+                        constexpr int N = index, P = N / (TB * TB), I = N / TB % TB, J = N % TB;
+                        to[I][J] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P == 0 ? fl[B][I] : fh[B][I], P == 1 ? hl[B][J] : hh[B][J], to[I][J], 0, 0, 0);
+                        asm volatile("" : "+v"(to[I][J]));           // holds it between the reads and loads around it
                         if constexpr (N % kEvery == kEvery - 1) between(std::integral_constant<int, N / kEvery>{});
                     });
-                    if constexpr (kFromZero && I > 0)
+                    if constexpr (kFromZero)
 #pragma unroll
-                        for (int j = 0; j < TB; ++j) acc[I - 1][j] += sum[0][(I - 1) & 1][j];
-                });
-                if constexpr (kFromZero)
+                        for (int i = 0; i < TB * TB; ++i) acc[i / TB][i % TB] += sum[1 - B][i / TB][i % TB];
+                } else {
+                    static_for<TB>([&](auto row) {
+                        constexpr int I = row;
+                        f32x4 (&to)[TB] = kFromZero ? sum[0][I & 1] : acc[I];
+                        if constexpr (kFromZero) {
 #pragma unroll
-                    for (int j = 0; j < TB; ++j) acc[TB - 1][j] += sum[0][(TB - 1) & 1][j];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        auto multiply = [&](auto from) { multiply_with(from, nothing); };
-        auto add_last = [&](auto from) {
-            constexpr int B = from;
-            if constexpr (TB == 2 && kFromZero)
+                            for (int j = 0; j < TB; ++j) to[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                            if constexpr (kAll)
 #pragma unroll
-                for (int i = 0; i < TB; ++i)
+                                for (int j = 0; j < TB; ++j) to[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[B][I], hl[B][j], to[j], 0, 0, 0);
+                        }
+                        static_for<3 * TB>([&](auto index) {
+                            constexpr int P = index / TB, J = index % TB, N = (I * 3 + P) * TB + J;
+                            to[J] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P == 0 ? fl[B][I] : fh[B][I], P == 1 ? hl[B][J] : hh[B][J], to[J], 0, 0, 0);
+                            asm volatile("" : "+v"(to[J]));
+                            if constexpr (N % kEvery == kEvery - 1) between(std::integral_constant<int, N / kEvery>{});
+                        });
+                        if constexpr (kFromZero && I > 0)
 #pragma unroll
-                    for (int j = 0; j < TB; ++j) acc[i][j] += sum[B][i][j];
-        };
-        constexpr int kInFlight = (RING - 2) * kPerWave;         // a wave's loads behind the stage it waits for
-        // behind the last stage the last again, never read: so many loads are in flight behind a stage throughout
-        auto at_most = [&](int t) { return t < stages ? t : stages - 1; };
-        constexpr std::integral_constant<int, 0> even{};
-        constexpr std::integral_constant<int, 1> odd{};
+                            for (int j = 0; j < TB; ++j) acc[I - 1][j] += sum[0][(I - 1) & 1][j];
+                    });
+                    if constexpr (kFromZero)
 #pragma unroll
-        for (int t = 0; t < RING - 1; ++t)
+                        for (int j = 0; j < TB; ++j) acc[TB - 1][j] += sum[0][(TB - 1) & 1][j];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            auto multiply = [&](auto from) { multiply_with(from, nothing); };
+            auto add_last = [&](auto from) {
+                constexpr int B = from;
+                if constexpr (TB == 2 && kFromZero)
 #pragma unroll
-            for (int d = 0; d < kPerWave; ++d) issue(at_most(t), t, d);
-        wait_and_meet<kInFlight>();
+                    for (int i = 0; i < TB; ++i)
 #pragma unroll
-        for (int d = 0; d < kPerWave; ++d) issue(at_most(RING - 1), RING - 1, d);
-        static_for<4 * TB>([&](auto r) { fragment(0, even, r); });
-        int slot = 0;
-        auto step = [&](int t, auto from, auto to) {             // multiplies stage t, reads stage t + 1
-            const int next = slot + 1 == RING ? 0 : slot + 1;
+                        for (int j = 0; j < TB; ++j) acc[i][j] += sum[B][i][j];
+            };
+            constexpr int kInFlight = (RING - 2) * kPerWave;         // a wave's loads behind the stage it waits for
+            // behind the last stage the last again, never read: so many loads are in flight behind a stage throughout
+            auto at_most = [&](int t) { return t < stages ? t : stages - 1; };
+            constexpr std::integral_constant<int, 0> even{};
+            constexpr std::integral_constant<int, 1> odd{};
+#pragma unroll
+            for (int t = 0; t < RING - 1; ++t)
+#pragma unroll
+                for (int d = 0; d < kPerWave; ++d) issue(at_most(t), t, d);
             wait_and_meet<kInFlight>();
-            const int ahead = at_most(t + RING);
-            multiply_with(from, [&](auto n) {
-                constexpr int N = n;
-                if constexpr (N % 3 == 2) issue(ahead, slot, N / 3);
-                else fragment(next, to, std::integral_constant<int, N - N / 3>{});
-            });
-            slot = next;
+#pragma unroll
+            for (int d = 0; d < kPerWave; ++d) issue(at_most(RING - 1), RING - 1, d);
+            static_for<4 * TB>([&](auto r) { fragment(0, even, r); });
+            int slot = 0;
+            auto step = [&](int t, auto from, auto to) {             // multiplies stage t, reads stage t + 1
+                const int next = slot + 1 == RING ? 0 : slot + 1;
+                wait_and_meet<kInFlight>();
+                const int ahead = at_most(t + RING);
+                multiply_with(from, [&](auto n) {
+                    constexpr int N = n;
+                    if constexpr (N % 3 == 2) issue(ahead, slot, N / 3);
+                    else fragment(next, to, std::integral_constant<int, N - N / 3>{});
+                });
+                slot = next;
+            };
+            // pairs of stages, for the two sets of registers; an odd last one by itself
+            int t = 0;
+            for (; t + 2 < stages; t += 2) {
+                step(t, even, odd);
+                step(t + 1, odd, even);
+            }
+            if (t + 1 < stages) {
+                step(t, even, odd);
+                multiply(odd);
+                add_last(odd);
+            } else {
+                multiply(even);
+                add_last(even);
+            }
         };
-        // pairs of stages, for the two sets of registers; an odd last one by itself
-        int t = 0;
-        for (; t + 2 < stages; t += 2) {
-            step(t, even, odd);
-            step(t + 1, odd, even);
-        }
-        if (t + 1 < stages) {
-            step(t, even, odd);
-            multiply(odd);
-            add_last(odd);
+        // The matrix chooses, not the launch: its precision does not depend on what else is in the call.
+        if constexpr (STAGE == STAGE_POLY || STAGE == STAGE_MUL) {
+            if (a.mp <= kOrthoLoRows) run(std::true_type{});
+            else run(std::false_type{});
         } else {
-            multiply(even);
-            add_last(even);
+            run(std::false_type{});
         }
     }
 
@@ -546,14 +556,13 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     }
 }
 
-// ALL: products of lo halves too (see add_products).
-template <int STAGE, typename S, bool ALL = false>
+template <int STAGE, typename S>
 __global__ __launch_bounds__(S::kThreads, 2) void ortho_product_kernel(OrthoShapes g, OrthoParams p, StageArgs s) {
-    product<float, STAGE, S, ALL>(g, p, s, nullptr);
+    product<float, STAGE, S>(g, p, s, nullptr);
 }
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads, 2) void ortho_finish_kernel(OrthoShapes g, OrthoParams p, StageArgs s, OrthoGroup items) {
-    product<T, STAGE_FINISH, S, false>(g, p, s, &items);
+    product<T, STAGE_FINISH, S>(g, p, s, &items);
 }
 
 // Adds up the parts of X X^T, one block of four waves per sub-tile (16 TB squared), and lays it out both ways round.
@@ -1072,7 +1081,6 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         else f(LoneTile{});
     };
     long long upper[2] = {}, full[2] = {};
-    int largest = 0;
     bool any64 = false, any128 = false, gram_of[2] = {}, reduce_of[2] = {};
     for (int i = 0; i < g.count; ++i) {
         const OrthoItem &it = g.item[i];
@@ -1084,7 +1092,6 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 upper[k] += (long long)it.batch * upper_tiles<S>(a.mp);
                 full[k] += (long long)it.batch * all_tiles<S>(a);
             });
-        largest = ortho_max(largest, a.mp);
         any64 |= a.mp == 64;
         any128 |= a.mp == 128;
         gram_of[a.sub == 64] = true;
@@ -1095,10 +1102,6 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     // 22.4 and 16.4.  Q X of 832 x 1536 three times, 252 large tiles: 27.7, 31.8 on small ones).
     auto pick = [](const long long (&n)[2]) { return n[0] >= 200 ? 0 : n[1] > 256 ? 1 : 2; };
     const int symmetric_tile = pick(upper), full_tile = pick(full);
-    // Where no square has more than 512 rows the products of lo halves are taken along: they cost little there (launches),
-    // and the plain float32 form is the more accurate the smaller the matrix (200 x 3000: 2.2e-6 of the result without, 2.0e-6
-    // with, plain 1.8e-6; 777 x 1501: 1.6e-6, 1.5e-6, plain 3.0e-6; three of them 304 us without, 332 with).
-    const bool all_products = largest <= 512;
     auto blocks = [&](auto &group, auto per_matrix) {
         int n = 0;
         for (int i = 0; i < g.count; ++i) {
@@ -1126,12 +1129,6 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         constexpr int STAGE = stage;
         with_tile(tile, [&](auto shape) {
             typedef decltype(shape) S;
-            if constexpr (STAGE == STAGE_POLY || STAGE == STAGE_MUL) {
-                if (all_products) {
-                    ortho_product_kernel<STAGE, S, true><<<grid, S::kThreads, 0, st>>>(shapes, p, s);
-                    return;
-                }
-            }
             ortho_product_kernel<STAGE, S><<<grid, S::kThreads, 0, st>>>(shapes, p, s);
         });
     };
