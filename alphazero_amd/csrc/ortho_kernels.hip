@@ -7,7 +7,9 @@
 // every kOrthoSegment = 3 steps: five steps (3 + 2) are as accurate as five plain ones (normal numbers, error over the
 // result's size against the plain float32 form's: 200 x 3000 2.0e-6 / 1.8e-6, 1024 x 11520 1.5e-6 / 5.1e-6, 128 x 2048
 // 5e-7 / 1.6e-6; one segment of five on a square matrix 1.6e-5 / 1.8e-6).
-// All m x m matrices are symmetric: half of their tiles are computed, the other half mirrored.
+// All m x m matrices are symmetric: where a product is a launch, half of their tiles are computed and the other half
+// mirrored.  Up to kOrthoSegmentRows rows their diagonals are held apart in float32 whichever kernel multiplies (beside
+// a large matrix 100 x 130 is off by 7e-7 of the result, as alone; with the diagonals among the halves 2.1e-6).
 //
 // Arithmetic: every operand is value * 2^k = hi + lo, two halves (22 bits), and a product is three matrix
 // instructions (hi lo + lo hi + hi hi) into float32.  The exponents k keep every entry below 2^15: the host bounds
@@ -164,7 +166,7 @@ __device__ __forceinline__ size_t unit_offset(int rb, int kb, int k) { return ((
 
 // The numbers of a wave's tile in LDS (S x S, rows of `stride` floats) as hi + lo units of a matrix with K columns, the
 // tile's first row being r0 and its first column c0: as they stand, or (TURNED) its transpose, whose first row is c0.
-// change(v, row, column, unit): last word on eight numbers of a row before they are rounded.
+// change(v, row, column, unit, its number): last word on eight numbers of a row before they are rounded.
 template <int S, bool TURNED, typename F>
 __device__ __forceinline__ void emit_units(const float *tile, int stride, unsigned char *dst, int r0, int c0, int k, F &&change) {
     const int lane = threadIdx.x & 63;
@@ -177,23 +179,27 @@ __device__ __forceinline__ void emit_units(const float *tile, int stride, unsign
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = TURNED ? tile[(c + e) * stride + r] : tile[r * stride + c + e];
         unsigned char *at = dst + unit_offset(r0 / 16 + rb, c0 / 32 + kb, k) + lane * 16;
-        change(v, r0 + r, c0 + c, at);
+        change(v, r0 + r, c0 + c, at, u);
         half8 lo;
         *reinterpret_cast<half8 *>(at) = pack_hi(v, lo);
         *reinterpret_cast<half8 *>(at + 1024) = lo;
     }
 }
-// Keeps the diagonal in float32 on the way.
+// Keeps the diagonal in float32 on the way; a square held apart (OrthoArea::apart) has zeros there in its units.
 struct KeepDiagonal {
     float *diag;
-    __device__ __forceinline__ void operator()(float (&v)[8], int r, int c, unsigned char *) const {
+    bool apart;
+    __device__ __forceinline__ void operator()(float (&v)[8], int r, int c, unsigned char *, int) const {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (r == c + e) diag[r] = v[e];
+            if (r == c + e) {
+                diag[r] = v[e];
+                if (apart) v[e] = 0.f;
+            }
     }
 };
 struct Unchanged {
-    __device__ __forceinline__ void operator()(float (&)[8], int, int, unsigned char *) const {}
+    __device__ __forceinline__ void operator()(float (&)[8], int, int, unsigned char *, int) const {}
 };
 
 // u / (|u| + eps) * 2^kx as units, X and its transpose, zero-padded.  One block per 64 x 64 tile.  Bound by memory:
@@ -258,6 +264,7 @@ __device__ __forceinline__ int sub_tile(int i, int j, int side) { return i * sid
 struct StageArgs {
     int f, g[2], out[2];         // squares: factors and result (MUL: up to two with the same first factor, by blockIdx.y;
                                  // POLY: A and P; GRAM: A; APPLY, FINISH: Q)
+    int whole[2];                // POLY, MUL: the result is the segment's last Q, which keeps its diagonal in the units
     int xt;                      // which transposed planes APPLY / FINISH read (APPLY writes the other one)
     float out_scale[2];          // 2^(k_out - k_f - k_g); FINISH: 2^(-k_f - k_g)
     float a, b, c;               // POLY: coefficients, times 2^(k_out), 2^(k_out - k_A), 2^(k_out - 2 k_A)
@@ -318,6 +325,38 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     const int which = STAGE == STAGE_MUL ? blockIdx.y : 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kg = wave / kGroup, in_group = wave % kGroup, wr = in_group / S::WC, wc = in_group % S::WC;
+    const int r0 = ti * S::kRows + wr * kSub, c0 = tj * S::kCols + wc * kSub;
+    // What the matrix unit does not see: POLY's lower terms, and where the diagonals are held apart the products with them,
+    // F G = O_F O_G + D_F O_G + O_F D_G + D_F D_G (POLY: both factors are A).  Small tiles read their part of the factors
+    // while they wait for the first operands (five matrices of up to 515 rows, one step: 155 us without, 132 so).
+    constexpr bool kRest = STAGE == STAGE_POLY || STAGE == STAGE_MUL, kAhead = kRest && TB == 2;
+    constexpr int kTileUnits = kSub / 16 * (kSub / 32);
+    struct Part { half8 f[2], g[2]; float df, dg[8]; };          // of a unit: hi and lo halves, diagonals
+    Part ahead[kAhead ? kTileUnits : 1];
+    const bool apart = kRest && a.apart;
+    const int f_square = s.f, g_square = STAGE == STAGE_MUL ? s.g[which] : s.f;
+    auto read_part = [&](Part &part, int r, int c, size_t at) {
+        auto units = [&](int square, half8 (&to)[2]) {
+            const unsigned char *from = area + a.sq(square) + at;
+            to[0] = *reinterpret_cast<const half8 *>(from), to[1] = *reinterpret_cast<const half8 *>(from + 1024);
+        };
+        if (STAGE == STAGE_POLY || apart) units(f_square, part.f);
+        if (!apart) return;
+        if (STAGE == STAGE_MUL) units(g_square, part.g);
+        part.df = reinterpret_cast<const float *>(area + a.diag_of(f_square))[r];
+        const f32x4 *dg = reinterpret_cast<const f32x4 *>(area + a.diag_of(g_square) + c * sizeof(float));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part.dg[e] = dg[e / 4][e % 4];
+    };
+    if constexpr (kAhead) {
+        if (kg == 0 && r0 <= c0 && c0 < a.mp)
+#pragma unroll
+            for (int u = 0; u < kTileUnits; ++u) {
+                const int rb = u / (kSub / 32), kb = u % (kSub / 32);
+                read_part(ahead[u], r0 + rb * 16 + (lane & 15), c0 + kb * 32 + (lane >> 4) * 8,
+                          unit_offset(r0 / 16 + rb, c0 / 32 + kb, a.mp) + lane * 16);
+            }
+    }
     f32x4 acc[TB][TB] = {};
     {
         const int kdim = STAGE == STAGE_GRAM ? a.np : a.mp, k_units = kdim / 32;
@@ -485,7 +524,6 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         __syncthreads();
         if (kg == 1) return;
     }
-    const int r0 = ti * S::kRows + wr * kSub, c0 = tj * S::kCols + wc * kSub;
     // behind the padding, or below the diagonal, where the mirror image of another sub-tile goes
     if (r0 >= a.mp || c0 >= (symmetric ? a.mp : a.np) || (symmetric && r0 > c0)) return;
     if (STAGE == STAGE_GRAM && a.splits > 1) {
@@ -504,23 +542,45 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
                 mine[(16 * i + 4 * (lane >> 4) + e) * kStride + 16 * j + (lane & 15)] = acc[i][j][e] * out_scale;
     if constexpr (symmetric) {
         unsigned char *dst = area + a.sq(s.out[which]);
-        if constexpr (STAGE == STAGE_POLY) {
-            const unsigned char *from = area + a.sq(s.f);
-            auto add_lower = [&](float (&v)[8], int r, int c, unsigned char *at) {
+        if constexpr (STAGE == STAGE_POLY || STAGE == STAGE_MUL) {
+            float *d_out = reinterpret_cast<float *>(area + a.diag_of(s.out[which]));
+            const bool whole = s.whole[which];
+            auto add_rest = [&](float (&v)[8], int r, int c, unsigned char *at, int u) {
                 float *keep = mine + (r - r0) * kStride + c - c0;         // for the mirror image
-                const half8 hi = *reinterpret_cast<const half8 *>(from + (at - dst)), lo = *reinterpret_cast<const half8 *>(from + (at - dst) + 1024);
+                Part part;
+                if constexpr (kAhead) part = ahead[u];
+                else read_part(part, r, c, at - dst);
+                float f[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) keep[e] = v[e] += s.b * ((float)hi[e] + (float)lo[e]) + (r == c + e ? s.a : 0.f);
+                for (int e = 0; e < 8; ++e) f[e] = (float)part.f[0][e] + (float)part.f[1][e];
+                if constexpr (STAGE == STAGE_POLY) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += s.b * f[e] + (r == c + e ? s.a : 0.f);
+                }
+                if (apart) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float g_e = STAGE == STAGE_MUL ? (float)part.g[0][e] + (float)part.g[1][e] : f[e];
+                        v[e] += out_scale * (part.df * g_e + f[e] * part.dg[e]);
+                        if (r == c + e) {
+                            v[e] += out_scale * (part.df * part.dg[e]) + (STAGE == STAGE_POLY ? s.b * part.df : 0.f);
+                            d_out[r] = v[e];
+                            if (!whole) v[e] = 0.f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) keep[e] = v[e];
             };
-            emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, add_lower);
-            if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
+            if (STAGE == STAGE_POLY || apart) emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, add_rest);
+            else emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
         } else {
-            if (STAGE == STAGE_GRAM && r0 == c0)
-                emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, KeepDiagonal{reinterpret_cast<float *>(area + a.diag)});
+            if (r0 == c0)
+                emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, KeepDiagonal{reinterpret_cast<float *>(area + a.diag_of(s.out[0])), a.apart});
             else
                 emit_units<kSub, false>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
-            if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
         }
+        if (r0 != c0) emit_units<kSub, true>(mine, kStride, dst, r0, c0, a.mp, Unchanged{});
     } else if constexpr (STAGE == STAGE_APPLY) {
         emit_units<kSub, false>(mine, kStride, area + a.x, r0, c0, a.np, Unchanged{});
         emit_units<kSub, true>(mine, kStride, area + a.xt(1 - s.xt), r0, c0, a.mp, Unchanged{});
@@ -596,7 +656,7 @@ __global__ __launch_bounds__(256) void ortho_reduce_kernel(OrthoShapes g, StageA
     __syncthreads();
     // a wave takes a quarter of the units, each way round
     unsigned char *dst = area + a.sq(s.out[0]);
-    const KeepDiagonal keep{reinterpret_cast<float *>(area + a.diag)};       // (off the diagonal nothing is kept)
+    const KeepDiagonal keep{reinterpret_cast<float *>(area + a.diag_of(s.out[0])), a.apart};       // (off the diagonal nothing is kept)
     constexpr int kQuarter = kSub / 2;
     const int qr = wave / 2 * kQuarter, qc = wave % 2 * kQuarter;
     if constexpr (kQuarter >= 32) {
@@ -899,7 +959,7 @@ __global__ __launch_bounds__(MP / 16 / B * (MP / 16 / B) * 64) void ortho_segmen
             }
         }
     };
-    const float *diag = reinterpret_cast<const float *>(ws + area.diag);
+    const float *diag = reinterpret_cast<const float *>(ws + area.diag_of(a_from));
 #pragma unroll
     for (int i = 0; i < B; ++i)
 #pragma unroll
@@ -1171,7 +1231,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 polynomial_bounds(c, rho * 1.001, p_max, lp_max, lpp_max);
                 // the first step's P is the segment's Q
                 const int kp = exponent_for(p_max), pout = i == 0 ? SQ_Q0 : SQ_P;
-                s.f = cur; s.out[0] = pout;
+                s.f = cur; s.out[0] = pout; s.whole[0] = len == 1;
                 s.a = (float)std::ldexp(c[0], kp); s.b = (float)std::ldexp(c[1], kp - ka); s.c = (float)std::ldexp(c[2], kp - 2 * ka);
                 all.step[i].a = s.a; all.step[i].b = s.b; all.step[i].c = s.c;
                 if (!segments) launch(std::integral_constant<int, STAGE_POLY>{}, symmetric_tile, n, s);
@@ -1181,14 +1241,14 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 s.f = pout;
                 const int kt = exponent_for(lp_max);
                 if (i + 1 < len) {
-                    s.g[pair] = cur; s.out[pair] = SQ_T;
+                    s.g[pair] = cur; s.out[pair] = SQ_T; s.whole[pair] = 0;
                     s.out_scale[pair++] = all.step[i].t_scale = (float)std::ldexp(1.0, kt - kp - ka);
                 }
                 if (i == 0) {
                     q = SQ_Q0; kq = kp;
                 } else {
                     const int kn = exponent_for(q_max), next = q == SQ_Q0 ? SQ_Q1 : SQ_Q0;
-                    s.g[pair] = q; s.out[pair] = next;
+                    s.g[pair] = q; s.out[pair] = next; s.whole[pair] = i + 1 == len;
                     s.out_scale[pair++] = all.step[i].q_scale = (float)std::ldexp(1.0, kn - kp - kq);
                     q = next; kq = kn;
                 }
@@ -1196,7 +1256,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                     launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile == 2 && n * pair > 256 ? 1 : symmetric_tile, dim3(n, pair), s);
                 if (i + 1 < len) {
                     const int kn = exponent_for(lpp_max), next = cur == SQ_A0 ? SQ_A1 : SQ_A0;
-                    s.f = SQ_T; s.g[0] = pout; s.out[0] = next;
+                    s.f = SQ_T; s.g[0] = pout; s.out[0] = next; s.whole[0] = 0;
                     s.out_scale[0] = all.step[i].a_scale = (float)std::ldexp(1.0, kn - kt - kp);
                     if (!segments) launch(std::integral_constant<int, STAGE_MUL>{}, symmetric_tile, dim3(n, 1), s);
                     cur = next; ka = kn;

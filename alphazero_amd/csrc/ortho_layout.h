@@ -9,6 +9,9 @@ constexpr int kOrthoPad = 64;            // matrices are padded with zeros to a 
 constexpr int kOrthoItems = 20;          // matrices (or equal batches of them) per group of launches
 constexpr int kOrthoMaxSteps = 16;
 constexpr int kOrthoSegment = 3;         // Newton-Schulz steps between two looks at the matrix itself
+// Matrices up to this side take all products of a segment in one launch, a block each, where all of a call are as small;
+// their squares' diagonals are held apart in float32, there and beside larger ones.
+constexpr int kOrthoSegmentRows = 128;
 // Squares of up to so many rows take the products of lo halves along: they cost little there (launches), and the plain
 // float32 form is the more accurate the smaller the matrix (200 x 3000: 2.2e-6 of the result without, 2.0e-6 with, plain
 // 1.8e-6; 777 x 1501: 1.6e-6, 1.5e-6, plain 3.0e-6; three of them 304 us without, 332 with).
@@ -61,10 +64,12 @@ struct OrthoArea {
     int sub_tiles;               // of those on and above the diagonal
     int splits;                  // parts that the long side is cut into for X X^T
     int parts_used;              // partial sums of squares
-    size_t parts, x, xt0, sq0, diag, partial, bytes;     // diag: float32 diagonal of X X^T
+    bool apart;                  // squares hold zeros on their diagonals, which lie beside them in float32
+    size_t parts, x, xt0, sq0, diag0, partial, bytes;
     size_t wide, square;         // bytes of an m x n and of an m x m matrix
     __host__ __device__ size_t xt(int i) const { return xt0 + i * wide; }
     __host__ __device__ size_t sq(int i) const { return sq0 + i * square; }
+    __host__ __device__ size_t diag_of(int i) const { return diag0 + i * mp * sizeof(float); }
 };
 enum OrthoSquare { SQ_A0 = 0, SQ_A1 = 1, SQ_T = 2, SQ_P = 3, SQ_Q0 = 4, SQ_Q1 = 5 };
 
@@ -87,6 +92,7 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols, int splits) 
     a.sub = a.mp > 256 ? 64 : 32;
     a.sub_tiles = ortho_triangle(a.mp / a.sub);
     a.splits = splits;
+    a.apart = a.mp <= kOrthoSegmentRows;
     const long long count = (long long)rows * cols;
     a.parts_used = (int)(count / 4096 < 1 ? 1 : count / 4096 < kOrthoNormParts ? count / 4096 : kOrthoNormParts);
     a.wide = (size_t)a.mp * a.np * 4;
@@ -96,7 +102,7 @@ __host__ __device__ inline OrthoArea ortho_area(int rows, int cols, int splits) 
     a.x = o; o += a.wide;
     a.xt0 = o; o += 2 * a.wide;
     a.sq0 = o; o += 6 * a.square;
-    a.diag = o; o += (size_t)a.mp * sizeof(float);
+    a.diag0 = o; o += 6 * a.mp * sizeof(float);
     a.partial = o;
     if (a.splits > 1) o += (size_t)a.splits * a.sub_tiles * a.sub * a.sub * sizeof(float);
     a.bytes = o;
@@ -118,8 +124,6 @@ struct OrthoSmallSteps {
 inline bool ortho_is_small(int rows, int cols) {
     return ortho_min(rows, cols) <= kOrthoSmallRows && ortho_max(rows, cols) <= kOrthoSmallCols;
 }
-// Matrices up to this side take all products of a segment in one launch, a block each.
-constexpr int kOrthoSegmentRows = 128;
 struct OrthoSegmentStep {
     float a, b, c;               // P = a I + b A + c A^2, times 2^(k_P), 2^(k_P - k_A), 2^(k_P - 2 k_A)
     float t_scale, a_scale;      // T = P A, A <- T P: 2^(k_out - k_f - k_g)

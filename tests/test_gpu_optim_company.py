@@ -31,3 +31,48 @@ def test_products_of_lo_halves_go_by_the_matrix_itself():
     alone, beside = _orthogonalized([small]), _orthogonalized([small, large])
     assert torch.equal(alone[0], beside[0])
     assert torch.equal(_orthogonalized([large])[0], beside[1])
+
+
+def _formula(x, steps=5, abc=(3.4445, -4.7750, 2.0315)):
+    """In x's own precision."""
+    tall = x.shape[0] > x.shape[1]
+    x = x.T.contiguous() if tall else x
+    x = x / (x.norm() + 1e-7)
+    for _ in range(steps):
+        g = x @ x.T.contiguous()
+        x = abc[0] * x + (abc[1] * g + abc[2] * (g @ g)) @ x
+    return x.T if tall else x
+
+
+def _matrix(kind, rows, cols, seed):
+    """Normal numbers; rows and columns of different sizes, as gradients have; singular values over three decades."""
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g)
+    if kind == "gradient":
+        x = x * torch.exp(0.5 * torch.randn(rows, 1, generator=g)) * torch.exp(0.5 * torch.randn(1, cols, generator=g)) * 1e-3
+    if kind == "decaying":
+        u, _, v = torch.linalg.svd(x.double(), full_matrices=False)
+        x = (u * 10.0 ** torch.linspace(0, -3, min(rows, cols), dtype=torch.float64) @ v).float()
+    return x.cuda()
+
+
+# up to 128 rows, beside matrices of more than 128, of more than 512, and the network's own convolutions
+LISTS = {"large": [(128, 2048), (7, 1024), (600, 900)], "middle": [(100, 130), (60, 1000), (515, 129), (300, 211)],
+         "many": [(65, 130), (128, 128), (200, 3000), (130, 140), (512, 512), (640, 700)]}
+
+
+@pytest.mark.parametrize("kind", ["normal", "gradient", "decaying"])
+@pytest.mark.parametrize("shapes", LISTS.values(), ids=LISTS)
+def test_precision_does_not_depend_on_the_other_matrices(shapes, kind):
+    """Each matrix of a list: at most three times the plain float32 form's error, and three times its own error alone.  What
+    rounds is the same in both cases, but for the terms with a diagonal, 24 bits of the other factor alone and 22 + 1 (a
+    sign) beside others, a factor of two; half as much again for sums in another order."""
+    torch = _torch()
+    xs = [_matrix(kind, r, c, i + 1) for i, (r, c) in enumerate(shapes)]
+    beside = _orthogonalized(xs)
+    for x, y in zip(xs, beside):
+        want = _formula(x.double())
+        error = lambda t: ((t.double() - want).norm() / want.norm()).item()
+        alone, plain = error(_orthogonalized([x])[0]), error(_formula(x))
+        assert error(y) <= 3 * plain and error(y) <= 3 * alone, (tuple(x.shape), error(y), alone, plain)
