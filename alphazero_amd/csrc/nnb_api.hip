@@ -3,6 +3,7 @@
 // allocated here: the engine lives in the caller's workspace.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <cstdarg>
@@ -879,37 +880,45 @@ int to_ortho_params(const nnb_newton_schulz *ns, OrthoParams &p) {
     return NNB_OK;
 }
 
-// Calls emit(group) for groups of at most kOrthoItems items whose areas take kOrthoGroupBytes (or one matrix's, if that
-// is more); a large batch is cut.  Returns the bytes of the largest group.
+// Calls emit(group) for groups of at most kOrthoItems items: first of the matrices that one block works on in LDS, up to
+// kOrthoSmallBatch of them, then of the others, whose areas take kOrthoGroupBytes together (or one matrix's, if that is
+// more); a large batch is cut.  So a matrix's way is its own, whatever else is in the call.  Returns the bytes of
+// workspace: the largest group's, and where there is a matrix at all no less than kAlign.
 constexpr size_t kOrthoGroupBytes = (size_t)1 << 30;
+constexpr size_t kOrthoSmallBatch = (size_t)1 << 20;         // blocks of 1024 threads: a launch has less than 2^32
 template <typename F> size_t ortho_groups(const OrthoItem *items, size_t count, F &&emit) {
     OrthoGroup g = {};
-    size_t used = 0, most = 0;
+    size_t used = 0, matrices = 0, most = 0;
     auto flush = [&] {
-        if (g.count) emit(g);
-        most = used > most ? used : most;
+        if (!g.count) return;
+        emit(g);
+        most = std::max(most, std::max(used, kAlign));
         g.count = 0;
-        used = 0;
+        used = matrices = 0;
     };
-    for (size_t i = 0; i < count; ++i) {
-        const size_t each = ortho_area(items[i].rows, items[i].cols).bytes;
-        for (int done = 0; done < items[i].batch;) {
-            if (g.count == kOrthoItems || (g.count && used + each > kOrthoGroupBytes)) flush();
-            const size_t room = (kOrthoGroupBytes - (used < kOrthoGroupBytes ? used : kOrthoGroupBytes)) / each;
-            OrthoItem &it = g.item[g.count++];
-            it = items[i];
-            const size_t left = (size_t)(items[i].batch - done);
-            it.batch = (int)(room < 1 ? 1 : room < left ? room : left);
-            const size_t size = dtype_bytes(it.type);
-            if (it.x) it.x = static_cast<const char *>(it.x) + done * it.x_bs * (long long)size;
-            if (it.out) it.out = static_cast<char *>(it.out) + done * it.o_bs * (long long)size;
-            it.ws = used;
-            it.ws_stride = each;
-            used += it.batch * each;
-            done += it.batch;
+    for (const bool small : {true, false}) {
+        for (size_t i = 0; i < count; ++i) {
+            if (ortho_is_small(items[i].rows, items[i].cols) != small) continue;
+            const size_t each = small ? 0 : ortho_area(items[i].rows, items[i].cols).bytes;
+            for (int done = 0; done < items[i].batch;) {
+                if (g.count == kOrthoItems || (g.count && used + each > kOrthoGroupBytes) || matrices == kOrthoSmallBatch) flush();
+                const size_t room = small ? kOrthoSmallBatch - matrices
+                                          : (kOrthoGroupBytes - std::min(used, kOrthoGroupBytes)) / each;
+                OrthoItem &it = g.item[g.count++];
+                it = items[i];
+                it.batch = (int)std::min(std::max(room, (size_t)1), (size_t)(items[i].batch - done));
+                const size_t size = dtype_bytes(it.type);
+                if (it.x) it.x = static_cast<const char *>(it.x) + done * it.x_bs * (long long)size;
+                if (it.out) it.out = static_cast<char *>(it.out) + done * it.o_bs * (long long)size;
+                it.ws = used;
+                it.ws_stride = each;
+                used += it.batch * each;
+                if (small) matrices += it.batch;
+                done += it.batch;
+            }
         }
+        flush();
     }
-    flush();
     return most;
 }
 

@@ -1123,15 +1123,12 @@ void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
 }  // namespace
 
 void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
-    bool small = true, segments = true;
-    for (int i = 0; i < g.count; ++i) {
-        small &= ortho_is_small(g.item[i].rows, g.item[i].cols);
-        segments &= ortho_min(g.item[i].rows, g.item[i].cols) <= kOrthoSegmentRows;
-    }
-    if (small) {
+    if (ortho_is_small(g.item[0].rows, g.item[0].cols)) {        // then all of the group are
         launch_small(st, g, p);
         return;
     }
+    bool segments = true;
+    for (int i = 0; i < g.count; ++i) segments &= ortho_min(g.item[i].rows, g.item[i].cols) <= kOrthoSegmentRows;
     OrthoShapes shapes = {};
     shapes.count = g.count;
     shapes.ws = g.ws;

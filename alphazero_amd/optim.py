@@ -106,6 +106,8 @@ def muon_update(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
         m' = momentum m + g;   u = g + momentum m' (nesterov) or m'
         w' = w (1 - lr weight_decay) - lr max(1, rows / cols)^(1/2) orthogonalize(u)
 
+    A matrix's precision goes by its own size; what else is in the call can only change the order of its sums.
+
     weights and grads of one type (float32, float16, bfloat16), momenta float32, all contiguous on one device, without
     elements in common.  Returns
     (weights, momenta): the given tensors, updated, or new ones with inplace=False."""

@@ -455,7 +455,8 @@ int nnb_orthogonalize(void *stream, int type, int64_t batch, int64_t rows, int64
  *     w' = w * (1 - lr * weight_decay) - lr * max(1, rows / cols)^(1/2) * orthogonalize(u)
  * weight, grad and weight_out of type `type`, momentum and momentum_out float32, all contiguous; weight_out may be
  * weight and momentum_out momentum, otherwise nothing may overlap.  `matrices` and `params` are host memory, read
- * before the call returns (a captured call keeps their values).  A matrix with rows or cols = 0 is skipped. */
+ * before the call returns (a captured call keeps their values).  A matrix with rows or cols = 0 is skipped.
+ * How precisely a matrix is treated goes by its own size; the others of a call can only change the order of its sums. */
 typedef struct nnb_muon_matrix {
     const void *weight, *grad;
     const float *momentum;

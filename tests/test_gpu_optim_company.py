@@ -76,3 +76,39 @@ def test_precision_does_not_depend_on_the_other_matrices(shapes, kind):
         error = lambda t: ((t.double() - want).norm() / want.norm()).item()
         alone, plain = error(_orthogonalized([x])[0]), error(_formula(x))
         assert error(y) <= 3 * plain and error(y) <= 3 * alone, (tuple(x.shape), error(y), alone, plain)
+
+
+@pytest.mark.parametrize("kind", ["normal", "gradient", "decaying"])
+@pytest.mark.parametrize("shapes", [[(33, 70), (128, 32), (128, 2048), (600, 900)], [(64, 64), (33, 33), (515, 129), (300, 211)],
+                                    [(33, 33)] * 3 + [(65, 130), (640, 700), (190, 60)]], ids=["large", "middle", "many"])
+def test_small_matrices_take_their_own_way(shapes, kind):
+    """Up to 64 x 192 alone a matrix is formed afresh for every step, and so it has to be beside others: the same bounds."""
+    test_precision_does_not_depend_on_the_other_matrices(shapes, kind)
+
+
+@pytest.mark.parametrize("rows,cols,batch", [(65, 66, 2000), (4, 5, 20000)])
+def test_large_batches(rows, cols, batch):
+    """2000 matrices of 65 x 66 need more workspace than one group of launches is given; many small ones need none."""
+    torch = _torch()
+    import ctypes
+    from alphazero_amd import _lib, optim
+    n = ctypes.c_size_t()
+    _lib.check(_lib.load().nnb_orthogonalize_workspace_bytes(batch, rows, cols, ctypes.byref(n)), "bytes")
+    one = ctypes.c_size_t()
+    _lib.check(_lib.load().nnb_orthogonalize_workspace_bytes(1, rows, cols, ctypes.byref(one)), "bytes")
+    assert n.value < batch * one.value
+    x = torch.randn(batch, rows, cols, generator=torch.Generator().manual_seed(rows)).cuda()
+    got = optim.orthogonalize(x).double()
+
+    def formula(x):
+        x = x / (x.norm(dim=(1, 2), keepdim=True) + 1e-7)
+        for _ in range(5):
+            g = x @ x.mT.contiguous()
+            x = 3.4445 * x + (-4.7750 * g + 2.0315 * (g @ g)) @ x
+        return x
+    want = formula(x.double())
+    error = lambda t: (t - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))
+    ours, plain = error(got), error(formula(x).double())
+    assert ours.pow(2).mean().sqrt() <= 3 * plain.pow(2).mean().sqrt()
+    # one matrix's error goes by its smallest singular values, by this bound of the worst (see test_gpu_optim.FAITHFUL)
+    assert ours.max() <= 2 * 2.0 ** -20 * 4.7750 * 3.4445 ** 3

@@ -120,3 +120,20 @@ def test_mx4_linear_refuses_more_features_than_a_grid_holds():
             a = _lib.Mx4LinearArgs(rows=rows, cols=32, out_features=features, x=4096, x_row_stride=32, x_col_stride=1,
                                    w_codes=4096, w_scales=4096, y=4096, y_row_stride=features)
             assert lib.nnb_mx4_linear(None, C.byref(a), C.c_void_p(4096), 1 << 30) == -1
+
+
+def test_matrices_in_one_blocks_lds_need_no_workspace_of_their_own():
+    import ctypes as C
+    from alphazero_amd import _lib
+    lib, n = _lib.load(), C.c_size_t()
+
+    def muon(*shapes):
+        items = (_lib.MuonMatrix * len(shapes))(*[_lib.MuonMatrix(rows=r, cols=c) for r, c in shapes])
+        assert lib.nnb_muon_workspace_bytes(len(shapes), items, C.byref(n)) == 0
+        return n.value
+    for batch, rows, cols in ((1, 1, 1), (1 << 20, 64, 64), ((1 << 31) - 1, 64, 192), (7, 192, 64)):
+        assert lib.nnb_orthogonalize_workspace_bytes(batch, rows, cols, C.byref(n)) == 0 and n.value == 256, (rows, cols)
+    assert muon((64, 64)) == muon(*[(3, 5)] * 100) == 256
+    assert muon() == muon((0, 5), (7, 0)) == 0
+    large = muon((200, 300))
+    assert large > 1 << 20 and muon((64, 64), (200, 300), (192, 64)) == large and muon((65, 193), (200, 300)) > large
