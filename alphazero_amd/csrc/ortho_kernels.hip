@@ -296,7 +296,11 @@ template <typename S> __host__ __device__ inline int upper_tiles(int mp) {
     return ortho_triangle(tiles_a_side<S>(mp));
 }
 
-template <typename T, int STAGE, typename S>
+// What the squares of a call have in common: more than kOrthoLoRows rows or fewer each, all over kOrthoSegmentRows; or
+// nothing, and every block looks at its own matrix.  (Looking costs 1024 x 11520 alone 1.4 %, three of 1501 x 777 2.4.)
+enum OrthoKind { KIND_LARGE, KIND_MIDDLE, KIND_MIXED };
+
+template <typename T, int STAGE, typename S, int KIND>
 __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams &p, const StageArgs &s, const OrthoGroup *items) {
     constexpr int TB = S::TB, RING = S::RING, kSub = S::kSub, kStride = kSub + 4, kUnits = S::kUnits, kGroup = S::WR * S::WC;
     constexpr bool symmetric = STAGE == STAGE_GRAM || STAGE == STAGE_POLY || STAGE == STAGE_MUL;
@@ -329,11 +333,11 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     // What the matrix unit does not see: POLY's lower terms, and where the diagonals are held apart the products with them,
     // F G = O_F O_G + D_F O_G + O_F D_G + D_F D_G (POLY: both factors are A).  Small tiles read their part of the factors
     // while they wait for the first operands (five matrices of up to 515 rows, one step: 155 us without, 132 so).
-    constexpr bool kRest = STAGE == STAGE_POLY || STAGE == STAGE_MUL, kAhead = kRest && TB == 2;
+    constexpr bool kRest = STAGE == STAGE_POLY || STAGE == STAGE_MUL, kAhead = kRest && TB == 2 && KIND == KIND_MIXED;
     constexpr int kTileUnits = kSub / 16 * (kSub / 32);
     struct Part { half8 f[2], g[2]; float df, dg[8]; };          // of a unit: hi and lo halves, diagonals
     Part ahead[kAhead ? kTileUnits : 1];
-    const bool apart = kRest && a.apart;
+    const bool apart = kRest && KIND == KIND_MIXED && a.apart;
     const int f_square = s.f, g_square = STAGE == STAGE_MUL ? s.g[which] : s.f;
     auto read_part = [&](Part &part, int r, int c, size_t at) {
         auto units = [&](int square, half8 (&to)[2]) {
@@ -500,7 +504,7 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
         };
         // The matrix chooses, not the launch: its precision does not depend on what else is in the call.
         if constexpr (STAGE == STAGE_POLY || STAGE == STAGE_MUL) {
-            if (a.mp <= kOrthoLoRows) run(std::true_type{});
+            if (KIND == KIND_MIDDLE || (KIND == KIND_MIXED && a.mp <= kOrthoLoRows)) run(std::true_type{});
             else run(std::false_type{});
         } else {
             run(std::false_type{});
@@ -616,13 +620,13 @@ __device__ __forceinline__ void product(const OrthoShapes &g, const OrthoParams 
     }
 }
 
-template <int STAGE, typename S>
+template <int STAGE, typename S, int KIND>
 __global__ __launch_bounds__(S::kThreads, 2) void ortho_product_kernel(OrthoShapes g, OrthoParams p, StageArgs s) {
-    product<float, STAGE, S>(g, p, s, nullptr);
+    product<float, STAGE, S, KIND>(g, p, s, nullptr);
 }
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads, 2) void ortho_finish_kernel(OrthoShapes g, OrthoParams p, StageArgs s, OrthoGroup items) {
-    product<T, STAGE_FINISH, S>(g, p, s, &items);
+    product<T, STAGE_FINISH, S, KIND_MIXED>(g, p, s, &items);
 }
 
 // Adds up the parts of X X^T, one block of four waves per sub-tile (16 TB squared), and lays it out both ways round.
@@ -1138,6 +1142,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         else f(LoneTile{});
     };
     long long upper[2] = {}, full[2] = {};
+    int smallest = INT32_MAX, largest = 0;
     bool any64 = false, any128 = false, gram_of[2] = {}, reduce_of[2] = {};
     for (int i = 0; i < g.count; ++i) {
         const OrthoItem &it = g.item[i];
@@ -1149,6 +1154,8 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
                 upper[k] += (long long)it.batch * upper_tiles<S>(a.mp);
                 full[k] += (long long)it.batch * all_tiles<S>(a);
             });
+        smallest = ortho_min(smallest, a.mp);
+        largest = ortho_max(largest, a.mp);
         any64 |= a.mp == 64;
         any128 |= a.mp == 128;
         gram_of[a.sub == 64] = true;
@@ -1158,6 +1165,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     // (one product of squares: 1024, 136 small tiles, 13.9 us with two groups, 17.1 without; 832 three times, 273 tiles,
     // 22.4 and 16.4.  Q X of 832 x 1536 three times, 252 large tiles: 27.7, 31.8 on small ones).
     auto pick = [](const long long (&n)[2]) { return n[0] >= 200 ? 0 : n[1] > 256 ? 1 : 2; };
+    const int kind = smallest > kOrthoLoRows ? KIND_LARGE : smallest > kOrthoSegmentRows && largest <= kOrthoLoRows ? KIND_MIDDLE : KIND_MIXED;
     const int symmetric_tile = pick(upper), full_tile = pick(full);
     auto blocks = [&](auto &group, auto per_matrix) {
         int n = 0;
@@ -1186,7 +1194,14 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         constexpr int STAGE = stage;
         with_tile(tile, [&](auto shape) {
             typedef decltype(shape) S;
-            ortho_product_kernel<STAGE, S><<<grid, S::kThreads, 0, st>>>(shapes, p, s);
+            auto of_kind = [&](auto k) { ortho_product_kernel<STAGE, S, k><<<grid, S::kThreads, 0, st>>>(shapes, p, s); };
+            if constexpr (STAGE == STAGE_POLY || STAGE == STAGE_MUL) {
+                if (kind == KIND_LARGE) of_kind(std::integral_constant<int, KIND_LARGE>{});
+                else if (kind == KIND_MIDDLE) of_kind(std::integral_constant<int, KIND_MIDDLE>{});
+                else of_kind(std::integral_constant<int, KIND_MIXED>{});
+            } else {
+                of_kind(std::integral_constant<int, KIND_MIXED>{});
+            }
         });
     };
     auto gram = [&](const StageArgs &s) {
