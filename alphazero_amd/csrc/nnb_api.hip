@@ -880,30 +880,31 @@ int to_ortho_params(const nnb_newton_schulz *ns, OrthoParams &p) {
     return NNB_OK;
 }
 
-// Calls emit(group) for groups of at most kOrthoItems items: first of the matrices that one block works on in LDS, up to
-// kOrthoSmallBatch of them, then of the others, whose areas take kOrthoGroupBytes together (or one matrix's, if that is
-// more); a large batch is cut.  So a matrix's way is its own, whatever else is in the call.  Returns the bytes of
-// workspace: the largest group's, and where there is a matrix at all no less than kAlign.
+// Calls emit(group) for groups of at most kOrthoItems items whose areas take kOrthoGroupBytes together (or one matrix's, if
+// that is more); a large batch is cut.  Matrices that one block works on in LDS have no area; they take what room the last
+// of the other groups has, first in it, and groups of their own.  Returns the bytes of workspace: the largest group's, and
+// where there is a matrix at all no less than kAlign.
 constexpr size_t kOrthoGroupBytes = (size_t)1 << 30;
 constexpr size_t kOrthoSmallBatch = (size_t)1 << 20;         // blocks of 1024 threads: a launch has less than 2^32
 template <typename F> size_t ortho_groups(const OrthoItem *items, size_t count, F &&emit) {
     OrthoGroup g = {};
-    size_t used = 0, matrices = 0, most = 0;
+    size_t used = 0, smalls = 0, most = 0;                   // of the present group: bytes, small matrices
+    auto is_small = [](const OrthoItem &it) { return ortho_is_small(it.rows, it.cols); };
     auto flush = [&] {
         if (!g.count) return;
+        std::stable_partition(g.item, g.item + g.count, is_small);
         emit(g);
         most = std::max(most, std::max(used, kAlign));
         g.count = 0;
-        used = matrices = 0;
+        used = smalls = 0;
     };
-    for (const bool small : {true, false}) {
+    for (const bool small : {false, true})
         for (size_t i = 0; i < count; ++i) {
-            if (ortho_is_small(items[i].rows, items[i].cols) != small) continue;
+            if (is_small(items[i]) != small) continue;
             const size_t each = small ? 0 : ortho_area(items[i].rows, items[i].cols).bytes;
             for (int done = 0; done < items[i].batch;) {
-                if (g.count == kOrthoItems || (g.count && used + each > kOrthoGroupBytes) || matrices == kOrthoSmallBatch) flush();
-                const size_t room = small ? kOrthoSmallBatch - matrices
-                                          : (kOrthoGroupBytes - std::min(used, kOrthoGroupBytes)) / each;
+                if (g.count == kOrthoItems || (used && used + each > kOrthoGroupBytes) || smalls == kOrthoSmallBatch) flush();
+                const size_t room = small ? kOrthoSmallBatch - smalls : (kOrthoGroupBytes - std::min(used, kOrthoGroupBytes)) / each;
                 OrthoItem &it = g.item[g.count++];
                 it = items[i];
                 it.batch = (int)std::min(std::max(room, (size_t)1), (size_t)(items[i].batch - done));
@@ -913,12 +914,11 @@ template <typename F> size_t ortho_groups(const OrthoItem *items, size_t count, 
                 it.ws = used;
                 it.ws_stride = each;
                 used += it.batch * each;
-                if (small) matrices += it.batch;
+                if (small) smalls += it.batch;
                 done += it.batch;
             }
         }
-        flush();
-    }
+    flush();
     return most;
 }
 

@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "kernels.h"
@@ -76,12 +77,12 @@ __device__ __forceinline__ void load_row(const T *row, long long cs, int c, int 
 // Sum of squares of u, in double (a gradient's squares leave float32's range long before the gradient does), as partial
 // sums that the next kernel adds in a fixed order; the optimiser step's new momentum is written on the way.  Bound by
 // memory: 1024 x 11520 in float32 12.5 us (3.8 TB/s), 27.5 with the momentum (5.2 TB/s).
+// The part `local` of a matrix, by 256 threads; all of the block meet here, those behind the last part too.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroup g, OrthoParams p) {
+__device__ __forceinline__ void norm_part(const OrthoGroup &g, const OrthoParams &p, const OrthoItem &it, int local, int tid, double *wave_sum) {
     constexpr int N = 16 / sizeof(T);
-    int local;
-    const OrthoItem &it = g.item[find_item(g, blockIdx.x, local)];
     const OrthoArea a = ortho_area(it.rows, it.cols, 1);
+    const bool live = local < it.batch * a.parts_used;
     const int b = it.batch == 1 ? 0 : local / a.parts_used, part = local - b * a.parts_used;
     // a matrix without gaps is one long row
     const bool flat = it.x_cs == 1 && (it.x_rs == it.cols || it.rows == 1);
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroup g, OrthoPara
     const unsigned total = (unsigned)rows * (unsigned)per_row;
     const T *x = static_cast<const T *>(it.x) + b * it.x_bs;
     double sum = 0.0;
-    for (unsigned i = part * 256 + threadIdx.x; i < total; i += a.parts_used * 256) {
+    for (unsigned i = part * 256 + tid; live && i < total; i += a.parts_used * 256) {
         const unsigned r = flat ? 0 : i / per_row;
         const int c = (int)(i - r * per_row) * N;
         float v[N];
@@ -116,14 +117,20 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroup g, OrthoPara
 #pragma unroll
         for (int e = 0; e < N; ++e) sum += (double)v[e] * (double)v[e];
     }
-    __shared__ double wave_sum[4];
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = sum;
+    if ((tid & 63) == 0) wave_sum[tid >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0)
+    if (tid == 0 && live)
         reinterpret_cast<double *>(g.ws + it.ws + b * it.ws_stride + a.parts)[part] =
             (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroup g, OrthoParams p) {
+    __shared__ double wave_sum[4];
+    int local;
+    const OrthoItem &it = g.item[find_item(g, blockIdx.x, local)];
+    norm_part<T>(g, p, it, local, threadIdx.x, wave_sum);
 }
 
 __device__ __forceinline__ half8 pack_hi(const float (&v)[8], half8 &lo) {
@@ -740,6 +747,8 @@ __device__ __forceinline__ void multiply_units(const unsigned char *f, const uns
 // So a wave has one block of 16 of a square, its parts of A and X stay in float32 registers, blocks of padding are left
 // out, and X Y's tiles come out of the matrix unit both ways round, for the two orders of units they are stored in
 // (128 x 32, five steps: 28.0 us with two blocks to a wave, values read back from LDS and halves scattered, now 21.5).
+// Beside larger matrices their norms are taken in the same launch, four parts to a block (the step of the network with
+// two launches 536 us, so 516).
 template <typename T, int NP>
 __global__ __launch_bounds__(1024) void ortho_small_kernel(OrthoGroup g, OrthoParams p, OrthoSmallSteps steps) {
     constexpr int M = kOrthoSmallRows, kWide = M * NP * 4, kSquare = M * M * 4, TN = NP / 64;
@@ -748,6 +757,10 @@ __global__ __launch_bounds__(1024) void ortho_small_kernel(OrthoGroup g, OrthoPa
     float *diag_a = reinterpret_cast<float *>(sq_b + kSquare), *diag_b = diag_a + M;
     int batch;
     const OrthoItem &it = g.item[find_item(g, blockIdx.x, batch)];
+    if (!ortho_is_small(it.rows, it.cols)) {
+        norm_part<T>(g, p, it, batch * 4 + threadIdx.x / 256, threadIdx.x % 256, reinterpret_cast<double *>(lds) + threadIdx.x / 256 * 4);
+        return;
+    }
     const bool tall = it.rows > it.cols;
     const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1088,6 +1101,7 @@ template <typename S> int all_tiles(const OrthoArea &a) {
     return (a.mp + S::kRows - 1) / S::kRows * ((a.np + S::kCols - 1) / S::kCols);
 }
 
+// The small matrices of the group, and the others' norms.
 void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     OrthoSmallSteps steps = {};
     double rho = 1.0;
@@ -1110,9 +1124,14 @@ void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
         rho = std::fmax(lpp_max, 1e-6);
     }
     for (int i = 0; i < g.count; ++i) {
+        const OrthoItem &it = g.item[i];
         g.first[i] = blocks;
-        blocks += g.item[i].batch;
-        widest = ortho_max(widest, ortho_max(g.item[i].rows, g.item[i].cols));
+        if (ortho_is_small(it.rows, it.cols)) {
+            blocks += it.batch;
+            widest = ortho_max(widest, ortho_max(it.rows, it.cols));
+        } else {
+            blocks += (it.batch * ortho_area(it.rows, it.cols, 1).parts_used + 3) / 4;
+        }
     }
     for (int i = g.count; i < kOrthoItems; ++i) g.first[i] = INT32_MAX;
     g.blocks = blocks;
@@ -1127,9 +1146,13 @@ void launch_small(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
 }  // namespace
 
 void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
-    if (ortho_is_small(g.item[0].rows, g.item[0].cols)) {        // then all of the group are
+    int smalls = 0;                                              // they come first
+    while (smalls < g.count && ortho_is_small(g.item[smalls].rows, g.item[smalls].cols)) ++smalls;
+    if (smalls) {
         launch_small(st, g, p);
-        return;
+        if (smalls == g.count) return;
+        std::copy(g.item + smalls, g.item + g.count, g.item);
+        g.count -= smalls;
     }
     bool segments = true;
     for (int i = 0; i < g.count; ++i) segments &= ortho_min(g.item[i].rows, g.item[i].cols) <= kOrthoSegmentRows;
@@ -1220,7 +1243,7 @@ void launch_orthogonalize(hipStream_t st, OrthoGroup &g, const OrthoParams &p) {
     with_dtype(p.type, [&](auto type) {
         typedef decltype(type) T;
         int n = blocks(g, [](const OrthoArea &a) { return a.parts_used; });
-        ortho_norm_kernel<T><<<n, 256, 0, st>>>(g, p);
+        if (!smalls) ortho_norm_kernel<T><<<n, 256, 0, st>>>(g, p);
         double rho = 1.0;                       // bound of A's largest eigenvalue
         int kx = exponent_for(1.0), xt = 0;
         n = blocks(g, [](const OrthoArea &a) { return a.mp / 64 * (a.np / 64); });

@@ -121,7 +121,7 @@ struct OrthoSmallSteps {
     float pow_kx;                // 2^(k_X) at the start
     OrthoSmallStep step[kOrthoMaxSteps];
 };
-inline bool ortho_is_small(int rows, int cols) {
+__host__ __device__ inline bool ortho_is_small(int rows, int cols) {
     return ortho_min(rows, cols) <= kOrthoSmallRows && ortho_max(rows, cols) <= kOrthoSmallCols;
 }
 struct OrthoSegmentStep {
