@@ -103,6 +103,7 @@ SIGNATURES = {
     "nnb_mx4_quantize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, _P]),
     "nnb_mx4_dequantize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, _P, _P]),
     "nnb_mx4_linear_workspace_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_size_t)]),
+    "nnb_debug_mx4_form": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
     "nnb_mx4_linear": (C.c_int, [_P, C.POINTER(Mx4LinearArgs), _P, C.c_size_t]),
     "nnb_orthogonalize_workspace_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
     "nnb_orthogonalize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_int64, _P, C.POINTER(C.c_int64), _P,

@@ -191,7 +191,11 @@ void launch_mx4_quantize(hipStream_t st, int type, long long rows, int cols, con
                          long long col_stride, const int32_t *row_count, uint8_t *codes, uint8_t *scales);
 void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, const uint8_t *codes, const uint8_t *scales,
                            void *out);
-// Few rows are quantised inside the product's own launch: then launch_mx4_linear takes them as `x`, not as codes.
+// The kernel that multiplies codes; f32, wide: the result's type, and whether its rows take 16-byte stores.
+enum Mx4Form { MX4_ROWS, MX4_ONE_PER_CU, MX4_TWO_PER_CU, MX4_LARGE };
+Mx4Form mx4_form(long long rows, int n, int kp, bool f32, bool wide, long long order_rows);
+// Few rows are quantised inside the product's own launch: then launch_mx4_linear takes them as `x`, not as codes.  With
+// order_rows the results are wide rows of float32.
 bool mx4_linear_fuses(long long rows, int cols, int n = 0, long long order_rows = 0);
 void launch_mx4_linear(hipStream_t st, Mx4Linear a, const Mx4Rows *x);
 

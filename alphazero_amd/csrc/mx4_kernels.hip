@@ -14,6 +14,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "kernels.h"
 #include "lds_loads.h"
 #include "mfma_tiles.h"
@@ -555,62 +558,96 @@ void launch_mx4_dequantize(hipStream_t st, int type, long long rows, int cols, c
 
 namespace {
 
-// Which kernel multiplies: the cheapest by these costs in microseconds (256 CUs; measured at rows 1 .. 2048 of 1024 x 11520,
-// 4096 x 4096, 8192 x 1024, 512 x 512 and 300 x 16384 layers and at 8192^3, within 20 %):
-//   rows kernel     3 + (1.2 + K / 2300) per 256 blocks of (64 rows x 16 features)
-//   128 x 128, one block of eight waves per CU (a ring of four stages)   3.5 + 0.6 per stage of 256 elements and 256 tiles
-//   128 x 128, two blocks of four waves per CU (two stages each)         3.5 + 0.9 per stage and 512 tiles
-//   256 x 256       8 + 1.65 per stage and 256 tiles (8192^3; less since its loads are spread)
-// For example 1024 rows of 11520 -> 1024: 26 / 31 / 35 / 86 us in this order, 2048 rows of 1024 -> 8192: 95 / 30 / 23 / 25.
+// Which kernel multiplies: the cheapest by a model of the time in microseconds, fitted to 178 sizes of 17 to 8192 rows, 64 to
+// 8192 features and 100 to 16384 columns, 70 of them random, each run in all four forms with a float32 or bfloat16 result
+// (profiles/mx4_forms.txt).  The model is off by 8 % of the rows kernel's time in the mean, 4 of the small tiles' and 6 of the
+// large ones', by 37 at worst; what it picks takes 0.5 % more than the fastest form in the mean, and 11 at most but for one
+// size of 30.  Measured, rows / one / two / large:
+//       64 rows of 8192 -> 8192   12.6 / 18.8 / 24.1 / 45.9   rows        64 rows of 1024 -> 8192    5.2 /  6.1 /  7.1 / 13.5   rows
+//      256 rows of 8192 -> 8192   42.4 / 20.1 / 25.6 / 49.2   one       2048 rows of 1024 -> 8192   93.5 / 27.3 / 21.8 / 22.5   two
+//     2048 rows of 8192 -> 8192    -   / 95.8 / 82.5 / 69.5   large     4096 rows of 4096 -> 4096    157 / 51.7 / 46.9 / 42.7   large
 // The rows kernel and the tiles add a row's products in different orders, but all forms of each in one: with `order_rows`
 // the choice between the two goes by that count, so that a row's results do not depend on how many come with it.
-struct ProductCosts {
-    double rows, one, two, large;
-    bool rows_form;
-};
 
-ProductCosts product_costs(long long rows, int n, int kp) {
-    auto rounds = [&](int r, int f, int at_once) {
-        const long long blocks = (rows + r - 1) / r * ((n + f - 1) / f);
-        return (double)((blocks + at_once - 1) / at_once);
-    };
-    const double stages = kp / 256;
-    ProductCosts c;
-    c.rows = 3.0 + rounds(64, 16, 256) * (1.2 + kp / 2300.0);
-    c.one = 3.5 + rounds(128, 128, 256) * stages * 0.6;
-    c.two = 3.5 + rounds(128, 128, 512) * stages * 0.9;
-    c.large = 8.0 + rounds(256, 256, 256) * stages * 1.65;
-    c.rows_form = rows <= 16 || (c.rows <= c.one && c.rows <= c.two && c.rows <= c.large);
-    return c;
+// As few rows per block (16, 32, 64) as still leave at most a block per CU (128 rows of 11520 -> 1024: 7.2 / 6.2 / 7.6 us with
+// 16 / 32 / 64 rows, 64 rows 4.8 / 5.6 / 7.3).
+int rows_per_block(long long rows, int n) {
+    const long long feature_tiles = (n + 15) / 16;
+    if (rows <= 16 || (rows + 15) / 16 * feature_tiles <= 256) return 16;
+    return rows <= 32 || (rows + 31) / 32 * feature_tiles <= 256 ? 32 : 64;
+}
+
+// Blocks of 64 rows x 16 features, each CU's in turn, the columns' part of a short row hidden behind the latency of its reads;
+// or the rows' way from memory to the eight XCDs, where few features leave every XCD almost all of them to read.
+double rows_cost(long long rows, int n, int kp) {
+    const int per_block = rows_per_block(rows, n), feature_tiles = (n + 15) / 16;
+    const double blocks = (double)((rows + per_block - 1) / per_block) * feature_tiles;
+    const double compute = std::max(1.0, blocks / 256) * (per_block / 64.0) * std::max(1.35, kp / 1660.0);
+    return 2.4 + std::max(compute, (double)rows * kp / 2 * std::min(8, feature_tiles) / 4.6e6);
+}
+
+// A tile form: `at_once` tiles of `side` squared work together, which takes a time per stage of 256 elements and one for
+// the results, both the longer the more of the tiles there are (a crowd shares memory and power; two blocks a CU, its pipes).
+struct TileCost {
+    int side, at_once, crowd;                // crowd: 1 linear, 2 quadratic in the share of tiles that are there
+    double start, stage, crowded_stage, end, store, f32_store, narrow, narrow_store;
+};
+constexpr TileCost kOnePerCu = {128, 256, 1, 2.4, 0.43, 0.14, 1.8, 2.0, 0.45, 1.7, 2.3};     // eight waves, ring of four stages
+constexpr TileCost kTwoPerCu = {128, 512, 2, 3.9, 0.56, 0.50, 1.0, 3.6, 0.50, 0.8, 7.0};     // four waves, two stages each
+constexpr TileCost kLarge = {256, 256, 1, 5.4, 1.10, 0.50, 6.4, 4.4, 0.80, 5.2, 2.8};
+
+double tile_cost(const TileCost &c, long long rows, int n, int kp, bool f32, bool wide) {
+    const double tiles = (double)((rows + c.side - 1) / c.side) * ((n + c.side - 1) / c.side);
+    const double rounds = std::ceil(tiles / c.at_once), share = tiles / (rounds * c.at_once);
+    const double stages = kp / 256 * (c.stage + c.crowded_stage * (c.crowd == 2 ? share * share : share));
+    const double stores = c.end + c.store * share * (f32 ? 1.0 + c.f32_store : 1.0) + (wide ? 0.0 : c.narrow + c.narrow_store * share);
+    return c.start + rounds * (stages + stores);
+}
+
+Mx4Form cheapest_tiles(long long rows, int n, int kp, bool f32, bool wide, double &cost) {
+    const double one = tile_cost(kOnePerCu, rows, n, kp, f32, wide), two = tile_cost(kTwoPerCu, rows, n, kp, f32, wide),
+                 large = tile_cost(kLarge, rows, n, kp, f32, wide);
+    cost = std::min(one, std::min(two, large));
+    return cost == one ? MX4_ONE_PER_CU : cost == two ? MX4_TWO_PER_CU : MX4_LARGE;
+}
+
+bool rows_form(long long rows, int n, int kp, bool f32, bool wide) {
+    double tiles;
+    cheapest_tiles(rows, n, kp, f32, wide, tiles);
+    return rows <= 16 || rows_cost(rows, n, kp) <= tiles;
 }
 
 template <typename T> void launch_product(hipStream_t st, const Mx4Linear &a) {
     auto tiles = [&](int r, int f) { return (a.rows + r - 1) / r * ((a.n + f - 1) / f); };
-    const ProductCosts cost = product_costs(a.rows, a.n, a.kp);
-    if (a.order_rows > 0 ? product_costs(a.order_rows, a.n, a.kp).rows_form : cost.rows_form) {
-        auto rows_form = [&](auto rt) {
+    switch (mx4_form(a.rows, a.n, a.kp, sizeof(T) == 4, a.wide, a.order_rows)) {
+    case MX4_ROWS: {
+        auto of_rows = [&](auto rt) {
             constexpr int RT = rt;
             mx4_rows_kernel<T, RT, float, false><<<(unsigned)tiles(RT * 16, 16), kRowsWaves * 64, 0, st>>>(a, nullptr, 0, 0, 0);
         };
-        // as few rows per block as still leave at most a block per CU (128 rows of 11520 -> 1024: 7.2 / 6.2 / 7.6 us with
-        // 16 / 32 / 64 rows, 64 rows 4.8 / 5.6 / 7.3)
-        if (a.rows <= 16 || tiles(16, 16) <= 256) rows_form(std::integral_constant<int, 1>{});
-        else if (a.rows <= 32 || tiles(32, 16) <= 256) rows_form(std::integral_constant<int, 2>{});
-        else rows_form(std::integral_constant<int, 4>{});
-    } else if (cost.large <= cost.one && cost.large <= cost.two) {
-        mx4_tile_kernel<T, 2, 2, 4, 4, 2, 1><<<(unsigned)tiles(256, 256), 256, 0, st>>>(a);
-    } else if (cost.two < cost.one) {
-        mx4_tile_kernel<T, 2, 2, 2, 2, 2, 2><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a);
-    } else {
-        mx4_tile_kernel<T, 4, 2, 1, 2, 4, 3><<<(unsigned)tiles(128, 128), 512, 0, st>>>(a);
+        const int per_block = rows_per_block(a.rows, a.n);
+        if (per_block == 16) of_rows(std::integral_constant<int, 1>{});
+        else if (per_block == 32) of_rows(std::integral_constant<int, 2>{});
+        else of_rows(std::integral_constant<int, 4>{});
+        break;
+    }
+    case MX4_LARGE: mx4_tile_kernel<T, 2, 2, 4, 4, 2, 1><<<(unsigned)tiles(256, 256), 256, 0, st>>>(a); break;
+    case MX4_TWO_PER_CU: mx4_tile_kernel<T, 2, 2, 2, 2, 2, 2><<<(unsigned)tiles(128, 128), 256, 0, st>>>(a); break;
+    case MX4_ONE_PER_CU: mx4_tile_kernel<T, 4, 2, 1, 2, 4, 3><<<(unsigned)tiles(128, 128), 512, 0, st>>>(a); break;
     }
 }
 
 }  // namespace
 
+Mx4Form mx4_form(long long rows, int n, int kp, bool f32, bool wide, long long order_rows) {
+    double cost;
+    const bool by_rows = order_rows > 0 ? rows_form(order_rows, n, kp, f32, wide) : rows_form(rows, n, kp, f32, wide);
+    return by_rows ? MX4_ROWS : cheapest_tiles(rows, n, kp, f32, wide, cost);
+}
+
 bool mx4_linear_fuses(long long rows, int cols, int n, long long order_rows) {
     return rows <= 16 && rows * mx4_padded(cols) <= kMx4FusedElements &&
-           (order_rows <= 0 || product_costs(order_rows, n, mx4_padded(cols)).rows_form);
+           (order_rows <= 0 || rows_form(order_rows, n, mx4_padded(cols), true, true));
 }
 
 void launch_mx4_linear(hipStream_t st, Mx4Linear a, const Mx4Rows *x) {

@@ -1478,6 +1478,13 @@ int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *p, void *workspace, 
     return NNB_OK;
 }
 
+int nnb_debug_mx4_form(int64_t rows, int64_t cols, int64_t out_features, int y_type) {
+    size_t bytes;
+    if (int rc = nnb_mx4_linear_workspace_bytes(rows, cols, out_features, 0, &bytes)) return rc;
+    if (int rc = check_dtype(y_type, "y_type")) return rc;
+    return mx4_form(rows, (int)out_features, mx4_padded((int)cols), y_type == NNB_F32, out_features * dtype_bytes(y_type) % 16 == 0, 0);
+}
+
 int nnb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, size_t *bytes_out) {
     if (!bytes_out) return fail(NNB_ERR_ARG, "bytes_out is null");
     if (batch < 0 || batch > 0x7fffffffLL) return fail(NNB_ERR_ARG, "batch %lld out of range [0, 2^31)", (long long)batch);

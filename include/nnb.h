@@ -429,6 +429,9 @@ typedef struct nnb_mx4_linear_args {
 /* Bytes of workspace nnb_mx4_linear needs (0 is possible). */
 int nnb_mx4_linear_workspace_bytes(int64_t rows, int64_t cols, int64_t out_features, int x_quantized, size_t *bytes_out);
 int nnb_mx4_linear(void *stream, const nnb_mx4_linear_args *args, void *workspace, size_t workspace_bytes);
+/* Which kernel multiplies such a product into contiguous rows of y_type, for tests and measurements: 0 blocks of 16 to 64
+ * rows x 16 features, 1 and 2 tiles of 128 x 128, one or two of them per CU, 3 tiles of 256 x 256; or a negative status. */
+int nnb_debug_mx4_form(int64_t rows, int64_t cols, int64_t out_features, int y_type);
 
 /* Newton-Schulz orthogonalisation.  X = x / (|x|_F + eps), then `steps` times
  *     X <- a X + b (X X^T) X + c (X X^T)^2 X      with step i's (a, b, c) = coefficients[i],

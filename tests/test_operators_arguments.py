@@ -137,3 +137,27 @@ def test_matrices_in_one_blocks_lds_need_no_workspace_of_their_own():
     assert muon() == muon((0, 5), (7, 0)) == 0
     large = muon((200, 300))
     assert large > 1 << 20 and muon((64, 64), (200, 300), (192, 64)) == large and muon((65, 193), (200, 300)) > large
+
+
+ROWS, ONE_PER_CU, TWO_PER_CU, LARGE = range(4)
+
+
+# measured either side of where one form becomes faster than another (profiles/mx4_forms.txt)
+@pytest.mark.parametrize("rows,cols,out,y_type,form", [
+    (1, 11520, 1024, 0, ROWS), (512, 11520, 1024, 2, ROWS), (2048, 11520, 1024, 2, ONE_PER_CU), (4096, 11520, 1024, 0, ONE_PER_CU),
+    (8192, 11520, 1024, 2, TWO_PER_CU), (64, 8192, 8192, 2, ROWS), (256, 8192, 8192, 2, ONE_PER_CU), (1024, 8192, 8192, 2, TWO_PER_CU),
+    (2048, 8192, 8192, 2, LARGE), (8192, 8192, 8192, 2, LARGE), (17, 1024, 8192, 2, ROWS), (64, 1024, 8192, 0, ROWS),
+    (512, 1024, 8192, 2, ONE_PER_CU), (2048, 1024, 8192, 2, TWO_PER_CU), (64, 256, 2048, 2, ROWS), (512, 256, 2048, 2, ONE_PER_CU),
+    (8192, 256, 2048, 2, TWO_PER_CU), (2048, 4096, 4096, 2, TWO_PER_CU), (4096, 4096, 4096, 2, LARGE), (4096, 4096, 4096, 0, LARGE),
+    (512, 1024, 1024, 0, ROWS), (2048, 1024, 1024, 2, ONE_PER_CU), (8192, 256, 8192, 2, TWO_PER_CU), (1024, 16384, 300, 2, ROWS),
+    (8192, 16384, 300, 2, ONE_PER_CU), (86, 102, 489, 0, ROWS), (1957, 193, 213, 0, ROWS), (5084, 9483, 171, 0, ONE_PER_CU)])
+def test_mx4_linear_takes_the_form_that_measured_fastest(rows, cols, out, y_type, form):
+    from alphazero_amd import _lib
+    assert _lib.load().nnb_debug_mx4_form(rows, cols, out, y_type) == form
+
+
+def test_mx4_form_refuses_what_the_product_refuses():
+    from alphazero_amd import _lib
+    lib = _lib.load()
+    for args in ((-1, 64, 8, 0), (4, 0, 8, 0), (4, 64, 2 ** 27, 0), (4, 64, 8, 3)):
+        assert lib.nnb_debug_mx4_form(*args) == -1
