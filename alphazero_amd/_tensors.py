@@ -39,9 +39,12 @@ def ptr(t: torch.Tensor) -> C.c_void_p:
 
 
 def no_grad(what: str, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NnbError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
-    no_tangent(what, *tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NnbError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:
+        no_tangent(what, *tensors)
 
 
 def no_tangent(what: str, *tensors):

@@ -100,7 +100,8 @@ class MX4Tensor:
 
 def _rows_view(x: torch.Tensor) -> torch.Tensor:
     """x as [rows, cols] without a copy where its strides allow one view."""
-    x = resolved(x)
+    if x.is_neg():
+        x = resolved(x)
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
 
 
@@ -193,7 +194,7 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
             rows, x_ptr, x_codes, x_scales = v.shape[0], v.data_ptr(), None, None
             row_stride, col_stride = v.stride()
         w_codes, w_scales = weight._pointers()
-        b = resolved(bias).contiguous() if bias is not None else None
+        b = None if bias is None else resolved(bias).contiguous()
         y_type = dtype_code(out, "out")
         bias_type, b_ptr = (0, None) if b is None else (dtype_code(b, "bias"), b.data_ptr())
         args = Mx4LinearArgs(rows, cols, n, x_ptr, row_stride, col_stride, x_codes, x_scales, w_codes, w_scales, b_ptr,
