@@ -201,11 +201,12 @@ __device__ __forceinline__ void store_features(const Mx4Linear &a, long long r, 
 // before they multiply; all waves meet once per stage, when its last operands are in registers: from then on its place in
 // the ring is free for the stage RING further on, and the next one's operands are read while the last AHEAD k-steps
 // multiply.
-// What bounds it: 8192 x 8192 x 8192 takes 278 us after a quantisation (4.0 PFLOP/s), 329 in a row of its own and 212 there
-// with codes of zero: the power cap (without the loads, 68 KB a stage for 2048 clocks of products, 291; touching lines
-// ahead of them saved nothing).  4096 rows of
-// 11520 -> 1024 take 33.2 us (2.9 PFLOP/s) on 128 x 128 tiles: 4 of it to store, the rest the operands' way out of LDS, 96 KB a
-// stage for 512 clocks of products (29 without the loads; four waves with half the reads 38).
+// What bounds it: 8192 x 8192 x 8192 takes 292 us (profiles/operators_kernel_stats.csv; boxes differ by a tenth), at which
+// the power cap holds the clock: in a row of products alone, where one box took 329, codes of zero took 212, and 291 without
+// the loads (68 KB a stage for 2048 clocks of products; touching lines ahead of them saved nothing).  4096 rows of
+// 11520 -> 1024 take 33.3 us on 128 x 128 tiles: 4 of it to store, the rest some 1350 clocks for each of the 45 stages, in which
+// the products are 512 and the 96 KB of operands out of LDS 768 at 128 B a clock; what keeps these from overlapping is not
+// known (29 us without the loads; four waves with half the reads 38).
 
 template <typename T, int WX, int WW, int TX, int TW, int RING, int AHEAD>
 __global__ __launch_bounds__(WX *WW * 64, 1) void mx4_tile_kernel(Mx4Linear a) {

@@ -5,8 +5,9 @@ is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (or its negative) times that scale, to near
 ones to 6.  A block with an infinity or a NaN reads as NaN.  The matrix units multiply such numbers four times as fast
 as halves, and a weight takes 4.25 bits.
 
-    weight = mx4.quantize(layer.weight)                    # once
-    y = mx4.linear(x, weight, bias=layer.bias, relu=True)  # x is quantised on the way in, sums are float32
+    with torch.no_grad():
+        weight = mx4.quantize(layer.weight)                    # once
+        y = mx4.linear(x, weight, bias=layer.bias, relu=True)  # x is quantised on the way in, sums are float32
 
 The functions run on the tensors' device, on torch's current stream there; they wait for nothing and can be captured into
 a graph.  They have no derivatives and refuse tensors that ask for a backward pass or carry a forward-mode tangent.
