@@ -43,7 +43,7 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     hipcc = _hipcc()
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers.append(os.path.join(os.path.dirname(HERE), "include", "nnb.h"))
-    objs = []
+    objs, running = [], []                                 # compiled side by side: one source takes half of the time
     for src, extra in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(CSRC, src.replace(".hip", ".o"))
@@ -51,8 +51,14 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
             cmd = [hipcc, *COMMON, *extra, "-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)
-            subprocess.check_call(cmd)
+            running.append((cmd, o, subprocess.Popen(cmd)))
         objs.append(o)
+    failed = [(cmd, o, p.returncode) for cmd, o, p in running if p.wait() != 0]
+    for cmd, o, _ in failed:
+        if os.path.exists(o):                              # an older one would pass for its result
+            os.remove(o)
+    if failed:
+        raise subprocess.CalledProcessError(failed[0][2], failed[0][0])
     if force or _stale(LIB, objs):
         cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
         if verbose:
