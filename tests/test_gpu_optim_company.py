@@ -113,3 +113,37 @@ def test_large_batches(rows, cols, batch):
     assert ours.pow(2).mean().sqrt() <= 3 * plain.pow(2).mean().sqrt()
     # one matrix's error goes by its smallest singular values, by this bound of the worst (see test_gpu_optim.FAITHFUL)
     assert ours.max() <= 2 * 2.0 ** -20 * 4.7750 * 3.4445 ** 3
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 7])
+def test_step_counts_of_mixed_lists(steps, dtype):
+    """A segment of one step ends with the product that another one begins with: its Q is whole at once.  The bound is that of
+    test_gpu_optim (FAITHFUL), for the step's move from zero weights, and one rounding to the type."""
+    torch = _torch()
+    from alphazero_amd import optim
+    half_step = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8}[dtype]
+    xs = [_matrix("gradient", r, c, i + 3).to(getattr(torch, dtype))
+          for i, (r, c) in enumerate([(33, 70), (120, 250), (64, 400), (1, 300), (200, 300), (530, 600), (1, 1)])]
+    w, _ = optim.muon_update([torch.zeros_like(x) for x in xs], xs, [torch.zeros(x.shape, device="cuda") for x in xs], lr=1.0,
+                             momentum=0.0, nesterov=False, steps=steps, inplace=False)
+    for x, y in zip(xs, w):
+        want = -_formula(x.double(), steps) * math.sqrt(max(1.0, x.shape[0] / x.shape[1]))
+        assert (y.double() - want).norm() <= (2 * 2.0 ** -20 * 4.7750 * 3.4445 ** 3 + half_step) * want.norm(), tuple(x.shape)
+
+
+def test_zero_nan_and_infinity_beside_other_matrices():
+    torch = _torch()
+    shapes = [(40, 60), (100, 130), (1, 300), (2, 500), (150, 70), (600, 700)]
+    xs = [_matrix("normal", r, c, i + 1) for i, (r, c) in enumerate(shapes)]
+    want = _orthogonalized(xs)
+    for i in range(len(shapes)):
+        for value in (0.0, float("nan"), float("inf")):
+            changed = [x.clone() for x in xs]
+            if value == 0.0:
+                changed[i].zero_()
+            else:
+                changed[i][-1, shapes[i][1] // 2] = value
+            got = _orthogonalized(changed)
+            assert not got[i].any() if value == 0.0 else got[i].isnan().all(), (i, value)
+            assert all(torch.equal(a, b) for k, (a, b) in enumerate(zip(got, want)) if k != i), (i, value)
